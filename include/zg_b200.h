@@ -527,6 +527,74 @@ ZG_API int zg_attention_ex(const void* q, const void* k, const void* v, int64_t 
  * (examples/train_vit_cifar10.py:183) applied to a candidate's output. */
 ZG_API int zg_gelu(const void* x, void* y, int64_t n, int dtype, void* stream);
 
+/* ------------------------------------- long sequences and their cache -- */
+
+/* Rotary positions with one or several axes on queries and keys:
+ *   pair p of a head (columns a, b), of axis x_p and frequency f_p, turns by
+ *   t = positions[token, x_p] * f_p:
+ *     y_a = x_a cos t - x_b sin t,  y_b = x_a sin t + x_b cos t
+ * q [T, H, D] and k [T, K, D] with tokens ldq and ldk elements apart (views
+ * of a fused projection); q_out [T, H, D], k_out [T, K, D] contiguous.
+ * axes: HOST array of A rotated widths (even, their sum at most D <= 256);
+ * the columns behind them are copied.  f_p = base^(-i/n) for pair i of an
+ * axis of n pairs, or with `joint` base^(-i/N) for pair i of all N.  A pair
+ * is columns (i, i + N), or with `interleaved` (2i, 2i + 1).  positions
+ * [pos_rows, A] (pos_type 0: int32, 1: int64, 2: float32), token t at row
+ * t % pos_rows.  inverse != 0 turns by -t (the transpose).  Angles are
+ * formed and reduced in 64 bits.  No counterpart in the reference (its
+ * blocks, examples/train_vit_cifar10.py:137-191, add a position table). */
+ZG_API int zg_rotary(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* positions, int pos_type,
+                     int64_t T, int64_t pos_rows, int H, int K, int D, int A, const int32_t* axes, double base,
+                     int interleaved, int joint, int inverse, int dtype, void* q_out, void* k_out, void* stream);
+
+/* Causal softmax attention over sequences of any length:
+ *   o[z, i, h] = sum_j softmax_j(q[z, i, h] . k[z, j, h / (H/K)] / sqrt(D)) v[z, j, h / (H/K)]
+ * over j <= i with i - j < window (0: no window) or j < sinks, and
+ * j < lengths[z] (NULL: S).  q [Z, S, H, D], k, v [Z, S, K, D], K dividing H,
+ * D <= 256, positions ldq, ldk, ldv elements apart (sequences S times that);
+ * o [Z, S, H, D] contiguous.  Rows i >= lengths[z] are zeros, a length
+ * outside [0, S] gives NaN rows; keys and values that a row does not see
+ * do not reach it, whatever they hold.  bf16 with D <= 128 and a multiple of
+ * 8, 16-byte aligned pointers and pitches that are multiples of 8 run on the
+ * tensor cores, other calls in float32 on the FMA pipe.  Extends the
+ * softmax(einsum(q, k) / sqrt(D)) @ v of the reference's ViT block
+ * (examples/train_vit_cifar10.py:166-172). */
+ZG_API int zg_window_attention(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                               const int32_t* lengths, int64_t Z, int64_t S, int H, int K, int D, int window,
+                               int sinks, int dtype, void* o, void* stream);
+
+/* Writes new tokens into a paged key-value cache.  Pages [n_pages, page, K,
+ * D], keys and values apart; table [B, max_pages] names each sequence's pages
+ * in order.  Token s of sequence b, k[b, s] and v[b, s] (B*S rows ldk and ldv
+ * elements apart), goes to position lengths[b] + s for s < counts[b] (NULL:
+ * S).  new_lengths[b] = lengths[b] + counts[b]; or -1, with nothing written,
+ * where the length or count is negative, the count above S or the table's
+ * row too short, and -1 where a page is not one of the pool's (its tokens
+ * are not written).  Two tokens of one call must not go to one place.  At
+ * most 2^30 positions in a row of the table.  No counterpart in the reference. */
+ZG_API int zg_append_pages(void* k_pages, void* v_pages, int64_t n_pages, int page, int K, int D, const void* k,
+                           int64_t ldk, const void* v, int64_t ldv, int64_t B, int64_t S, const int32_t* table,
+                           int max_pages, const int32_t* lengths, const int32_t* counts, int dtype,
+                           int32_t* new_lengths, void* stream);
+
+/* Attention of each sequence's newest token (position lengths[b] - 1) over
+ * its paged cache:
+ *   o[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(D)) v_j
+ * over the last `window` positions (0: all) and the first `sinks`; key head
+ * h / (H/K).  q [B, H, D] with sequences ldq elements apart, o [B, H, D]
+ * contiguous, D <= 256.  A length of 0 gives zeros; a length that the table
+ * cannot hold, or a visible page that is not one of the pool's, gives NaN.
+ * bf16 pages with D a multiple of 8 are 16-byte aligned (and q 4-byte, ldq
+ * even).  At most 2^30 positions in a row of the table and in the pool.  The
+ * workspace (16-byte aligned) holds the splits' partial sums; 0 bytes where
+ * one split does. */
+ZG_API size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int D, int max_pages, int page, int window,
+                                                int sinks, int dtype);
+ZG_API int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,
+                              int page, const int32_t* table, int max_pages, const int32_t* lengths, int64_t B, int H,
+                              int K, int D, int window, int sinks, int dtype, void* o, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------- integer QAT linear -- */
 
 /* Integer linear with LUT activation for P candidates (no reference

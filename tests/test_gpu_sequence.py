@@ -1,0 +1,364 @@
+"""Rotary positions, windowed attention and the paged cache against plain
+float64 forms, at the sizes and masks where they can go wrong.  The bounds
+are derived in ``sequence_oracle``."""
+import math
+
+import pytest
+import torch
+
+import sequence_oracle as so
+import zerograd_b200 as zg
+from zerograd_b200 import _lib as L
+
+pytestmark = pytest.mark.gpu
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _rand(shape, dtype, g, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def _ok():
+    torch.cuda.synchronize()
+    assert L.load().zg_device_error(1) == 0
+
+
+# ------------------------------------------------------------------- rotary
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("joint,inverse", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("lead,S,H,K,D,axes", [
+    ((2,), 5, 3, 1, 64, (64,)),
+    ((), 1, 12, 4, 64, (64,)),
+    ((3, 2), 7, 4, 2, 128, (32, 48, 48)),
+    ((1,), 63, 6, 6, 72, (36, 36)),
+    ((2,), 9, 2, 2, 80, (16, 8)),      # columns behind the pairs stay
+    ((2,), 3, 2, 1, 10, (2, 6)),       # no 16-byte words
+    ((300,), 4, 1, 1, 256, (256,)),
+])
+def test_rotary(cuda, dtype, interleaved, joint, inverse, lead, S, H, K, D, axes):
+    g = torch.Generator().manual_seed(S * D + H)
+    x = _rand((*lead, S, H + 2 * K, D), dtype, g)
+    pos = torch.randint(0, 200000, (S, len(axes)), generator=g)
+    xc = x.to(cuda)
+    q, k = zg.rotary(xc[..., :H, :], xc[..., H:H + K, :], pos.to(cuda), axes, interleaved=interleaved, joint=joint,
+                     inverse=inverse)
+    want = so.rotary(x[..., :H, :], x[..., H:H + K, :], pos, axes, 10000.0, interleaved, joint, inverse)
+    for got, (w, size), name in ((q, want[0], "q"), (k, want[1], "k")):
+        assert got.dtype == dtype and got.is_contiguous()
+        so.assert_within(got, w, so.rotary_tolerance(w, size, dtype), name)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, torch.float32])
+def test_rotary_positions_per_sequence(cuda, kind):
+    g = torch.Generator().manual_seed(1)
+    q, k = _rand((3, 4, 5, 2, 32), F32, g), _rand((3, 4, 5, 1, 32), F32, g)
+    for shape in ((5, 2), (4, 5, 2), (3, 4, 5, 2)):
+        pos = torch.randint(-1000, 1 << 20, shape, generator=g).to(kind)
+        if kind == torch.float32:
+            pos = pos / 8
+        got = zg.rotary(q.to(cuda), k.to(cuda), pos.to(cuda), (20, 12), base=500.0)
+        for y, (w, size) in zip(got, so.rotary(q, k, pos, (20, 12), 500.0)):
+            so.assert_within(y, w, so.rotary_tolerance(w, size, F32), str(shape))
+
+
+def test_rotary_inverse_is_the_transpose(cuda):
+    """<R q, y> = <q, R' y>, and R' R = 1, within float32's roundings."""
+    g = torch.Generator().manual_seed(2)
+    q, k, y = (_rand((2, 6, 3, 48), F32, g).to(cuda) for _ in range(3))
+    pos = torch.randint(0, 5000, (6, 3), generator=g).to(cuda)
+    r, _ = zg.rotary(q, k, pos, (16, 16, 16), joint=True)
+    back, ry = zg.rotary(r, y, pos, (16, 16, 16), joint=True, inverse=True)
+    assert (back - q).abs().max() < 4 * 2.0 ** -21 * q.abs().max()
+    lhs, rhs = (r.double() * y.double()).sum(), (q.double() * ry.double()).sum()
+    assert abs(lhs - rhs) < 4 * 2.0 ** -21 * (q.double().norm() * y.double().norm())
+
+
+def test_rotary_of_nothing(cuda):
+    q = torch.empty(0, 5, 2, 32, device=cuda)
+    a, b = zg.rotary(q, q, torch.zeros(5, 1, dtype=torch.int64, device=cuda), (32,))
+    assert a.shape == b.shape == q.shape
+
+
+# --------------------------------------------------------- window attention
+
+WINDOW_CASES = [
+    # Z, S, H, K, D, window, sinks, ragged
+    (1, 1, 1, 1, 64, None, 0, False),
+    (2, 17, 4, 2, 64, None, 0, False),
+    (2, 128, 2, 2, 64, None, 0, False),
+    (1, 129, 2, 1, 128, 1, 0, False),      # each token sees itself alone
+    (1, 300, 3, 1, 128, 1, 4, False),
+    (2, 256, 4, 4, 64, 64, 4, False),
+    (2, 511, 2, 2, 64, 127, 0, True),
+    (1, 640, 6, 2, 128, 200, 130, True),   # sinks over more than one tile
+    (3, 333, 2, 1, 128, 100, 3, True),
+    (1, 777, 2, 2, 80, 200, 3, True),
+    (2, 400, 2, 1, 40, None, 0, True),
+    (1, 1100, 2, 1, 96, 257, 1, False),
+    (1, 900, 1, 1, 64, 899, 1, False),
+    (1, 900, 1, 1, 64, 5000, 9000, False),  # wider than the sequence
+    (70, 40, 5, 1, 32, 16, 2, True),
+    (2, 150, 2, 2, 20, 33, 2, True),        # no 16-byte rows: the FMA path in bf16 too
+    (2, 150, 4, 2, 256, 33, 2, True),
+    (1, 70, 1, 1, 3, None, 0, False),
+]
+
+
+def _lengths(Z, S):
+    return torch.tensor([(S, 0, 1, S // 2 + 1, max(S - 1, 0))[z % 5] for z in range(Z)], dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Z,S,H,K,D,window,sinks,ragged", WINDOW_CASES)
+def test_window_attention(cuda, dtype, Z, S, H, K, D, window, sinks, ragged):
+    g = torch.Generator().manual_seed(S * D + H)
+    x = _rand((Z, S, H + 2 * K, D), dtype, g)
+    q, k, v = x[:, :, :H], x[:, :, H:H + K], x[:, :, H + K:]
+    lengths = _lengths(Z, S) if ragged else None
+    xc = x.to(cuda)
+    o = zg.window_attention(xc[:, :, :H], xc[:, :, H:H + K], xc[:, :, H + K:], window, sinks,
+                            None if lengths is None else lengths.to(cuda))
+    _ok()
+    assert o.dtype == dtype and o.is_contiguous()
+    want, mag = so.window_attention(q, k, v, window, sinks, lengths)
+    so.assert_within(o, want, so.attention_tolerance(q, k, want, mag, dtype, S))
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 64), (BF, 20)])
+def test_window_attention_masked_places_hold_anything(cuda, dtype, D):
+    """Infinities, NaN and the type's lowest value behind a sequence and in
+    positions that a row does not see leave it as it is."""
+    Z, S, H, K, window, sinks = 2, 300, 2, 1, 50, 2
+    g = torch.Generator().manual_seed(5)
+    q, k, v = _rand((Z, S, H, D), dtype, g), _rand((Z, S, K, D), dtype, g), _rand((Z, S, K, D), dtype, g)
+    lengths = torch.tensor([190, 300], dtype=torch.int32)
+    want, mag = so.window_attention(q, k, v, window, sinks, lengths)
+    low = torch.finfo(dtype).min
+    for at, t in ((200, q), (230, k), (260, k)):
+        t[0, at:at + 20] = math.nan if at != 260 else low
+    k[0, 191], v[0, 191], v[0, 192], v[0, 255] = math.inf, math.nan, -math.inf, low
+    # position 100 of sequence 1: seen by rows 100 .. 149 alone
+    v[1, 100, 0, 3], k[1, 101] = math.nan, 0
+    want1, mag1 = so.window_attention(q[1:], k[1:], v[1:], window, sinks)
+    want[1:], mag[1:] = want1, mag1
+    o = zg.window_attention(*(t.to(cuda) for t in (q, k, v)), window, sinks, lengths.to(cuda))
+    _ok()
+    assert torch.isnan(o[1, 100:150, :, 3]).all() and int(torch.isnan(o).sum()) == 50 * H
+    tol = so.attention_tolerance(q, torch.where(k.double().abs() < 1e3, k, 0), want, mag, dtype, S)
+    so.assert_within(o, want, tol)
+
+
+def test_window_attention_bad_lengths(cuda):
+    q = torch.ones(3, 5, 2, 64, device=cuda, dtype=BF)
+    o = zg.window_attention(q, q, q, lengths=torch.tensor([-1, 6, 3], device=cuda))
+    assert torch.isnan(o[:2]).all() and (o[2, :3] == 1).all() and (o[2, 3:] == 0).all()
+
+
+def test_window_attention_large_scores(cuda):
+    """Scores to several hundred, the largest coming late: the running maximum moves."""
+    g = torch.Generator().manual_seed(6)
+    S, D = 600, 64
+    q, k, v = (_rand((1, S, 2, D), BF, g, 3) for _ in range(3))
+    k *= torch.linspace(0.1, 6, S)[None, :, None, None].to(BF)
+    o = zg.window_attention(*(t.to(cuda) for t in (q, k, v)), 400, 2)
+    want, mag = so.window_attention(q, k, v, 400, 2)
+    so.assert_within(o, want, so.attention_tolerance(q, k, want, mag, BF, S))
+
+
+# -------------------------------------------------------------- paged cache
+
+
+def _pool(lengths, page, K, D, dtype, g, spare=3):
+    need = [-(-n // page) for n in lengths]
+    n = sum(need) + spare
+    kp, vp = _rand((n, page, K, D), dtype, g), _rand((n, page, K, D), dtype, g)
+    order = torch.randperm(n, generator=g).to(torch.int32)
+    table = torch.full((len(lengths), max(need + [1])), -7, dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(need):
+        table[b, :m] = order[at:at + m]
+        at += m
+    return kp, vp, table
+
+
+PAGED_CASES = [
+    # lengths, H, K, D, page, window, sinks
+    ([1], 1, 1, 64, 16, None, 0),
+    ([0, 1, 15, 16, 17], 4, 2, 64, 16, None, 0),
+    ([700], 12, 4, 128, 16, None, 0),
+    ([3000, 10, 2047], 4, 1, 128, 64, None, 0),
+    ([3000, 10, 2047], 4, 4, 64, 24, 100, 4),
+    ([5000, 1], 2, 1, 128, 1, 1, 0),
+    ([1500, 64, 200], 40, 2, 64, 8, None, 0),     # 20 heads of a key head: two row tiles
+    ([900, 333], 16, 1, 80, 16, 512, 1),
+    ([900, 333], 3, 3, 256, 128, None, 0),
+    ([400, 333, 77], 5, 1, 20, 16, 300, 2),       # no 16-byte rows in bf16
+    ([60, 3], 2, 2, 7, 5, None, 0),
+    ([40000], 8, 8, 32, 256, None, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths,H,K,D,page,window,sinks", PAGED_CASES)
+def test_paged_attention(cuda, dtype, lengths, H, K, D, page, window, sinks):
+    g = torch.Generator().manual_seed(sum(lengths) + D)
+    kp, vp, table = _pool(lengths, page, K, D, dtype, g)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    q = _rand((len(lengths), H, D), dtype, g)
+    want, mag = so.paged_attention(q, kp, vp, table, n, window, sinks)
+    tol = so.attention_tolerance(q, kp, want, mag, dtype, max(lengths))
+    # what lies behind a sequence, in its last page and in pages of nobody, is not read
+    seen = torch.zeros(kp.shape[:2], dtype=torch.bool)
+    for b, m in enumerate(lengths):
+        j = torch.arange(m)
+        if window is not None:
+            j = j[(j >= m - window) | (j < sinks)]
+        seen[table[b].long()[j // page], j % page] = True
+    kp[~seen], vp[~seen] = math.nan, math.inf
+    o = zg.paged_attention(q.to(cuda), kp.to(cuda), vp.to(cuda), table.to(cuda), n.to(cuda), window, sinks)
+    torch.cuda.synchronize()
+    assert o.dtype == dtype
+    so.assert_within(o, want, tol)
+    again = zg.paged_attention(q.to(cuda), kp.to(cuda), vp.to(cuda), table.to(cuda).long(), n.to(cuda).long(), window,
+                               sinks)
+    assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_paged_attention_bad_pages_and_lengths(cuda, dtype):
+    """A page outside the pool or a length outside the table gives that sequence NaN."""
+    g = torch.Generator().manual_seed(3)
+    lengths = [900, 900, 900, 40, 900, 900]
+    kp, vp, table = _pool(lengths, 16, 2, 64, dtype, g)
+    q = _rand((6, 4, 64), dtype, g)
+    table[0, 30], table[1, 2] = -1, kp.shape[0]
+    n = torch.tensor(lengths, dtype=torch.int32)
+    n[4], n[5] = -1, table.shape[1] * 16 + 1
+    o = zg.paged_attention(q.to(cuda), kp.to(cuda), vp.to(cuda), table.to(cuda), n.to(cuda))
+    assert torch.isnan(o[[0, 1, 4, 5]]).all()
+    want, mag = so.paged_attention(q[2:4], kp, vp, table[2:4], n[2:4])
+    so.assert_within(o[2:4], want, so.attention_tolerance(q, kp, want, mag, dtype, 900))
+    # the bad entries do not matter where the token does not see them
+    o = zg.paged_attention(q[:2].to(cuda), kp.to(cuda), vp.to(cuda), table[:2].to(cuda), n[:2].to(cuda), 100, 3)
+    assert torch.isfinite(o).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("S,K,D,page", [(1, 4, 128, 16), (37, 2, 64, 16), (5, 1, 3, 4), (130, 2, 20, 1), (9, 12, 64, 64)])
+def test_append_pages(cuda, dtype, S, K, D, page):
+    g = torch.Generator().manual_seed(S + D)
+    had = [0, 3, page, 2 * page - 1, 50]
+    counts = [S, S // 2, 0, S, 1]
+    kp, vp, table = _pool([h + S for h in had], page, K, D, dtype, g)
+    x = _rand((5, S, 2 * K, D), dtype, g)
+    k, v = x[:, :, :K], x[:, :, K:]
+    wk, wv = kp.clone(), vp.clone()
+    for b in range(5):
+        for s in range(counts[b]):
+            at = had[b] + s
+            wk[table[b, at // page], at % page], wv[table[b, at // page], at % page] = k[b, s], v[b, s]
+    ck, cv, xc = kp.to(cuda), vp.to(cuda), x.to(cuda)
+    n = torch.tensor(had, device=cuda)
+    new = zg.append_pages(ck, cv, xc[:, :, :K], xc[:, :, K:], table.to(cuda), n, torch.tensor(counts, device=cuda))
+    assert new.tolist() == [h + c for h, c in zip(had, counts)] and n.tolist() == had
+    assert torch.equal(ck.cpu(), wk) and torch.equal(cv.cpu(), wv)
+
+
+def test_append_pages_that_do_not_fit(cuda):
+    """Nothing is written past a table's row, for bad lengths and counts, or to a page outside the pool."""
+    page, K, D, S = 4, 1, 64, 6
+    kp = torch.zeros(8, page, K, D, device=cuda, dtype=BF)
+    vp = torch.zeros_like(kp)
+    table = torch.tensor([[0, 1], [2, 3], [4, 5], [6, 7], [-1, 7], [6, 8]], dtype=torch.int32, device=cuda)
+    x = torch.ones(6, S, K, D, device=cuda, dtype=BF)
+    had = torch.tensor([0, 3, -1, 0, 2, 2], device=cuda)
+    counts = torch.tensor([6, 6, 1, 7, 3, 3], device=cuda)
+    new = zg.append_pages(kp, vp, x, x, table, had, counts)
+    assert new.tolist() == [6, -1, -1, -1, -1, -1]
+    filled = kp.float().sum((2, 3)) / D
+    want = torch.zeros(8, page, device=cuda)
+    want[0], want[1, :2] = 1, 1
+    want[7, 0] = 1      # the token of sequence 4 whose page is one of the pool's
+    want[6, 2:] = 1     # those of sequence 5
+    assert torch.equal(filled, want) and torch.equal(kp, vp)
+    o = zg.paged_attention(torch.ones(6, 2, D, device=cuda, dtype=BF), kp, vp, table, new)
+    assert (o[0] == 1).all() and torch.isnan(o[1:]).all()
+
+
+# ------------------------------------------------------- a run of them together
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (F32, 48)])
+def test_prompt_and_tokens(cuda, dtype, D):
+    """A padded batch's prompt (rotary, windowed attention, append) and then
+    token after token (rotary, append, paged attention) agree with the windowed
+    attention of the whole sequences."""
+    B, S, T, H, K, page, window, sinks = 3, 50, 30, 4, 2, 16, 24, 3
+    g = torch.Generator().manual_seed(8)
+    prompt = torch.tensor([50, 17, 1], dtype=torch.int32)
+    x = _rand((B, S + T, H + 2 * K, D), dtype, g).to(cuda)  # a fused projection of the whole sequences
+    kp, vp, table = (t.to(cuda) for t in _pool([S + T] * B, page, K, D, dtype, g))
+    lengths = prompt.to(cuda)
+    pos = torch.arange(S + T, device=cuda)[:, None]
+    qr, kr = zg.rotary(x[:, :, :H], x[:, :, H:H + K], pos, (D,))
+    v = x[:, :, H + K:]
+    whole = zg.window_attention(qr, kr, v, window, sinks)
+    o = zg.window_attention(qr[:, :S].contiguous(), kr[:, :S].contiguous(), v[:, :S], window, sinks, lengths)
+    n = zg.append_pages(kp, vp, kr[:, :S], v[:, :S], table, torch.zeros_like(lengths), lengths)
+    assert torch.equal(n, lengths)
+    tol = 2.0 ** -6 if dtype == BF else 2.0 ** -18  # two results of values below 4, each off by its own bound
+    for b in range(B):
+        assert (o[b, :prompt[b]] - whole[b, :prompt[b]]).abs().max() <= 4 * tol
+    rows = torch.arange(B, device=cuda)
+    for _ in range(T):
+        tok = x[rows, n.long()]
+        q1, k1 = zg.rotary(tok[:, None, :H], tok[:, None, H:H + K], n[:, None, None], (D,))
+        n = zg.append_pages(kp, vp, k1, tok[:, None, H + K:], table, n)
+        o1 = zg.paged_attention(q1[:, 0], kp, vp, table, n, window, sinks)
+        want = whole[rows, n.long() - 1]
+        assert (o1 - want).abs().max() <= 4 * tol
+    assert n.tolist() == [80, 47, 31]
+
+
+def test_under_vmap(cuda):
+    """Each op of a candidate's forward is one launch for the population, with
+    the bits of the calls candidate by candidate."""
+    P, B, S, H, K, D, page = 3, 2, 20, 4, 2, 64, 8
+    g = torch.Generator().manual_seed(9)
+    x = _rand((P, B, S, H + 2 * K, D), BF, g).to(cuda)
+    kp, vp, table = (t.to(cuda) for t in _pool([S] * (P * B), page, K, D, BF, g))
+    table = table.reshape(P, B, -1)
+    pos = torch.arange(S, device=cuda)[:, None]
+    lengths = torch.tensor([S, 7], dtype=torch.int32, device=cuda)
+
+    def candidate(xx, tt):
+        q, k = zg.rotary(xx[:, :, :H], xx[:, :, H:H + K], pos, (32,))
+        v = xx[:, :, H + K:]
+        o = zg.window_attention(q, k, v, 9, 1, lengths)
+        n = zg.append_pages(kp, vp, k, v, tt, torch.zeros_like(lengths), lengths)
+        return o, zg.paged_attention(q[:, 0], kp, vp, tt, n, 9, 1), n
+
+    kp0, vp0 = kp.clone(), vp.clone()
+    L.profile_begin()
+    got = torch.func.vmap(candidate)(x, table)
+    prof = L.profile_end()
+    assert len(prof) == 4 and all(c == 1 for c, _ in prof.values()), prof
+    k1, v1 = kp.clone(), vp.clone()
+    kp.copy_(kp0)
+    vp.copy_(vp0)
+    want = [candidate(x[p], table[p]) for p in range(P)]
+    for i in range(3):
+        assert torch.equal(got[i], torch.stack([w[i] for w in want]))
+    assert torch.equal(kp, k1) and torch.equal(vp, v1)
+    # per-candidate positions, the same for each of a candidate's sequences
+    shift = torch.arange(P, device=cuda)[:, None, None] * 100 + pos
+    a, _ = torch.func.vmap(lambda xx, pp: zg.rotary(xx[:, :, :H], xx[:, :, H:H + K], pp, (32,)))(x, shift)
+    b = torch.stack([zg.rotary(x[p, :, :, :H], x[p, :, :, H:H + K], shift[p], (32,))[0] for p in range(P)])
+    assert torch.equal(a, b)
+    with pytest.raises(NotImplementedError):
+        torch.func.vmap(lambda c: zg.paged_attention(x[0, :, 0, :H], c, c, table[0], lengths))(
+            torch.stack([kp, kp]))

@@ -18,18 +18,20 @@ from ._block import attention, layer_norm, rms_norm
 from ._ops import gelu, quantize_int8_columns
 from ._graph import CapturedGeneration
 from ._optimizer import StepMetrics, ZeroGrad, ZeroGradState
+from ._sequence import append_pages, paged_attention, rotary, window_attention
 from ._replay import replay, replay_entry
 from ._transforms import adamw, apply_updates, sgd
 from . import checkpoint, random
 from .checkpoint import load_checkpoint, save_checkpoint
 
 __all__ = [
-    "attention", "load_checkpoint", "save_checkpoint", "checkpoint",
+    "append_pages", "attention", "load_checkpoint", "save_checkpoint", "checkpoint",
     "CandidateContext", "CalibrationResult", "CapturedGeneration", "DeviceShard", "DistributedZeroGrad", "ExchangedReplay",
     "Manifest", "ManifestEntry",
     "ParameterLayout", "ParameterPath", "ParameterTree", "ShardResult", "StepMetrics", "ZeroGrad",
     "ZeroGradState", "adamw", "allgather_losses", "apply_updates", "candidate_key", "compute_partition_sizes",
     "gelu", "quantize_int8_columns", "group_key", "layer_norm", "matrix_factors", "perturbed_linear", "perturbed_table_lookup", "perturbed_tied_logits",
-    "perturbed_vector", "random", "replay", "replay_entry", "rms_norm", "scaled_factor", "sgd", "shape_centered_loss",
+    "perturbed_vector", "paged_attention", "random", "replay", "replay_entry", "rms_norm", "rotary", "scaled_factor", "sgd", "shape_centered_loss",
     "step_key", "table_factors", "validate_losses", "vector_noise",
+    "window_attention",
 ]

@@ -98,6 +98,15 @@ SIGNATURES = {
     "zg_layer_norm": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i64, _i32, _f32, _i32, _vp, _vp]),
     "zg_rms_norm": (_i32, [_vp, _i32, _vp, _i32, _i32, _i64, _i32, _f32, _i32, _vp, _vp]),
     "zg_attention": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "zg_rotary": (_i32, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _f64, _i32, _i32,
+                         _i32, _i32, _vp, _vp, _vp]),
+    "zg_window_attention": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
+                                   _i32, _vp, _vp]),
+    "zg_append_pages": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _vp,
+                               _vp, _i32, _vp, _vp]),
+    "zg_paged_attention_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "zg_paged_attention": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32,
+                                  _i32, _i32, _vp, _vp, _sz, _vp]),
     "zg_int8_lut_linear_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "zg_int8_lut_linear": (_i32, [_vp, _i32, _vp, _vp, _f32, _f32, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                                   _i32, _f32, _vp, _vp, _vp, _sz, _vp]),

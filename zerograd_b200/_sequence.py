@@ -1,0 +1,389 @@
+"""Attention over long sequences and its key-value cache, population-batched.
+
+The reference writes a candidate's attention as user code over whole, short
+sequences (``examples/train_vit_cifar10.py:166-172``).  These ops take it to
+long ones, and to a fitness that is taken from generated answers:
+
+* :func:`rotary`: rotary positions with one or several axes (time, height,
+  width) on queries and keys, ``zg_rotary``;
+* :func:`window_attention`: causal attention of any length, grouped key
+  heads, a sliding window with a few first tokens that stay visible, padded
+  batches, ``zg_window_attention``;
+* :func:`append_pages`: writes new tokens into a paged key-value cache,
+  ``zg_append_pages``;
+* :func:`paged_attention`: the attention of one new token over that cache,
+  with the same window, ``zg_paged_attention``.
+
+Like the ops of ``_block.py`` each is one population launch under
+``torch.func.vmap`` over candidates, and evaluates forward only (evolution
+strategies take no gradients; :func:`rotary` with ``inverse=True`` is its own
+transpose).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib as L
+from ._block import _as, _row_pitch
+from ._ops import _NS, _movedim0
+
+_INT_MAX = 2 ** 31 - 1
+_POSITION_CODES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_no_transform = torch._C._functorch.peek_interpreter_stack
+
+
+def _plain_call(*ts) -> bool:
+    """True when a call needs none of what the dispatcher adds (vmap, an
+    autograd error, a tracing mode): the op is then launched without it,
+    which a single token's call notices (about 20 us of host time)."""
+    if _no_transform() is not None or torch._C._len_torch_dispatch_stack() or torch.compiler.is_compiling():
+        return False
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if t is not None and (type(t) is not torch.Tensor or (grad and t.requires_grad)):
+            return False
+    return True
+
+
+def _call(dev: torch.device, name: str, *args) -> None:
+    """The entry point on `dev`'s current stream (the last argument), with
+    `dev` current while it is called."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        L.call(name, *args, L.stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            L.call(name, *args, L.stream_ptr(dev))
+
+
+def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
+    """Whole numbers as contiguous int32; wider ones that int32 cannot hold
+    become -1 or the largest, which the kernels refuse as they would the
+    number itself."""
+    if t.dtype == torch.int32:
+        return t.contiguous()
+    if t.dtype != torch.int64:
+        raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
+    return t.clamp(-1, _INT_MAX).to(torch.int32).contiguous()
+
+
+def _pitched(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`t` [..., S, H, D] with its row pitch, copied if its rows have none."""
+    ld = _row_pitch(t)
+    if ld is None:
+        t = t.contiguous()
+        ld = int(t.shape[-2]) * int(t.shape[-1])
+    return t, ld
+
+
+def _span(window: int | None, sinks: int) -> tuple[int, int]:
+    """Window and sinks as the kernels take them (0: no window)."""
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1 (or None for no window), got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    return 0 if window is None else min(int(window), _INT_MAX), min(int(sinks), _INT_MAX)
+
+
+# ------------------------------------------------------------------- rotary
+
+
+def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: tuple, base: float,
+                  interleaved: bool, joint: bool, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """q [..., S, H, D] and k [..., S, K, D] turned by `positions`
+    [pos.., S, A], whose leading axes are the last ones of q's (none: shared
+    by all); outputs contiguous."""
+    dev = L.require_cuda(q, k, positions)
+    if q.ndim < 3 or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise ValueError("q and k must be [..., S, H, D] and [..., S, K, D] with the same leading axes and D")
+    tokens = tuple(q.shape[:-2])
+    if (positions.ndim < 2 or positions.shape[-1] != len(axes) or positions.ndim - 1 > len(tokens)
+            or tuple(positions.shape[:-1]) != tokens[len(tokens) - (positions.ndim - 1):]):
+        raise ValueError(f"positions of shape {tuple(positions.shape)} do not give {len(axes)} axes for the tokens "
+                         f"{tokens}")
+    if positions.dtype not in _POSITION_CODES:
+        raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
+    dt = q.dtype
+    code = L.dtype_code(dt)
+    H, D = int(q.shape[-2]), int(q.shape[-1])
+    K = int(k.shape[-2])
+    (q, ldq), (k, ldk) = _pitched(q), _pitched(_as(k, dt))
+    positions = positions.contiguous()
+    qo = torch.empty(q.shape, dtype=dt, device=dev)
+    ko = torch.empty(k.shape, dtype=dt, device=dev)
+    widths = (ctypes.c_int32 * len(axes))(*axes)
+    _call(dev, "zg_rotary", L.ptr(q), ldq, L.ptr(k), ldk, L.ptr(positions), _POSITION_CODES[positions.dtype],
+          math.prod(tokens), math.prod(positions.shape[:-1]), H, K, D, len(axes), widths, base, int(interleaved),
+          int(joint), int(inverse), code, L.ptr(qo), L.ptr(ko))
+    return qo, ko
+
+
+@torch.library.custom_op(f"{_NS}::rotary", mutates_args=())
+def _rotary_op(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: list[int], base: float,
+               interleaved: bool, joint: bool, inverse: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    return launch_rotary(q, k, positions, axes, base, interleaved, joint, inverse)
+
+
+@torch.library.register_vmap(f"{_NS}::rotary")
+def _rotary_vmap(info, in_dims, q, k, positions, axes, base, interleaved, joint, inverse):
+    qd, kd, pd = in_dims[:3]
+    q, k, positions = _movedim0(q, qd), _movedim0(k, kd), _movedim0(positions, pd)
+    P = info.batch_size
+    q = q if qd is not None else q.expand(P, *q.shape)
+    k = k if kd is not None else k.expand(P, *k.shape)
+    if pd is not None and positions.ndim < q.ndim - 1:
+        # per candidate, shared by the axes between the candidates and the sequence
+        lead = q.shape[1:q.ndim - positions.ndim]
+        positions = positions.reshape(P, *(1,) * len(lead), *positions.shape[1:]).expand(
+            P, *lead, *positions.shape[1:])
+    return launch_rotary(q, k, positions, axes, base, interleaved, joint, inverse), (0, 0)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes, base: float = 10000.0,
+           interleaved: bool = False, joint: bool = False,
+           inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """Queries [..., S, H, D] and keys [..., S, K, D] with rotary positions,
+    in one launch; both are returned, in their own type.
+
+    ``axes`` gives the rotated columns of each axis, all even: ``(64,)`` for
+    text, ``(16, 24, 24)`` for time, height and width.  Their sum may be less
+    than D (at most 256): the columns behind stay as they are.  ``positions``
+    [S, A], or [..., S, A] with the leading axes of q (or the last of them),
+    whole numbers or float32.  Pair i of an axis of n pairs turns by
+    ``position * base ** (-i / n)``; with ``joint`` the pairs of all axes share
+    one spectrum, pair i of all N by ``base ** (-i / N)``.  A pair is columns
+    (i, i + N) of the head, or with ``interleaved`` (2 i, 2 i + 1).
+
+    Angles are formed and reduced in 64 bits, so far positions keep their
+    accuracy.  ``inverse`` turns back: the transpose, by which a gradient
+    goes through.  q and k may be views of one fused projection; outputs are
+    contiguous.  D of q and k, and their leading axes, are the same."""
+    axes = [int(a) for a in axes]
+    args = (q, k, positions, axes, float(base), bool(interleaved), bool(joint), bool(inverse))
+    return launch_rotary(*args) if _plain_call(q, k, positions) else _rotary_op(*args)
+
+
+# --------------------------------------------------------- window attention
+
+
+def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor | None,
+                            window: int, sinks: int) -> torch.Tensor:
+    """q [..., S, H, D], k and v [..., S, K, D], lengths [...] or None;
+    window 0: none."""
+    dev = L.require_cuda(q, k, v, lengths)
+    if q.ndim < 3 or k.shape != v.shape or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] \
+            or q.shape[-1] != k.shape[-1]:
+        raise ValueError("q must be [..., S, H, D], k and v [..., S, K, D] with the same leading axes and D")
+    dt = q.dtype
+    code = L.dtype_code(dt)
+    S, H, D = (int(d) for d in q.shape[-3:])
+    K = int(k.shape[-2])
+    if K < 1 or H % K:
+        raise ValueError(f"{H} query heads are not a multiple of {K} key heads")
+    Z = math.prod(q.shape[:-3])
+    if lengths is not None:
+        if tuple(lengths.shape) != tuple(q.shape[:-3]):
+            raise ValueError(f"lengths of shape {tuple(lengths.shape)} do not match the sequences "
+                             f"{tuple(q.shape[:-3])}")
+        lengths = _int32(lengths, "lengths")
+    (q, ldq), (k, ldk), (v, ldv) = _pitched(q), _pitched(_as(k, dt)), _pitched(_as(v, dt))
+    o = torch.empty(q.shape, dtype=dt, device=dev)
+    _call(dev, "zg_window_attention", L.ptr(q), ldq, L.ptr(k), ldk, L.ptr(v), ldv, L.ptr(lengths), Z, S, H, K, D,
+          window, sinks, code, L.ptr(o))
+    return o
+
+
+@torch.library.custom_op(f"{_NS}::window_attention", mutates_args=())
+def _window_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor | None, window: int,
+               sinks: int) -> torch.Tensor:
+    return launch_window_attention(q, k, v, lengths, window, sinks)
+
+
+@torch.library.register_vmap(f"{_NS}::window_attention")
+def _window_vmap(info, in_dims, q, k, v, lengths, window, sinks):
+    ts = [_movedim0(t, d) if t is not None else None for t, d in zip((q, k, v, lengths), in_dims)]
+    ts = [t if t is None or d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, in_dims)]
+    return launch_window_attention(*ts, window, sinks), 0
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int | None = None, sinks: int = 0,
+                     lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal softmax(q kᵀ / sqrt(D)) v per head over sequences of any length.
+
+    q [..., S, H, D], k and v [..., S, K, D]; K divides H and query head h
+    reads key head h // (H // K).  Position i sees position j <= i when
+    i - j < ``window`` (None: all of them) or j < ``sinks``.  ``lengths``
+    [...] (int32 or int64): the tokens of each sequence of a padded batch;
+    rows behind a sequence's length are zeros, whatever their inputs hold,
+    and a length outside [0, S] gives NaN rows.  D is at most 256; float32 or
+    bf16.
+
+    bf16 with D up to 128, a multiple of 8, runs on the tensor cores (scores
+    and sums in float32, weights rounded to bf16), other shapes and float32
+    on the FMA pipe.  q, k and v may be views of one fused projection; the
+    output is contiguous."""
+    w, s = _span(window, sinks)
+    args = (q, k, v, lengths, w, s)
+    return launch_window_attention(*args) if _plain_call(q, k, v, lengths) else _window_op(*args)
+
+
+# -------------------------------------------------------------- paged cache
+
+
+def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int]:
+    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("key and value pages must share one [pages, page size, K, D] shape and type")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("key and value pages must be contiguous")
+    L.dtype_code(k_pages.dtype)
+    N, page, K, D = (int(d) for d in k_pages.shape)
+    if page < 1 or K < 1 or D < 1:
+        raise ValueError(f"pages of shape {tuple(k_pages.shape)} hold nothing")
+    return N, page, K, D
+
+
+def _table(page_table: torch.Tensor, lengths: torch.Tensor, lead: tuple) -> tuple[torch.Tensor, torch.Tensor]:
+    if page_table.ndim < 1 or tuple(page_table.shape[:-1]) != lead or tuple(lengths.shape) != lead:
+        raise ValueError(f"a page table of shape {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} do not "
+                         f"match the sequences {lead}")
+    return _int32(page_table, "the page table"), _int32(lengths, "lengths")
+
+
+def launch_append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        page_table: torch.Tensor, lengths: torch.Tensor,
+                        counts: torch.Tensor | None) -> torch.Tensor:
+    """k and v [..., S, K, D] into the pages of the sequences [...]."""
+    dev = L.require_cuda(k_pages, v_pages, k, v, page_table, lengths, counts)
+    N, page, K, D = _pool(k_pages, v_pages)
+    if k.ndim < 3 or k.shape != v.shape or tuple(k.shape[-2:]) != (K, D):
+        raise ValueError(f"new keys and values must be [..., S, {K}, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
+        raise TypeError(f"new keys and values must have the pages' type {k_pages.dtype}")
+    lead = tuple(k.shape[:-3])
+    table, had = _table(page_table, lengths, lead)
+    if counts is not None:
+        if tuple(counts.shape) != lead:
+            raise ValueError(f"counts of shape {tuple(counts.shape)} do not match the sequences {lead}")
+        counts = _int32(counts, "counts")
+    (k, ldk), (v, ldv) = _pitched(k), _pitched(v)
+    new = torch.empty(lead, dtype=torch.int32, device=dev)
+    _call(dev, "zg_append_pages", L.ptr(k_pages), L.ptr(v_pages), N, page, K, D, L.ptr(k), ldk, L.ptr(v), ldv,
+          math.prod(lead), int(k.shape[-3]), L.ptr(table), int(table.shape[-1]), L.ptr(had), L.ptr(counts),
+          L.dtype_code(k_pages.dtype), L.ptr(new))
+    return new
+
+
+@torch.library.custom_op(f"{_NS}::append_pages", mutates_args=("k_pages", "v_pages"))
+def _append_op(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+               page_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor | None) -> torch.Tensor:
+    return launch_append_pages(k_pages, v_pages, k, v, page_table, lengths, counts)
+
+
+@torch.library.register_vmap(f"{_NS}::append_pages")
+def _append_vmap(info, in_dims, k_pages, v_pages, k, v, page_table, lengths, counts):
+    if in_dims[0] is not None or in_dims[1] is not None:
+        raise NotImplementedError("pages batched over candidates are not supported: one pool holds every candidate's")
+    if in_dims[4] is None:
+        raise NotImplementedError("a page table shared by the candidates would let them write the same pages")
+    ts = [_movedim0(t, d) if t is not None else None for t, d in zip((k, v, page_table, lengths, counts), in_dims[2:])]
+    ts = [t if t is None or d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, in_dims[2:])]
+    return launch_append_pages(k_pages, v_pages, *ts), 0
+
+
+def append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 page_table: torch.Tensor, lengths: torch.Tensor,
+                 counts: torch.Tensor | None = None) -> torch.Tensor:
+    """Writes new tokens into a paged key-value cache, in place, and returns
+    the sequences' new lengths (int32, ``lengths`` itself is left as it is).
+
+    ``k_pages`` and ``v_pages`` [pages, page size, K, D] are contiguous, of
+    any page size.  ``page_table`` [..., M] (int32 or int64) names the pages
+    of each sequence in order; entries behind a sequence's last page are not
+    read and may hold anything.  ``k`` and ``v`` [..., S, K, D] are the new
+    tokens, in the pages' type (views of a fused projection are fine); token
+    s goes to position ``lengths`` + s.  ``counts`` [...]: how many of the S
+    tokens each sequence of a padded batch has; the others are not written.
+
+    A sequence whose length or count is negative, whose count is above S or
+    whose tokens do not fit its row of the table is not written; a token
+    whose page is not one of the pool's is not written.  Such a sequence's new
+    length is -1, for which :func:`paged_attention` gives NaN.  Two tokens of
+    one call must not go to the same place (a page that two sequences share
+    is for reading): which of them stays is not defined.
+
+    Under vmap over candidates the pool is shared and each candidate has its
+    own table."""
+    args = (k_pages, v_pages, k, v, page_table, lengths, counts)
+    if not _plain_call(*args):
+        return _append_op(*args)
+    out = launch_append_pages(*args)
+    torch.autograd.graph.increment_version((k_pages, v_pages))
+    return out
+
+
+def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                           lengths: torch.Tensor, window: int, sinks: int) -> torch.Tensor:
+    """q [..., H, D] over the pages of the sequences [...]; window 0: none."""
+    dev = L.require_cuda(q, k_pages, v_pages, page_table, lengths)
+    N, page, K, D = _pool(k_pages, v_pages)
+    if q.ndim < 2 or int(q.shape[-1]) != D or int(q.shape[-2]) < 1 or int(q.shape[-2]) % K:
+        raise ValueError(f"q of shape {tuple(q.shape)} is not [..., H, {D}] with H a multiple of {K} key heads")
+    if q.dtype != k_pages.dtype:
+        raise TypeError(f"q must have the pages' type {k_pages.dtype}, got {q.dtype}")
+    lead = tuple(q.shape[:-2])
+    table, had = _table(page_table, lengths, lead)
+    H, B, M = int(q.shape[-2]), math.prod(lead), int(table.shape[-1])
+    code = L.dtype_code(q.dtype)
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if B == 0:
+        return o
+    rows, ldq = _pitched(q if q.ndim > 2 else q.unsqueeze(0))
+    if rows.data_ptr() % 4 or ldq % 2:
+        rows, ldq = rows.clone(memory_format=torch.contiguous_format), H * D
+    nbytes = L.query("zg_paged_attention_workspace_size", B, H, K, D, M, page, window, sinks, code)
+    ws = L.workspace(nbytes, dev) if nbytes else None
+    _call(dev, "zg_paged_attention", L.ptr(rows), ldq, L.ptr(k_pages), L.ptr(v_pages), N, page, L.ptr(table), M,
+          L.ptr(had), B, H, K, D, window, sinks, code, L.ptr(o), L.ptr(ws), nbytes)
+    return o
+
+
+@torch.library.custom_op(f"{_NS}::paged_attention", mutates_args=())
+def _paged_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              lengths: torch.Tensor, window: int, sinks: int) -> torch.Tensor:
+    return launch_paged_attention(q, k_pages, v_pages, page_table, lengths, window, sinks)
+
+
+@torch.library.register_vmap(f"{_NS}::paged_attention")
+def _paged_vmap(info, in_dims, q, k_pages, v_pages, page_table, lengths, window, sinks):
+    if in_dims[1] is not None or in_dims[2] is not None:
+        raise NotImplementedError("pages batched over candidates are not supported: one pool holds every candidate's")
+    dims = (in_dims[0], in_dims[3], in_dims[4])
+    ts = [_movedim0(t, d) for t, d in zip((q, page_table, lengths), dims)]
+    ts = [t if d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, dims)]
+    return launch_paged_attention(ts[0], k_pages, v_pages, ts[1], ts[2], window, sinks), 0
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, window: int | None = None, sinks: int = 0) -> torch.Tensor:
+    """softmax(q kᵀ / sqrt(D)) v of each sequence's newest token over its
+    paged cache: q [..., H, D] is the query of position ``lengths`` - 1, whose
+    key and value :func:`append_pages` has written.
+
+    ``k_pages``, ``v_pages``, ``page_table`` as for :func:`append_pages`; K
+    divides H and query head h reads key head h // (H // K).  The token sees
+    the last ``window`` positions (None: all) and the first ``sinks``, as a
+    row of :func:`window_attention` does.  Pages may be shared by sequences.
+    A sequence of length 0 gives zeros; a length the table cannot hold, or a
+    visible page that is not one of the pool's, gives NaN.  D is at most 256;
+    float32 or bf16 (bf16 with D a multiple of 8 multiplies on the tensor
+    cores, pages 16-byte aligned).  The cache is read once; the work is split
+    over its length and joined in a fixed order."""
+    w, s = _span(window, sinks)
+    args = (q, k_pages, v_pages, page_table, lengths, w, s)
+    return launch_paged_attention(*args) if _plain_call(*args[:5]) else _paged_op(*args)
+
+
+__all__ = ["append_pages", "paged_attention", "rotary", "window_attention", "launch_append_pages",
+           "launch_paged_attention", "launch_rotary", "launch_window_attention"]

@@ -1,0 +1,786 @@
+// zg_paged.cu -- a paged key-value cache: writing new tokens into its pages,
+// and the attention of one new token over them.
+//
+// Pages are [N, page, K, D] (keys and values apart); a sequence's tokens
+// 0 .. length - 1 lie in the pages its row of the page table names, in order.
+//
+//   append:    token (b, s) of sequence b goes to position lengths[b] + s.
+//   attention: o[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(D)) v_j over the
+//              positions j that the newest token (position length - 1) sees:
+//              the last `window` ones and the first `sinks`.
+//
+// Both are bound by HBM: append moves each token once, and attention reads
+// each visible key and value once for the G = H / K query heads that share
+// them (4 G D flops on 4 D bytes at bf16: G flops per byte, far below the
+// tensor cores' or, in float32, the FMA pipe's rate for any usual G).
+#include <math.h>
+
+#include "zg_common.cuh"
+
+namespace {
+
+constexpr int PG_WARPS = 4;
+constexpr int64_t PG_MOST = 1 << 30;  // positions of a table's row, and of a pool
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+    void *kp, *vp;
+    const void *k, *v;
+    const int32_t *table, *lengths, *counts;
+    int32_t* new_lengths;
+    int64_t n_pages, ldk, ldv, row;  // row: words (or elements) of a token's K heads
+    int64_t rows;                    // B * S
+    int page, max_pages, B, S;
+};
+
+// The tokens of sequence b that are written: none when they do not fit.
+__device__ __forceinline__ bool append_span(const AppendArgs& a, int b, int& start, int& count) {
+    start = a.lengths[b];
+    count = a.counts ? a.counts[b] : a.S;
+    return start >= 0 && count >= 0 && count <= a.S &&
+           (int64_t)start + count <= (int64_t)a.max_pages * a.page;
+}
+
+// A warp per token, W the word that it is copied in (16 bytes, or one
+// element where a row's length or alignment does not allow that), key and
+// value words loaded before either is stored.  The warps behind the tokens'
+// own take a sequence each and write its new length.
+template <typename W>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+    const int lane = threadIdx.x % 32;
+    const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / 32;
+    int start, count;
+    if (w >= a.rows) {
+        const int64_t b = w - a.rows;
+        if (b >= a.B) return;
+        bool ok = append_span(a, (int)b, start, count);
+        if (ok && count > 0) {
+            const int last = (start + count - 1) / a.page;
+            bool bad = false;
+            for (int p = start / a.page + lane; p <= last; p += 32) {
+                const int32_t id = a.table[b * a.max_pages + p];
+                bad |= id < 0 || id >= a.n_pages;
+            }
+            ok = !__any_sync(0xffffffffu, bad);
+        }
+        if (lane == 0) a.new_lengths[b] = ok ? start + count : -1;
+        return;
+    }
+    const int b = (int)(w / a.S), s = (int)(w % a.S);
+    if (!append_span(a, b, start, count) || s >= count) return;
+    const int at = start + s;
+    const int32_t id = a.table[(int64_t)b * a.max_pages + at / a.page];
+    if (id < 0 || id >= a.n_pages) return;
+    const int64_t to = ((int64_t)id * a.page + at % a.page) * a.row;
+    const W* ks = static_cast<const W*>(a.k) + w * a.ldk;
+    const W* vs = static_cast<const W*>(a.v) + w * a.ldv;
+    W* kd = static_cast<W*>(a.kp) + to;
+    W* vd = static_cast<W*>(a.vp) + to;
+    int64_t i = lane;
+    for (; i + 32 < a.row; i += 64) {
+        const W k0 = ks[i], k1 = ks[i + 32], v0 = vs[i], v1 = vs[i + 32];
+        kd[i] = k0;
+        kd[i + 32] = k1;
+        vd[i] = v0;
+        vd[i + 32] = v1;
+    }
+    if (i < a.row) {
+        const W k0 = ks[i], v0 = vs[i];
+        kd[i] = k0;
+        vd[i] = v0;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// attention of one token
+// ---------------------------------------------------------------------------
+struct PagedArgs {
+    const void *q, *kp, *vp;
+    const int32_t *table, *lengths;
+    void* o;
+    float* part;  // splits > 1: per unit and split, m [R], l [R], then R rows of sums
+    int64_t ldq, n_pages;
+    int page, max_pages, H, K, D, G, row_tiles, R;  // R: query rows of a unit (heads that share a key head)
+    int window, sinks, chunk, splits;
+    float scale;  // log2(e) / sqrt(D)
+};
+
+__host__ __device__ __forceinline__ int pad4(int d) { return (d + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int64_t part_floats(int R, int D) { return 2 * (int64_t)R + (int64_t)R * pad4(D); }
+
+// What the newest of `length` tokens sees: positions 0 .. s-1 and, behind a
+// gap, the last of them; vis of them in all.  vis < 0: the length is not one
+// the table can hold.
+struct Seen {
+    int vis, s, gap;
+    __device__ __forceinline__ int token(int t) const { return t < s ? t : t + gap; }
+};
+__device__ __forceinline__ Seen seen_by(const PagedArgs& a, int b) {
+    const int n = a.lengths[b];
+    if (n < 0 || (int64_t)n > (int64_t)a.max_pages * a.page) return Seen{-1, 0, 0};
+    const int w = a.window > 0 && a.window < n ? a.window : n;
+    const int s = a.sinks < n - w ? a.sinks : n - w;
+    return Seen{w + s, s, n - w - s};
+}
+
+// The place (page * page size + slot) of visible position t, -1 past `end`
+// or, with bad set, where the table names no page.
+__device__ __forceinline__ int place_of(const PagedArgs& a, const Seen& v, const int32_t* row, int t, int end,
+                                        bool& bad) {
+    if (t >= end) return -1;
+    const int tok = v.token(t), p = tok / a.page;
+    const int32_t id = row[p];
+    if (id < 0 || id >= a.n_pages) {
+        bad = true;
+        return -1;
+    }
+    return id * a.page + (tok - p * a.page);
+}
+
+__device__ __forceinline__ uint32_t shared_u32(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// 16 bytes from global to shared memory, zeros when `bytes` is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Joins the warps' (m, l, sums) of one unit in shared memory, in warp order,
+// and writes the output (one split) or this split's partial.
+// ms, ls [PG_WARPS][R]; os [PG_WARPS][R][pitch].
+template <typename T>
+__device__ __forceinline__ void join_warps(const PagedArgs& a, const float* ms, const float* ls, const float* os,
+                                           int pitch, int rows, int b, int h0, int64_t unit, int split, bool bad,
+                                           bool none) {
+    float* part = a.splits > 1 ? a.part + (unit * a.splits + split) * part_floats(a.R, a.D) : nullptr;
+    for (int i = threadIdx.x; i < rows * a.D; i += PG_WARPS * 32) {
+        const int r = i / a.D, d = i - r * a.D;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[w * a.R + r]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float l = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < PG_WARPS; ++w) {
+            const float f = exp2_fast(ms[w * a.R + r] - base);
+            l = fmaf(ls[w * a.R + r], f, l);
+            x = fmaf(os[(w * a.R + r) * pitch + d], f, x);
+        }
+        if (bad) l = __int_as_float(0x7fffffff);
+        if (part) {
+            if (d == 0) {
+                part[r] = M;
+                part[a.R + r] = l;
+            }
+            part[2 * a.R + r * pad4(a.D) + d] = x;
+        } else {
+            static_cast<T*>(a.o)[((int64_t)b * a.H + h0 + r) * a.D + d] = zg_from_float<T>(none ? 0.f : x / l);
+        }
+    }
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// bf16 with D a multiple of 8 (padded to DP with zeros): up to 16 query heads
+// of one key head are the rows of m16n8k16 products.  Every warp works alone
+// on tiles of 16 positions, its own ring of STAGES tiles filled by cp.async
+// (a tile's rows are fetched through the page table, whose entries are read
+// one tile earlier), with its own running maximum and sum; the four warps
+// meet once, at the end.  The products are a small part of the time the
+// bytes take: 16 rows of which G are used cost nothing that matters, and a
+// larger tile of the tensor cores of this chip would have to wait for 128
+// positions where a warp goes on after 16.
+template <int DP, int STAGES>
+__global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArgs a) {
+    using T = __nv_bfloat16;
+    constexpr int CPR = DP / 8;             // 16-byte chunks of a row
+    constexpr int TILE = 16 * DP * 2;       // bytes of 16 key (or value) rows
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float ms[PG_WARPS * 16], ls[PG_WARPS * 16];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t unit = blockIdx.x / a.splits;
+    const int split = (int)(blockIdx.x % a.splits);
+    const int rt = (int)(unit % a.row_tiles), kh = (int)(unit / a.row_tiles % a.K);
+    const int b = (int)(unit / a.row_tiles / a.K);
+    const int rows = a.G - rt * 16 < 16 ? a.G - rt * 16 : 16;
+    const int h0 = kh * a.G + rt * 16;
+    const Seen see = seen_by(a, b);
+    const int c0 = split * a.chunk;
+    const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;  // this split: [c0, end)
+    if (c0 >= see.vis && a.splits > 1) return;  // nothing here; the join knows by the length
+    const int32_t* table = a.table + (int64_t)b * a.max_pages;
+    const int tiles_all = end > c0 ? (end - c0 + 15) / 16 : 0;
+    const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
+    uint8_t* ring = smem + warp * (STAGES * 2 * TILE);
+    const T* kp = static_cast<const T*>(a.kp) + kh * a.D;
+    const T* vp = static_cast<const T*>(a.vp) + kh * a.D;
+    const int64_t token_pitch = (int64_t)a.K * a.D;
+    bool bad = false;
+
+    // lanes 0..15: the place of each row of this warp's tile i
+    auto places = [&](int i) {
+        return i < tiles && lane < 16 ? place_of(a, see, table, c0 + (warp + PG_WARPS * i) * 16 + lane, end, bad) : -1;
+    };
+    auto fetch = [&](int stage, int place) {
+        const uint32_t kd = shared_u32(ring + stage * 2 * TILE), vd = kd + TILE;
+#pragma unroll
+        for (int it = 0; it < CPR / 2; ++it) {
+            const int i = it * 32 + lane, r = i / CPR, c = i % CPR;
+            const int at = __shfl_sync(0xffffffffu, place, r);
+            const bool on = at >= 0 && c * 8 < a.D;
+            const int64_t off = on ? at * token_pitch + c * 8 : 0;
+            const uint32_t to = r * (DP * 2) + ((c ^ (r & 7)) * 16);
+            copy16(kd + to, kp + off, on ? 16 : 0);
+            copy16(vd + to, vp + off, on ? 16 : 0);
+        }
+    };
+
+    int place = places(0);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        const int next = places(s + 1);
+        if (s < tiles) fetch(s, place);
+        copy_commit();
+        place = next;
+    }
+
+    // queries as the rows of A: (row, k) = (lane / 4 [+ 8], 2 (lane % 4) [+ 8]) in k-steps of 16
+    uint32_t qf[DP / 16][4];
+    {
+        const T* q = static_cast<const T*>(a.q) + b * a.ldq + (int64_t)h0 * a.D;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = lane / 4 + (e & 1) * 8, d = k * 16 + (lane % 4) * 2 + (e >> 1) * 8;
+                qf[k][e] = r < rows && d < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)r * a.D + d) : 0u;
+            }
+    }
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows lane/4 and lane/4 + 8, in units of log2
+
+    const int k_row = (lane % 8) + 8 * (lane / 16), k_chunk = (lane / 8) % 2;
+    const int v_row = (lane % 8) + 8 * ((lane / 8) % 2), v_chunk = lane / 16;
+    for (int i = 0; i < tiles; ++i) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();  // every lane's copies of tile i have landed, and tile i-1 has been read
+        {
+            const int next = places(i + STAGES);
+            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place);
+            copy_commit();
+            place = next;
+        }
+        const uint32_t kt = shared_u32(ring + (i % STAGES) * 2 * TILE), vt = kt + TILE;
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t f[4];
+            ldmatrix4(f, kt + k_row * (DP * 2) + (((2 * k + k_chunk) ^ (k_row & 7)) * 16));
+            mma_bf16(s[0], qf[k], f[0], f[1]);
+            mma_bf16(s[1], qf[k], f[2], f[3]);
+        }
+        const int t0 = c0 + (warp + PG_WARPS * i) * 16;
+        float n0 = -INFINITY, n1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[j][e] = t0 + j * 8 + (lane % 4) * 2 + (e & 1) < end ? s[j][e] * a.scale : -INFINITY;
+                if (e < 2) n0 = fmaxf(n0, s[j][e]);
+                else n1 = fmaxf(n1, s[j][e]);
+            }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+        }
+        n0 = fmaxf(n0, m0);
+        n1 = fmaxf(n1, m1);
+        const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+            const float f0 = exp2_fast(m0 - b0), f1 = exp2_fast(m1 - b1);
+            l0 *= f0;
+            l1 *= f1;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d) {
+                o[d][0] *= f0;
+                o[d][1] *= f0;
+                o[d][2] *= f1;
+                o[d][3] *= f1;
+            }
+            m0 = n0;
+            m1 = n1;
+        }
+        // weights, rounded to bf16 as the second product's operand (their sum
+        // is of the unrounded ones): half a step of each weight, 2^-9
+        uint32_t p[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float p0 = exp2_fast(s[j][0] - b0), p1 = exp2_fast(s[j][1] - b0);
+            const float p2 = exp2_fast(s[j][2] - b1), p3 = exp2_fast(s[j][3] - b1);
+            l0 += p0 + p1;
+            l1 += p2 + p3;
+            p[2 * j] = pack_bf16(p0, p1);
+            p[2 * j + 1] = pack_bf16(p2, p3);
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+            uint32_t f[4];
+            ldmatrix4_t(f, vt + v_row * (DP * 2) + (((2 * d + v_chunk) ^ (v_row & 7)) * 16));
+            mma_bf16(o[2 * d], p, f[0], f[1]);
+            mma_bf16(o[2 * d + 1], p, f[2], f[3]);
+        }
+    }
+    copy_wait<0>();
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+    }
+    bad = __syncthreads_or(bad || see.vis < 0);  // the rings are free from here on
+    float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][16][DP]
+    const int r = lane / 4;
+    if (lane % 4 == 0) {
+        ms[warp * 16 + r] = m0;
+        ms[warp * 16 + r + 8] = m1;
+        ls[warp * 16 + r] = l0;
+        ls[warp * 16 + r + 8] = l1;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) {
+        float* to = os + (warp * 16 + r) * DP + d * 8 + (lane % 4) * 2;
+        *reinterpret_cast<float2*>(to) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(o[d][2], o[d][3]);
+    }
+    __syncthreads();
+    join_warps<T>(a, ms, ls, os, DP, rows, b, h0, unit, split, bad, see.vis == 0);
+}
+
+// Any type, width and alignment, in float32 on the FMA pipe.  A warp's tile
+// has 32 / PARTS positions: PARTS lanes share a position's dot products (each
+// a PARTS-th of the columns), then every lane takes the columns lane + 32 i
+// of the sums.  GT query heads at a time; the same ring of tiles as above,
+// its rows kept as they are stored, 16 bytes apart from the next one's banks.
+template <typename T, int PARTS, int GT>
+__global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArgs a, int vec) {
+    constexpr int TT = 32 / PARTS, STAGES = 3, NI = PARTS, DMAX = 32 * PARTS;
+    constexpr int PITCH = DMAX * (int)sizeof(T) + 16, TILE = TT * PITCH;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float ms[PG_WARPS * GT], ls[PG_WARPS * GT];
+    __shared__ __align__(16) float qs[GT][DMAX];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t unit = blockIdx.x / a.splits;
+    const int split = (int)(blockIdx.x % a.splits);
+    const int rt = (int)(unit % a.row_tiles), kh = (int)(unit / a.row_tiles % a.K);
+    const int b = (int)(unit / a.row_tiles / a.K);
+    const int rows = a.G - rt * GT < GT ? a.G - rt * GT : GT;
+    const int h0 = kh * a.G + rt * GT;
+    const Seen see = seen_by(a, b);
+    const int c0 = split * a.chunk;
+    const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;
+    if (c0 >= see.vis && a.splits > 1) return;
+    const int32_t* table = a.table + (int64_t)b * a.max_pages;
+    const int tiles_all = end > c0 ? (end - c0 + TT - 1) / TT : 0;
+    const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
+    uint8_t* ring = smem + warp * (STAGES * 2 * TILE);
+    const T* kp = static_cast<const T*>(a.kp) + kh * a.D;
+    const T* vp = static_cast<const T*>(a.vp) + kh * a.D;
+    const int64_t token_pitch = (int64_t)a.K * a.D;
+    bool bad = false;
+
+    for (int i = threadIdx.x; i < GT * DMAX; i += PG_WARPS * 32) {
+        const int r = i / DMAX, d = i % DMAX;
+        qs[r][d] = r < rows && d < a.D ? zg_to_float(static_cast<const T*>(a.q)[b * a.ldq + (int64_t)(h0 + r) * a.D + d]) * a.scale : 0.f;
+    }
+    // the columns past D stay zero in every stage
+    for (int i = lane; i < STAGES * 2 * TILE / 4; i += 32) reinterpret_cast<uint32_t*>(ring)[i] = 0u;
+    __syncthreads();
+
+    auto places = [&](int i) {
+        return i < tiles && lane < TT ? place_of(a, see, table, c0 + (warp + PG_WARPS * i) * TT + lane, end, bad) : -1;
+    };
+    const int words = vec ? a.D * (int)sizeof(T) / 16 : a.D;  // of a row
+    auto fetch = [&](int stage, int place) {
+        uint8_t* kd = ring + stage * 2 * TILE;
+        uint8_t* vd = kd + TILE;
+        int r = lane / words, c = lane - r * words;
+        for (int i = 0; i < TT * words; i += 32) {
+            const int at = __shfl_sync(0xffffffffu, place, r < TT ? r : 0);
+            if (r < TT) {
+                const int64_t off = at >= 0 ? at * token_pitch : 0;
+                if (vec) {
+                    constexpr int N = 16 / sizeof(T);
+                    copy16(shared_u32(kd + r * PITCH + c * 16), kp + off + (at >= 0 ? c * N : 0), at >= 0 ? 16 : 0);
+                    copy16(shared_u32(vd + r * PITCH + c * 16), vp + off + (at >= 0 ? c * N : 0), at >= 0 ? 16 : 0);
+                } else {
+                    reinterpret_cast<T*>(kd + r * PITCH)[c] = at >= 0 ? kp[off + c] : zg_from_float<T>(0.f);
+                    reinterpret_cast<T*>(vd + r * PITCH)[c] = at >= 0 ? vp[off + c] : zg_from_float<T>(0.f);
+                }
+            }
+            c += 32;
+            while (c >= words) {
+                c -= words;
+                ++r;
+            }
+        }
+    };
+    int place = places(0);
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        const int next = places(s + 1);
+        if (s < tiles) fetch(s, place);
+        copy_commit();
+        place = next;
+    }
+    float o[GT][NI], m[GT], l[GT];
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) o[g][i] = 0.f;
+    }
+    const int tok = lane % TT, part = lane / TT;
+    for (int i = 0; i < tiles; ++i) {
+        copy_wait<STAGES - 2>();
+        __syncwarp();
+        {
+            const int next = places(i + STAGES);
+            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place);
+            copy_commit();
+            place = next;
+        }
+        const uint8_t* kt = ring + (i % STAGES) * 2 * TILE;
+        const uint8_t* vt = kt + TILE;
+        float s[GT];
+#pragma unroll
+        for (int g = 0; g < GT; ++g) s[g] = 0.f;
+        const T* kr = reinterpret_cast<const T*>(kt + tok * PITCH) + part * 32;
+#pragma unroll
+        for (int d = 0; d < 32; d += 4) {
+            float kv[4];
+            if constexpr (sizeof(T) == 4) {
+                const float4 x = *reinterpret_cast<const float4*>(kr + d);
+                kv[0] = x.x; kv[1] = x.y; kv[2] = x.z; kv[3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(kr + d);
+                kv[0] = __uint_as_float(x.x << 16); kv[1] = __uint_as_float(x.x & 0xffff0000u);
+                kv[2] = __uint_as_float(x.y << 16); kv[3] = __uint_as_float(x.y & 0xffff0000u);
+            }
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                const float4 x = *reinterpret_cast<const float4*>(&qs[g][part * 32 + d]);
+                s[g] = fmaf(kv[0], x.x, fmaf(kv[1], x.y, fmaf(kv[2], x.z, fmaf(kv[3], x.w, s[g]))));
+            }
+        }
+        const bool on = c0 + (warp + PG_WARPS * i) * TT + tok < end;
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+#pragma unroll
+            for (int x = TT; x < 32; x <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], x);
+            s[g] = on ? s[g] : -INFINITY;
+            float n = s[g];
+#pragma unroll
+            for (int x = 1; x < TT; x <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
+            n = fmaxf(n, m[g]);
+            const float base = n == -INFINITY ? 0.f : n;
+            const float f = exp2f(m[g] - base);
+            m[g] = n;
+            s[g] = exp2f(s[g] - base);
+            l[g] = fmaf(l[g], f, part == 0 ? s[g] : 0.f);
+#pragma unroll
+            for (int c = 0; c < NI; ++c) o[g][c] *= f;
+        }
+#pragma unroll 4
+        for (int t = 0; t < TT; ++t) {
+            float v[NI];
+            const T* vr = reinterpret_cast<const T*>(vt + t * PITCH);
+#pragma unroll
+            for (int c = 0; c < NI; ++c) v[c] = zg_to_float(vr[lane + 32 * c]);
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                const float p = __shfl_sync(0xffffffffu, s[g], t);
+#pragma unroll
+                for (int c = 0; c < NI; ++c) o[g][c] = fmaf(p, v[c], o[g][c]);
+            }
+        }
+    }
+    copy_wait<0>();
+    bad = __syncthreads_or(bad || see.vis < 0);
+    float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][GT][DMAX]
+#pragma unroll
+    for (int g = 0; g < GT; ++g) {
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], x);
+        if (lane == 0) {
+            ms[warp * GT + g] = m[g];
+            ls[warp * GT + g] = l[g];
+        }
+#pragma unroll
+        for (int c = 0; c < NI; ++c) os[(warp * GT + g) * DMAX + lane + 32 * c] = o[g][c];
+    }
+    __syncthreads();
+    join_warps<T>(a, ms, ls, os, DMAX, rows, b, h0, unit, split, bad, see.vis == 0);
+}
+
+// Joins the splits of one query head: a block per (b, h), its warps over the
+// splits, summed in warp order.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
+    __shared__ float4 sums[8][64];
+    __shared__ float sum_l[8];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
+    const int kh = h / a.G, rt = h % a.G / a.R, r = h % a.G % a.R;
+    const int64_t unit = ((int64_t)b * a.K + kh) * a.row_tiles + rt;
+    const int vis = seen_by(a, b).vis;
+    const int n = vis > 0 ? (vis + a.chunk - 1) / a.chunk : 0;
+    const int64_t pf = part_floats(a.R, a.D);
+    const float* part = a.part + unit * a.splits * pf;
+    const int words = pad4(a.D) / 4;
+    float M = -INFINITY;
+    for (int s = lane; s < n; s += 32) M = fmaxf(M, part[s * pf + r]);
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    const float base = M == -INFINITY ? 0.f : M;
+    float l = 0.f;
+    float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+    for (int s = warp; s < n; s += 8) {
+        const float* p = part + s * pf;
+        const float f = exp2f(p[r] - base);
+        l = fmaf(p[a.R + r], f, l);
+        const float* row = p + 2 * a.R + r * (words * 4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            if (lane + 32 * j < words) {
+                // rows start on 8-byte boundaries at least (2 R floats, R even, or R = 1)
+                const float2 u = *reinterpret_cast<const float2*>(row + 4 * (lane + 32 * j));
+                const float2 w = *reinterpret_cast<const float2*>(row + 4 * (lane + 32 * j) + 2);
+                x[j].x = fmaf(u.x, f, x[j].x);
+                x[j].y = fmaf(u.y, f, x[j].y);
+                x[j].z = fmaf(w.x, f, x[j].z);
+                x[j].w = fmaf(w.y, f, x[j].w);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (lane + 32 * j < words) sums[warp][lane + 32 * j] = x[j];
+    if (lane == 0) sum_l[warp] = l;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= a.D) return;
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+        num += reinterpret_cast<const float*>(sums[w])[d];
+        den += sum_l[w];
+    }
+    const float out = vis < 0 ? __int_as_float(0x7fffffff) : vis == 0 ? 0.f : num / den;
+    static_cast<T*>(a.o)[((int64_t)b * a.H + h) * a.D + d] = zg_from_float<T>(out);
+}
+
+// How a call is cut: R query rows of a unit, and the units' splits.
+struct PagedPlan {
+    int R, row_tiles, chunk, splits;
+    bool mma;
+};
+
+PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window, int sinks, int dtype) {
+    PagedPlan p{};
+    const int G = H / K;
+    p.mma = dtype == ZG_BF16 && D % 8 == 0;
+    p.R = p.mma ? 16 : G == 1 ? 1 : G <= 4 ? 4 : 8;
+    p.row_tiles = (G + p.R - 1) / p.R;
+    int64_t vis = longest;
+    if (window > 0 && (int64_t)window + sinks < vis) vis = (int64_t)window + sinks;
+    if (vis < 1) vis = 1;
+    const int64_t units = B * K * p.row_tiles;
+    // Two blocks run on each of 148 SMs.  One sequence: as many splits as
+    // fill them once.  A batch: four times that, so that sequences of
+    // different lengths, cut into pieces of one length, even out.
+    const int64_t want = 2 * 148 * (B == 1 ? 1 : 4);
+    int64_t splits = want / units;
+    if (splits < 1) splits = 1;
+    if (splits > 128) splits = 128;
+    int64_t chunk = (vis + splits - 1) / splits;
+    if (chunk < 256) chunk = 256;  // less would be the pipeline's filling and the join
+    chunk = (chunk + 63) / 64 * 64;
+    p.chunk = (int)(chunk > INT32_MAX ? INT32_MAX / 64 * 64 : chunk);
+    p.splits = (int)((vis + p.chunk - 1) / p.chunk);
+    return p;
+}
+
+size_t paged_workspace(const PagedPlan& p, int64_t B, int K, int D) {
+    return p.splits > 1 ? (size_t)(B * K * p.row_tiles * p.splits * part_floats(p.R, D)) * sizeof(float) : 0;
+}
+
+bool paged_sizes_ok(int64_t n_pages, int page, int64_t B, int H, int K, int D, int max_pages) {
+    return n_pages >= 0 && page >= 1 && B >= 0 && H >= 1 && K >= 1 && D >= 1 && max_pages >= 0 && H % K == 0;
+}
+
+template <typename F>
+int set_smem(F* f, size_t bytes) {
+    if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+        return zg::fail(ZG_ERR_CUDA, "zg_paged_attention: shared memory attribute");
+    return ZG_OK;
+}
+
+template <int DP, int STAGES>
+int launch_mma(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
+    const size_t smem = (size_t)PG_WARPS * STAGES * 2 * 16 * DP * 2;
+    if (int rc = set_smem(paged_mma_kernel<DP, STAGES>, smem)) return rc;
+    zg::LaunchTimer zg_lt_("paged_attention", st);
+    paged_mma_kernel<DP, STAGES><<<(unsigned)blocks, PG_WARPS * 32, smem, st>>>(a);
+    return zg::check_launch("zg_paged_attention");
+}
+
+template <typename T, int PARTS, int GT>
+int launch_fma(const PagedArgs& a, int vec, int64_t blocks, cudaStream_t st) {
+    const size_t ring = (size_t)PG_WARPS * 3 * 2 * (32 / PARTS) * (32 * PARTS * sizeof(T) + 16);
+    const size_t out = (size_t)PG_WARPS * GT * 32 * PARTS * sizeof(float);
+    const size_t smem = ring > out ? ring : out;
+    if (int rc = set_smem(paged_fma_kernel<T, PARTS, GT>, smem)) return rc;
+    zg::LaunchTimer zg_lt_("paged_attention_fma", st);
+    paged_fma_kernel<T, PARTS, GT><<<(unsigned)blocks, PG_WARPS * 32, smem, st>>>(a, vec);
+    return zg::check_launch("zg_paged_attention");
+}
+
+template <typename T, int PARTS>
+int launch_fma_rows(const PagedArgs& a, int vec, int64_t blocks, cudaStream_t st) {
+    if (a.R == 1) return launch_fma<T, PARTS, 1>(a, vec, blocks, st);
+    if (a.R == 4) return launch_fma<T, PARTS, 4>(a, vec, blocks, st);
+    return launch_fma<T, PARTS, 8>(a, vec, blocks, st);
+}
+
+template <typename T>
+int launch_fma_any(const PagedArgs& a, int vec, int64_t blocks, cudaStream_t st) {
+    if (a.D <= 64) return launch_fma_rows<T, 2>(a, vec, blocks, st);
+    if (a.D <= 128) return launch_fma_rows<T, 4>(a, vec, blocks, st);
+    return launch_fma_rows<T, 8>(a, vec, blocks, st);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+extern "C" int zg_append_pages(void* k_pages, void* v_pages, int64_t n_pages, int page, int K, int D, const void* k,
+                               int64_t ldk, const void* v, int64_t ldv, int64_t B, int64_t S, const int32_t* table,
+                               int max_pages, const int32_t* lengths, const int32_t* counts, int dtype,
+                               int32_t* new_lengths, void* stream) {
+    if (!paged_sizes_ok(n_pages, page, B, K, K, D, max_pages) || S < 0 || B > INT32_MAX || S > INT32_MAX)
+        return zg::fail(ZG_ERR_INVALID, "zg_append_pages: bad sizes");
+    if (ldk < (int64_t)K * D || ldv < (int64_t)K * D)
+        return zg::fail(ZG_ERR_INVALID, "zg_append_pages: row pitch below K*D");
+    if (!zg::dtype_ok(dtype)) return zg::fail(ZG_ERR_INVALID, "zg_append_pages: bad dtype");
+    if ((int64_t)max_pages * page > PG_MOST) return zg::fail(ZG_ERR_INVALID, "zg_append_pages: table too long");
+    if (B == 0) return ZG_OK;
+    if (!lengths || !new_lengths || (max_pages && !table) || (S && (!k || !v)) || (n_pages && (!k_pages || !v_pages)))
+        return zg::fail(ZG_ERR_INVALID, "zg_append_pages: null pointer");
+    const int64_t blocks = (B * S + B + 7) / 8;
+    if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_append_pages: too many tokens");
+    const int esize = (int)zg::dtype_size(dtype);
+    const int n = 16 / esize;
+    const int64_t row = (int64_t)K * D;
+    const bool vec = row % n == 0 && ldk % n == 0 && ldv % n == 0 && aligned16(k) && aligned16(v) &&
+                     aligned16(k_pages) && aligned16(v_pages);
+    const int w = vec ? n : 1;
+    const AppendArgs a{k_pages, v_pages, k, v, table, lengths, counts, new_lengths, n_pages, ldk / w, ldv / w,
+                       row / w, B * S, page, max_pages, (int)B, (int)S};
+    cudaStream_t st = zg::as_stream(stream);
+    zg::LaunchTimer zg_lt_("append_pages", st);
+    if (vec)
+        append_kernel<uint4><<<(unsigned)blocks, 256, 0, st>>>(a);
+    else if (esize == 2)
+        append_kernel<uint16_t><<<(unsigned)blocks, 256, 0, st>>>(a);
+    else
+        append_kernel<uint32_t><<<(unsigned)blocks, 256, 0, st>>>(a);
+    return zg::check_launch("zg_append_pages");
+}
+
+extern "C" size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int D, int max_pages, int page,
+                                                    int window, int sinks, int dtype) {
+    if (!paged_sizes_ok(0, page, B, H, K, D, max_pages) || D > 256 || window < 0 || sinks < 0 || !zg::dtype_ok(dtype))
+        return 0;
+    return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), B, K, D);
+}
+
+extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
+                                  int64_t n_pages, int page, const int32_t* table, int max_pages,
+                                  const int32_t* lengths, int64_t B, int H, int K, int D, int window, int sinks,
+                                  int dtype, void* o, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!paged_sizes_ok(n_pages, page, B, H, K, D, max_pages))
+        return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: bad sizes");
+    if (D > 256) return zg::fail(ZG_ERR_UNSUPPORTED, "zg_paged_attention: head dim above 256");
+    if (window < 0 || sinks < 0) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: window and sinks must be >= 0");
+    if (ldq < (int64_t)H * D) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: row pitch below H*D");
+    if (!zg::dtype_ok(dtype)) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: bad dtype");
+    if ((int64_t)max_pages * page > PG_MOST || (n_pages && n_pages > PG_MOST / page))
+        return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: more positions than 32 bits count");
+    if (B == 0) return ZG_OK;
+    if (!q || !lengths || !o || (max_pages && !table) || (n_pages && (!k_pages || !v_pages)))
+        return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: null pointer");
+    PagedPlan p = paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype);
+    const size_t need = paged_workspace(p, B, K, D);
+    if (need && (!workspace || workspace_bytes < need))
+        return zg::fail(ZG_ERR_WORKSPACE, "zg_paged_attention: workspace of %zu bytes needed", need);
+    const int64_t blocks = B * K * p.row_tiles * p.splits;
+    if (blocks > INT32_MAX || B * H > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: too many rows");
+    const int n = 16 / (int)zg::dtype_size(dtype);
+    const int vec = D % n == 0 && aligned16(k_pages) && aligned16(v_pages);
+    PagedArgs a{q, k_pages, v_pages, table, lengths, o, static_cast<float*>(workspace), ldq, n_pages, page, max_pages,
+                H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.chunk, p.splits,
+                (float)(1.4426950408889634 / sqrt((double)D))};
+    cudaStream_t st = zg::as_stream(stream);
+    int rc;
+    if (p.mma && vec && ldq % 2 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0) {
+        rc = D <= 64 ? launch_mma<64, 4>(a, blocks, st)
+             : D <= 128 ? launch_mma<128, 3>(a, blocks, st) : launch_mma<256, 3>(a, blocks, st);
+    } else if (p.mma) {
+        return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: bf16 pages with D a multiple of 8 must be 16-byte "
+                                        "aligned, q 4-byte aligned with an even pitch");
+    } else {
+        rc = dtype == ZG_BF16 ? launch_fma_any<__nv_bfloat16>(a, vec, blocks, st)
+                              : launch_fma_any<float>(a, vec, blocks, st);
+    }
+    if (rc != ZG_OK || p.splits == 1) return rc;
+    zg::LaunchTimer zg_lt_("paged_join", st);
+    if (dtype == ZG_BF16)
+        paged_join_kernel<__nv_bfloat16><<<(unsigned)(B * H), 256, 0, st>>>(a);
+    else
+        paged_join_kernel<float><<<(unsigned)(B * H), 256, 0, st>>>(a);
+    return zg::check_launch("zg_paged_attention");
+}

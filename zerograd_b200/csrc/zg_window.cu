@@ -8,6 +8,8 @@
 // zeros.  4 D flops for each visible (i, j) and head.
 #include <math.h>
 
+#include <type_traits>
+
 #include "zg_ptx.cuh"
 #include "zg_tc.cuh"
 
@@ -27,6 +29,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The larger of two values, NaN if one is.
+__device__ __forceinline__ float max_nan(float x, float y) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+    return m;
+}
+
+// 2^y of two values on the FMA pipe, for y in [-120, 120]: y = n + f with n the
+// nearest whole number (by adding and taking off 1.5 * 2^23), 2^f by a
+// polynomial of degree 4 fitted to the relative error on [-1/2, 1/2] (2.7e-6,
+// 2^-18.5), n added to the exponent.  The special-function pipe has 16 results a
+// clock and SM, an eighth of the FMA pipe's rate: part of a row's weights
+// are formed here.
+__device__ __forceinline__ float2 exp2_fma(float2 y) {
+    const float2 one = make_float2(1.f, 1.f), magic = make_float2(12582912.f, 12582912.f);
+    y.x = fmaxf(y.x, -120.f);
+    y.y = fmaxf(y.y, -120.f);
+    const float2 t = ffma2_tc(y, one, magic);
+    const float2 n = ffma2_tc(t, one, make_float2(-12582912.f, -12582912.f));
+    const float2 f = ffma2_tc(n, make_float2(-1.f, -1.f), y);
+    float2 p = make_float2(0.00957010127604f, 0.00957010127604f);
+    p = ffma2_tc(p, f, make_float2(0.05591785907745f, 0.05591785907745f));
+    p = ffma2_tc(p, f, make_float2(0.24024744331837f, 0.24024744331837f));
+    p = ffma2_tc(p, f, make_float2(0.69312179088593f, 0.69312179088593f));
+    p = ffma2_tc(p, f, make_float2(0.99999928474426f, 0.99999928474426f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // The length of sequence z; -1 when it is not one of [0, S].
@@ -301,66 +332,79 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // Tensor-core path: bf16, D <= DP (64 or 128, zeros behind D).
 //
-// A persistent CTA per SM, 384 threads: warp 0 issues the TMA loads, warp 1
-// the MMAs, warps 4-7 and 8-11 are the softmax groups of two tiles of 128
-// query rows (one thread a row).  A work unit is a pair of neighbouring
-// tiles of one (z, head), so that each block of 128 keys and values is
-// fetched once for both; the units with the most visible keys come first.
-// Per block and tile: S = Q K^T into TMEM (M = N = 128), a row's maximum, the
-// weights p = 2^(s - m) as bf16 back into TMEM, O += P V with P read from
-// TMEM.  While one tile's group is at its weights, the tensor cores work for
-// the other.  Only blocks that a tile sees any key of are visited, and only
-// those at the edge of the mask test each key.
+// A persistent CTA per SM, 384 threads: warp 0 issues the TMA loads, warps
+// 1 and 2 the MMAs of a tile each, warps 4-7 and 8-11 are the softmax groups
+// of two tiles of 128 query rows (one thread a row).  A work unit is a pair of
+// neighbouring tiles of one (z, head), so that each block of 64 keys and
+// values is fetched once for both; the units with the most visible keys come
+// first.  Per block and tile: S = Q K^T into TMEM (M = 128, N = 64), a row's
+// maximum, the weights p = 2^(s - m) as bf16 back into TMEM over the scores,
+// O += P V with P read from TMEM.  Only blocks that a tile sees any key of are
+// visited, only those at the edge of a warp's mask test each key, and a warp
+// whose rows see none of a block's keys writes its zero weights at once.
+//
+// TMEM (512 columns): O of the two tiles; scores, one buffer of 64 columns a
+// tile with DP = 128 and two with DP = 64; weights, two buffers of 32 columns a
+// tile.  A group reads a block's scores into registers and says so, and the
+// next block's Q K^T runs under its softmax; the weights have columns of their
+// own, so that they do not hold it up.  (Weights over the scores they came
+// from, the next Q K^T behind P V: 2100 clocks a block of 64 at D = 128, 600 of
+// them waiting for scores.)
 //
 // The maximum m that weights are taken against is moved, and O rescaled by
 // its group, only when a row's true maximum is more than 2^8 above it: the
 // quotient O / l is the same, weights stay below 2^8 (and their relative
 // rounding in bf16 is what it was), and after the first blocks O is hardly
 // ever touched.
-//
-// TMEM (512 columns): S of the two tiles, O of the two tiles, and P: with
-// DP = 64 in columns of its own, so the next block's Q K^T is issued before P V
-// and runs under the next softmax; with DP = 128 over the scores it came from
-// (no column is left), so the next Q K^T waits for P V to have read it.
 // ---------------------------------------------------------------------------
 constexpr int WT_THREADS = 384;
-constexpr int WT_BLOCK = 128;  // keys of a block, rows of a tile
+constexpr int WT_POLY = 3;   // every third pair of weights comes from the polynomial
 
 template <int DP>
 struct WtShape {
-    static constexpr uint32_t TILE = 128 * DP * 2;       // bytes of a tile of rows: DP / 64 boxes of 128 x 64
-    static constexpr int STAGES = DP == 64 ? 8 : 5;      // ring of key and value blocks
-    static constexpr uint32_t RING = 2 * TILE;           // behind the two query tiles
-    static constexpr uint32_t CTRL = RING + STAGES * TILE;
+    static constexpr int KEYS = DP == 64 ? 128 : 64;         // keys of a block
+    static constexpr int HALVES = KEYS / 64;
+    static constexpr uint32_t QTILE = 128 * DP * 2;          // a query tile: DP / 64 boxes of 128 rows x 64 columns
+    static constexpr uint32_t BOX = KEYS * 128;              // KEYS rows x 64 columns
+    static constexpr uint32_t BLOCK = KEYS * DP * 2;         // a key or value block: DP / 64 boxes
+    static constexpr int STAGES = 5;                         // ring of blocks, the keys and behind them the values
+    static constexpr uint32_t RING = 2 * QTILE;
+    static constexpr uint32_t CTRL = RING + STAGES * 2 * BLOCK;
     static constexpr uint32_t SMEM = CTRL + 512;
-    static constexpr bool OWN_P = DP == 64;
-    // TMEM columns of tile t's scores, weights and outputs
-    static __device__ __forceinline__ uint32_t s_col(int t) { return t * 128; }
-    static __device__ __forceinline__ uint32_t p_col(int t) { return OWN_P ? 384 + t * 64 : t * 128; }
-    static __device__ __forceinline__ uint32_t o_col(int t) { return 256 + t * DP; }
+    static constexpr uint32_t PB = DP == 64 ? 1 : 2;         // buffers of weights of a tile
+    static constexpr uint32_t TILE_COLS = KEYS + PB * (KEYS / 2);
+    // TMEM columns of tile t's scores, of its weights of block n, and of its outputs
+    static __device__ __forceinline__ uint32_t s_col(int t) { return t * TILE_COLS; }
+    static __device__ __forceinline__ uint32_t p_col(int t, uint32_t n) { return t * TILE_COLS + KEYS + n % PB * (KEYS / 2); }
+    static __device__ __forceinline__ uint32_t o_col(int t) { return 2 * TILE_COLS + t * DP; }
+    static_assert(2 * TILE_COLS + 2 * DP == 512, "all of TMEM");
 };
 
+// With two buffers of weights a warp of a group may be a block ahead of the
+// others (never two: the scores after next wait until all have read the next
+// ones), so each has a barrier; and that a block's scores are there says, by
+// the order of the issuer's commits, that P V of two blocks before is done.
+// With one buffer a group waits for P V of the block before.
 struct WtCtrl {
-    uint64_t q_full, q_empty, kv_full[8], kv_empty[8], s_full[2], p_full[2], pv_done[2], o_empty[2], done;
+    uint64_t q_full[2], q_empty[2], kv_full[5], kv_empty[5], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2], done;
     uint32_t tmem_base;
 };
 static_assert(sizeof(WtCtrl) <= 512, "control block");
 
-// A unit: two tiles of 128 rows from i0, the blocks of keys that they see.
+// A unit as the role of tile t sees it: two tiles of 128 rows from i0, the
+// blocks of keys that either sees (first .. hi, next() from one to the next)
+// and those that this tile does.
 struct WtUnit {
-    int z, h, n, i0, sink_blocks, hi;
-    int lo[2];  // the first block of the tile's window
-    __device__ __forceinline__ bool alive(int t) const { return i0 + 128 * t < n; }
-    __device__ __forceinline__ int diag(int t) const { return i0 / WT_BLOCK + t; }
-    // whether tile t sees any key of block b
-    __device__ __forceinline__ bool takes(int t, int b) const {
-        return alive(t) && b <= diag(t) && (b >= lo[t] || b < sink_blocks);
-    }
-    __device__ __forceinline__ int first() const { return sink_blocks > 0 ? 0 : lo[0]; }
-    __device__ __forceinline__ int next(int b) const { return b + 1 < sink_blocks || b + 1 >= lo[0] ? b + 1 : lo[0]; }
+    int z, h, n, i0, sink_blocks, lo0, hi;
+    int lo, last;  // the first block of this tile's window, and its last (-1: a tile behind the sequence)
+    bool any, both;  // whether the sequence reaches the first tile, and the second
+    __device__ __forceinline__ bool takes(int b) const { return b <= last && (b >= lo || b < sink_blocks); }
+    __device__ __forceinline__ int first() const { return sink_blocks > 0 ? 0 : lo0; }
+    __device__ __forceinline__ int next(int b) const { return b + 1 < sink_blocks || b + 1 >= lo0 ? b + 1 : lo0; }
 };
 
-__device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int64_t u, int pairs) {
+template <int KEYS>
+__device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int64_t u, int pairs, int t) {
     WtUnit x;
     const int64_t zh_count = (int64_t)a.Z * a.H;
     const int pair = pairs - 1 - (int)(u / zh_count);
@@ -369,14 +413,22 @@ __device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int64_t u, int pa
     x.h = (int)(zh % a.H);
     x.n = length_of(a, x.z);
     x.i0 = pair * 256;
-    x.sink_blocks = (a.sinks + WT_BLOCK - 1) / WT_BLOCK;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int w = x.i0 + 128 * t - a.window + 1;
-        x.lo[t] = w > 0 ? w / WT_BLOCK : 0;
-    }
-    x.hi = x.diag(x.alive(1) ? 1 : 0);
+    x.any = x.i0 < x.n;
+    x.both = x.i0 + 128 < x.n;
+    x.sink_blocks = (a.sinks + KEYS - 1) / KEYS;
+    const int w0 = x.i0 - a.window + 1, w = w0 + 128 * t;
+    x.lo0 = w0 > 0 ? w0 / KEYS : 0;
+    x.lo = w > 0 ? w / KEYS : 0;
+    const int end = x.i0 + 256 < x.n ? x.i0 + 256 : x.n, mine = x.i0 + 128 * (t + 1);
+    x.hi = (end - 1) / KEYS;
+    x.last = (t ? x.both : x.any) ? ((mine < x.n ? mine : x.n) - 1) / KEYS : -1;
     return x;
+}
+
+// The i-th unit of a CTA: rows of gridDim.x units taken there and back, so
+// that the shorter units of a row go to the CTAs that had the longer ones.
+__device__ __forceinline__ int64_t wt_order(int64_t i) {
+    return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 // Bits 0 .. x of a word.
@@ -388,8 +440,51 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, int i, int n,
     return bits_upto(last - jc) & (~bits_upto(i - a.window - jc) | bits_upto(a.sinks - 1 - jc));
 }
 
+// Whether a phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// MMAs and commits issued by one elected lane of a converged warp, always the
+// same one.  The warp walks its blocks together, so that addresses and
+// descriptors are uniform values: a role entered by lane 0 alone had each
+// operand moved over for each instruction, 70 clocks an MMA.
+__device__ __forceinline__ void umma_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_ts_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+        : "memory");
 }
 
 template <int DP>
@@ -401,23 +496,25 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // shared byte; the swizzled tiles need it 1024-aligned, which is checked.
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
-        if (threadIdx.x == 0) atomicCAS(&g_zg_tc_error, 0u, 109u);
+        if (threadIdx.x == 0) atomicCAS(&g_zg_tc_error, 0u, 110u);
         return;
     }
     WtCtrl& c = *reinterpret_cast<WtCtrl*>(smem + W::CTRL);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
-        mbar_init(&c.q_full, 1);
-        mbar_init(&c.q_empty, 1);
-        mbar_init(&c.done, 1);
+        mbar_init(&c.done, 2);  // both issuers
         for (int i = 0; i < W::STAGES; ++i) {
             mbar_init(&c.kv_full[i], 1);
-            mbar_init(&c.kv_empty[i], 1);
+            mbar_init(&c.kv_empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
+            mbar_init(&c.q_full[t], 1);
+            mbar_init(&c.q_empty[t], 1);
             mbar_init(&c.s_full[t], 1);
-            mbar_init(&c.p_full[t], 128);
+            for (int i = 0; i < 2; ++i) mbar_init(&c.p_full[t][i], 128);
+            mbar_init(&c.s_read[t], 128);
             mbar_init(&c.pv_done[t], 1);
+            mbar_init(&c.o_full[t], 1);
             mbar_init(&c.o_empty[t], 128);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -428,136 +525,141 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tc_fence_after();
     const uint32_t tmem = c.tmem_base;
 
+    // A softmax thread holds a block's scores: the launch's 384 x 168
+    // registers are shared out as 128 x 72 and 256 x 216.
+    if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t slot = 0, nq = 0, issued = 0;  // loads issued; a stage's parity follows from the count
+            // blocks and query tiles loaded; a stage's parity follows from the count
+            uint32_t nk = 0, nq[2] = {0, 0};
             bool ok = true;
-            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const WtUnit x = wt_unit(a, u, pairs);
-                if (!x.alive(0)) continue;
-                const int kh = x.h / a.G, tiles = x.alive(1) ? 2 : 1;
-                if (!(ok = mbar_wait(&c.q_empty, (nq & 1) ^ 1, 101))) break;
-                mbar_expect_tx(&c.q_full, tiles * W::TILE);
-                for (int t = 0; t < tiles; ++t)
+            for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
+                const int64_t u = wt_order(it);
+                if (u >= units) continue;
+                const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, 0);
+                if (!x.any) continue;
+                const int kh = x.h / a.G;
+                auto queries = [&](int t) {
+                    if (!mbar_wait(&c.q_empty[t], (nq[t] & 1) ^ 1, 101)) return false;
+                    mbar_expect_tx(&c.q_full[t], W::QTILE);
                     for (int d = 0; d < DP / 64; ++d)
-                        tma_load_4d(smem + t * W::TILE + d * 16384, &tmQ, &c.q_full, 64 * d, x.h, x.i0 + 128 * t, x.z);
-                ++nq;
-                for (int b = x.first(); ok && b <= x.hi; b = x.next(b))
-                    for (int v = 0; v < 2; ++v, ++slot) {
-                        const uint32_t st = slot % W::STAGES;
-                        if (!(ok = mbar_wait(&c.kv_empty[st], ((slot / W::STAGES) & 1) ^ 1, 102))) break;
-                        mbar_expect_tx(&c.kv_full[st], W::TILE);
-                        for (int d = 0; d < DP / 64; ++d)
-                            tma_load_4d(smem + W::RING + st * W::TILE + d * 16384, v ? &tmV : &tmK, &c.kv_full[st], 64 * d,
-                                        kh, b * WT_BLOCK, x.z);
-                        issued = slot + 1;
-                    }
-            }
-            // loads still in flight (only after an abort) land before the CTA exits
-            for (uint32_t s = issued > W::STAGES ? issued - W::STAGES : 0; s < issued; ++s)
-                for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.kv_full[s % W::STAGES], (s / W::STAGES) & 1); ++i) {
-                }
-            if (nq)
-                for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.q_full, (nq - 1) & 1); ++i) {
-                }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc_s = idesc_bf16(128, 128, 0), idesc_o = idesc_bf16(128, DP, 1);
-            uint32_t slot = 0, nq = 0, ns[2] = {0, 0}, npv[2] = {0, 0}, nu[2] = {0, 0};
-            bool ok = true;
-            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const WtUnit x = wt_unit(a, u, pairs);
-                if (!x.alive(0)) continue;
-                if (!(ok = mbar_wait(&c.q_full, nq & 1, 103))) break;
-                ++nq;
-                bool pending[2] = {false, false}, started[2] = {false, false};
-                // S of tile t from the key block in slot sk
-                auto scores = [&](int t, uint32_t sk) {
-                    const uint32_t qa = smem_u32(smem + t * W::TILE), ka = smem_u32(smem + W::RING + sk % W::STAGES * W::TILE);
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k)
-                        umma_bf16(tmem + W::s_col(t), smem_desc(qa + (k / 4) * 16384 + (k % 4) * 32, 16, 1024),
-                                  smem_desc(ka + (k / 4) * 16384 + (k % 4) * 32, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
-                    umma_commit(&c.s_full[t]);
-                    ++ns[t];
-                };
-                // O of tile t += its weights times the value block in slot sv
-                auto outputs = [&](int t, uint32_t sv) {
-                    const uint32_t va = smem_u32(smem + W::RING + sv % W::STAGES * W::TILE);
-#pragma unroll
-                    for (int k = 0; k < WT_BLOCK / 16; ++k)
-                        umma_bf16_ts(tmem + W::o_col(t), tmem + W::p_col(t) + k * 8, smem_desc(va + k * 2048, 16384, 1024),
-                                     idesc_o, started[t] || k > 0 ? 1u : 0u);
-                    umma_commit(&c.pv_done[t]);
-                    ++npv[t];
-                    started[t] = true;
-                    pending[t] = false;
-                };
-                // one step: the weights of the last block (if a tile has any) and the scores of block b (b < 0: none)
-                auto step = [&](int b, uint32_t sk) {
-                    bool v_ready = false;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        bool need = b >= 0 && x.takes(t, b);
-                        if (pending[t]) {
-                            if (!mbar_wait(&c.p_full[t], (ns[t] - 1) & 1, 104)) return false;
-                            tc_fence_after();
-                            if (W::OWN_P && need) {
-                                scores(t, sk);
-                                need = false;
-                            }
-                            if (!v_ready && !mbar_wait(&c.kv_full[(sk - 1) % W::STAGES], ((sk - 1) / W::STAGES) & 1, 105))
-                                return false;
-                            v_ready = true;
-                            if (!started[t]) {
-                                // the last unit's outputs have been read
-                                if (!mbar_wait(&c.o_empty[t], (nu[t] & 1) ^ 1, 106)) return false;
-                                ++nu[t];
-                            }
-                            tc_fence_after();
-                            outputs(t, sk - 1);
-                            if (W::OWN_P && b >= 0 && x.takes(t, b)) pending[t] = true;
-                        }
-                        if (need) {
-                            // P shares the scores' columns: it has been read
-                            if (!W::OWN_P && npv[t] > 0 && !mbar_wait(&c.pv_done[t], (npv[t] - 1) & 1, 107)) return false;
-                            scores(t, sk);
-                            pending[t] = true;
-                        }
-                    }
+                        tma_load_4d(smem + t * W::QTILE + d * 16384, &tmQ, &c.q_full[t], 64 * d, x.h, x.i0 + 128 * t, x.z);
+                    ++nq[t];
                     return true;
                 };
-                const uint32_t s0 = slot;
-                for (int b = x.first(); ok && b <= x.hi; b = x.next(b), slot += 2) {
-                    if (!(ok = mbar_wait(&c.kv_full[slot % W::STAGES], (slot / W::STAGES) & 1, 108))) break;
-                    tc_fence_after();
-                    if (!(ok = step(b, slot))) break;
-                    if (slot > s0) umma_commit(&c.kv_empty[(slot - 1) % W::STAGES]);
-                    umma_commit(&c.kv_empty[slot % W::STAGES]);
+                if (!(ok = queries(0))) break;
+                // The second tile's queries come two blocks later: the first tile
+                // may be that far into its unit while the second ends its last.
+                int ahead = x.both ? 2 : -1;
+                for (int b = x.first(); b <= x.hi; b = x.next(b), ++nk) {
+                    if (ahead >= 0 && ahead-- == 0 && !(ok = queries(1))) break;
+                    const uint32_t st = nk % W::STAGES;
+                    if (!(ok = mbar_wait(&c.kv_empty[st], ((nk / W::STAGES) & 1) ^ 1, 102))) break;
+                    mbar_expect_tx(&c.kv_full[st], 2 * W::BLOCK);
+                    for (int d = 0; d < DP / 64; ++d) {
+                        uint8_t* to = smem + W::RING + st * 2 * W::BLOCK + d * W::BOX;
+                        tma_load_4d(to, &tmK, &c.kv_full[st], 64 * d, kh, b * W::KEYS, x.z);
+                        tma_load_4d(to + W::BLOCK, &tmV, &c.kv_full[st], 64 * d, kh, b * W::KEYS, x.z);
+                    }
                 }
-                if (!ok) break;
-                umma_commit(&c.q_empty);
-                if (!(ok = step(-1, slot))) break;
-                umma_commit(&c.kv_empty[(slot - 1) % W::STAGES]);
+                if (ok && ahead >= 0) ok = queries(1);  // a unit of two blocks or fewer
             }
-            // every MMA this thread issued has completed before TMEM is freed
-            umma_commit(&c.done);
-            for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.done, 0); ++i) {
+            // loads still in flight (only after an abort) land before the CTA exits
+            for (uint32_t s = nk > W::STAGES ? nk - W::STAGES : 0; s < nk; ++s)
+                for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.kv_full[s % W::STAGES], (s / W::STAGES) & 1); ++i) {
+                }
+            for (int t = 0; t < 2; ++t)
+                if (nq[t])
+                    for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.q_full[t], (nq[t] - 1) & 1); ++i) {
+                    }
+        }
+    } else if (warp <= 2) {
+        // one MMA issuer per tile; both give every block back to the loader
+        const int t = warp - 1;
+        const uint32_t idesc_s = idesc_bf16(128, W::KEYS, 0), idesc_o = idesc_bf16(128, DP, 1);
+        const uint32_t qa = smem_u32(smem + t * W::QTILE), ring = smem_u32(smem + W::RING);
+        uint32_t nk = 0, ns = 0, npv = 0, nu = 0;  // blocks, and of this tile scores, outputs, units
+        bool ok = true;
+        for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
+            const int64_t u = wt_order(it);
+            if (u >= units) continue;
+            const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
+            if (!x.any) continue;
+            if (x.last >= 0 && !(ok = warp_wait(&c.q_full[t], nu & 1, 103))) break;
+            bool started = false;
+            bool pending = false;  // P V of the last scores is to come
+            uint32_t vstage = 0;   // with the values of this stage
+            int vblock = -1;       // and the number of their block
+            auto outputs = [&]() {
+                const uint32_t st = vstage;
+                if (!warp_wait(&c.p_full[t][npv & 1], (npv >> 1) & 1, 104)) return false;
+                // the last unit's outputs have been read
+                if (!started && !warp_wait(&c.o_empty[t], (nu & 1) ^ 1, 105)) return false;
+                tc_fence_after();
+                const uint32_t va = ring + st * 2 * W::BLOCK + W::BLOCK;
+#pragma unroll
+                for (int k = 0; k < W::KEYS / 16; ++k)
+                    umma_ts_elect(tmem + W::o_col(t), tmem + W::p_col(t, npv) + k * 8, smem_desc(va + k * 2048, W::BOX, 1024),
+                                  idesc_o, started || k > 0 ? 1u : 0u);
+                umma_commit_elect(&c.pv_done[t]);
+                if (vblock == x.last) umma_commit_elect(&c.o_full[t]);
+                umma_commit_elect(&c.kv_empty[st]);
+                ++npv;
+                started = true;
+                pending = false;
+                return true;
+            };
+            for (int b = x.first(); b <= x.hi; b = x.next(b), ++nk) {
+                const uint32_t st = nk % W::STAGES, parity = (nk / W::STAGES) & 1;
+                if (!x.takes(b)) {
+                    if (pending) ok = outputs();
+                    // a block that is the other tile's alone is given back once it is here
+                    if (!ok || !(ok = warp_wait(&c.kv_full[st], parity, 106))) break;
+                    if (lane == 0) mbar_arrive(&c.kv_empty[st]);
+                    __syncwarp();
+                    continue;
+                }
+                if (!(ok = warp_wait(&c.kv_full[st], parity, 107))) break;
+                // the last scores are in their rows' registers
+                if (ns > 0 && !(ok = warp_wait(&c.s_read[t], (ns - 1) & 1, 108))) break;
+                tc_fence_after();
+                const uint32_t ka = ring + st * 2 * W::BLOCK;
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    umma_elect(tmem + W::s_col(t), smem_desc(qa + (k / 4) * 16384 + (k % 4) * 32, 16, 1024),
+                               smem_desc(ka + (k / 4) * W::BOX + (k % 4) * 32, 16, 1024), idesc_s, k > 0 ? 1u : 0u);
+                umma_commit_elect(&c.s_full[t]);
+                if (b == x.last) umma_commit_elect(&c.q_empty[t]);
+                ++ns;
+                if (pending && !(ok = outputs())) break;
+                pending = true;
+                vstage = st;
+                vblock = b;
             }
+            if (!ok || (pending && !(ok = outputs()))) break;
+            if (started) ++nu;
+        }
+        // every MMA this thread issued has completed before TMEM is freed
+        umma_commit_elect(&c.done);
+        for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&c.done, 0); ++i) {
         }
     } else if (warp >= 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int t = (warp - 4) / 4, quad = warp % 4;
         const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
-        const uint32_t sc = trow + W::s_col(t), pc = trow + W::p_col(t), oc = trow + W::o_col(t);
+        const uint32_t oc = trow + W::o_col(t);
         const int64_t ldo = (int64_t)a.H * a.D;
-        uint32_t nb = 0;  // blocks of this tile so far
+        const float2 one2 = make_float2(1.f, 1.f), scale2 = make_float2(a.scale, a.scale);
+        uint32_t nb = 0, nu = 0;  // blocks and units of this tile so far
+        bool s_ready = false;     // the next scores have been seen to be there
         bool ok = true;
-        for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const WtUnit x = wt_unit(a, u, pairs);
-            const int row0 = x.i0 + 128 * t, i = row0 + 32 * quad + lane;
+        for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
+            const int64_t u = wt_order(it);
+            if (u >= units) continue;
+            const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
+            const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;  // the warp's first row, this thread's
             __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
-            if (!x.alive(t)) {
+            if (x.last < 0) {
                 if (i < a.S) {
                     const uint32_t w = x.n < 0 ? 0x7fff7fffu : 0u;
                     for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4*>(o + d) = make_uint4(w, w, w, w);
@@ -568,90 +670,139 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             bool first = true;
             for (int b = x.first(); b <= x.hi; b = x.next(b)) {
-                if (!x.takes(t, b)) continue;
-                if (!(ok = warp_wait(&c.s_full[t], nb & 1, 110))) break;
+                if (!x.takes(b)) continue;
+                const uint32_t sc = trow + W::s_col(t), pc = trow + W::p_col(t, nb);
+                if (!s_ready && !(ok = warp_wait(&c.s_full[t], nb & 1, 111))) break;
                 tc_fence_after();
-                const int j0 = b * WT_BLOCK;
-                const bool edge = j0 + WT_BLOCK - 1 > row0 ||
-                                  (j0 <= row0 + 127 - a.window && j0 + WT_BLOCK > a.sinks);
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                {
-                    uint32_t r[2][32];
-                    tmem_ld32_nowait(sc, r[0]);
-#pragma unroll 2
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_wait_ld32(r[q & 1]);
-                        if (q < 3) tmem_ld32_nowait(sc + 32 * (q + 1), r[(q + 1) & 1]);
-                        if (edge) {
-                            const uint32_t on = seen_bits(a, i, x.n, j0 + 32 * q);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                mx4[e % 4] = fmaxf(mx4[e % 4], on >> e & 1 ? __uint_as_float(r[q & 1][e]) : -INFINITY);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) mx4[e % 4] = fmaxf(mx4[e % 4], __uint_as_float(r[q & 1][e]));
-                        }
+                const int j0 = b * W::KEYS;
+                // The maximum m is moved to the row's (mx, scaled) where that is more
+                // than 2^8 above; false when a wait ran out.
+                auto settle = [&](float mx, bool pv_seen) {
+                    // P V of the block before has read the weights' buffer and added to O
+                    const bool all_seen = __all_sync(0xffffffffu, pv_seen);
+                    if (W::PB == 1 && !first) {
+                        if (!all_seen && !warp_wait(&c.pv_done[t], (nb - 1) & 1, 112)) return false;
+                        tc_fence_after();
                     }
-                }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale;
-                if (W::OWN_P && !first) {
-                    // P V of the block before has read the weights and written O
-                    if (!(ok = warp_wait(&c.pv_done[t], (nb - 1) & 1, 111))) break;
-                    tc_fence_after();
-                }
-                if (__any_sync(0xffffffffu, mx > m + 8.f || (m == -INFINITY && mx > m))) {
-                    const float n = fmaxf(m, mx), f = exp2_fast(m - (n == -INFINITY ? 0.f : n));
+                    if (!__any_sync(0xffffffffu, !(mx <= m + 8.f))) return true;
+                    const float n = fmaxf(m, mx);
+                    float f = exp2_fast(m - (n == -INFINITY ? 0.f : n));
+                    // a score that is NaN or infinite: the row is formed again at the end
+                    if (!(mx < INFINITY)) f = __int_as_float(0x7fffffff);
                     m = n;
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         sum[e].x *= f;
                         sum[e].y *= f;
                     }
-                    if (!first) {
-#pragma unroll 1
-                        for (int d = 0; d < DP; d += 32) {
-                            float v[32];
-                            tmem_ld32(oc + d, v);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] *= f;
-                            __syncwarp();
-                            tmem_st32(oc + d, v);
-                        }
+                    if (first) return true;
+                    if (W::PB == 2) {
+                        if (!all_seen && !warp_wait(&c.pv_done[t], (nb - 1) & 1, 112)) return false;
+                        tc_fence_after();
                     }
-                }
-                first = false;
-                const float base = m == -INFINITY ? 0.f : m;
-                {
-                    uint32_t r[2][32];
-                    tmem_ld32_nowait(sc, r[0]);
-#pragma unroll 2
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_wait_ld32(r[q & 1]);
-                        if (q < 3) tmem_ld32_nowait(sc + 32 * (q + 1), r[(q + 1) & 1]);
-                        const uint32_t on = edge ? seen_bits(a, i, x.n, j0 + 32 * q) : 0xffffffffu;
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 32) {
+                        float v[32];
+                        tmem_ld32(oc + d, v);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] *= f;
+                        __syncwarp();
+                        tmem_st32(oc + d, v);
+                    }
+                    return true;
+                };
+                if (j0 + W::KEYS - 1 <= row0 && (j0 > row0 + 31 - a.window || j0 + W::KEYS <= a.sinks)) {
+                    // every row of this warp sees all of the block: its scores stay in registers
+                    uint32_t r[W::KEYS / 32][32];
+#pragma unroll
+                    for (int q = 0; q < W::KEYS / 32; ++q) tmem_ld32_nowait(sc + 32 * q, r[q]);
+#pragma unroll
+                    for (int q = 0; q < W::KEYS / 32; ++q) tmem_wait_ld32(r[q]);
+                    tc_fence_before();
+                    mbar_arrive(&c.s_read[t]);
+                    // asked now, used behind the maximum: an answer takes some 250 clocks
+                    // behind the exponentials in the same queue
+                    const bool pv_seen = !first && mbar_test_wait(&c.pv_done[t], (nb - 1) & 1);
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int q = 0; q < W::KEYS / 32; q += 2)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            mx4[e % 4] = max_nan(mx4[e % 4], max_nan(__uint_as_float(r[q][e]), __uint_as_float(r[q + 1][e])));
+                    const float mx = max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3])) * a.scale;
+                    if (!(ok = settle(mx, pv_seen))) break;
+                    const float2 base2 = make_float2(-m, -m);
+#pragma unroll
+                    for (int q = 0; q < W::KEYS / 32; ++q) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            float p0 = exp2_fast(fmaf(__uint_as_float(r[q & 1][2 * e]), a.scale, -base));
-                            float p1 = exp2_fast(fmaf(__uint_as_float(r[q & 1][2 * e + 1]), a.scale, -base));
-                            if (edge) {
-                                p0 = on >> (2 * e) & 1 ? p0 : 0.f;
-                                p1 = on >> (2 * e + 1) & 1 ? p1 : 0.f;
-                            }
-                            sum[e & 1] = ffma2_tc(make_float2(p0, p1), make_float2(1.f, 1.f), sum[e & 1]);
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-                            pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+                            const float2 y = ffma2_tc(
+                                make_float2(__uint_as_float(r[q][2 * e]), __uint_as_float(r[q][2 * e + 1])), scale2, base2);
+                            const float2 w = e % WT_POLY == WT_POLY - 1 ? exp2_fma(y)
+                                                                        : make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            sum[e & 1] = ffma2_tc(w, one2, sum[e & 1]);
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(w.x, w.y);
+                            pk[e] = *reinterpret_cast<const uint32_t*>(&v);
                         }
                         tmem_st16u(pc + 16 * q, pk);
                     }
+                } else {
+                    // The mask cuts the block: 32 keys at a time, read twice, those that no
+                    // row of the warp sees passed over.  Little code, as it runs seldom: the
+                    // two softmax groups' instructions share a cache.
+                    auto seen = [&](int jc) { return jc <= row0 + 31 && (jc + 31 > row0 - a.window || jc < a.sinks); };
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int q = 0; q < W::KEYS / 32; ++q) {
+                        const int jc = j0 + 32 * q;
+                        if (!seen(jc)) continue;
+                        float v[32];
+                        tmem_ld32(sc + 32 * q, v);
+                        const uint32_t on = seen_bits(a, i, x.n, jc);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) mx = max_nan(mx, on >> e & 1 ? v[e] : -INFINITY);
+                    }
+                    const bool pv_seen = !first && mbar_test_wait(&c.pv_done[t], (nb - 1) & 1);
+                    if (!(ok = settle(mx * a.scale, pv_seen))) break;
+                    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                    for (int q = 0; q < W::KEYS / 32; ++q) {
+                        const int jc = j0 + 32 * q;
+                        uint32_t pk[16];
+                        if (seen(jc)) {
+                            float v[32];
+                            tmem_ld32(sc + 32 * q, v);
+                            const uint32_t on = seen_bits(a, i, x.n, jc);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = on >> e & 1 ? exp2_fast(fmaf(v[e], a.scale, -base)) : 0.f;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                sum[e & 1] = ffma2_tc(make_float2(v[2 * e], v[2 * e + 1]), one2, sum[e & 1]);
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                                pk[e] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+                        }
+                        tmem_st16u(pc + 16 * q, pk);
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&c.s_read[t]);
                 }
+                // whether the next scores are there, asked while the stores go
+                const bool next_ready = mbar_test_wait(&c.s_full[t], (nb + 1) & 1);
+                first = false;
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&c.p_full[t]);
+                mbar_arrive(&c.p_full[t][nb & 1]);
                 ++nb;
+                s_ready = __all_sync(0xffffffffu, next_ready);
             }
             if (!ok) break;
-            if (!(ok = warp_wait(&c.pv_done[t], (nb - 1) & 1, 112))) break;
+            if (!(ok = warp_wait(&c.o_full[t], nu & 1, 113))) break;
+            ++nu;
             tc_fence_after();
             const float inv = 1.f / ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             const bool in = i < x.n;
@@ -677,7 +828,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             mbar_arrive(&c.o_empty[t]);
             for (uint32_t rows = __ballot_sync(0xffffffffu, !fine); rows; rows &= rows - 1) {
                 __syncwarp();  // the row's first values are written before these
-                window_row<__nv_bfloat16>(a, x.z, row0 + 32 * quad + __ffs(rows) - 1, x.h);
+                window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
             }
         }
     }
@@ -693,13 +844,13 @@ template <int DP>
 int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
     using W = WtShape<DP>;
     CUtensorMap tq, tk, tv;
-    const uint32_t box[4] = {64, 1, 128, 1};
-    auto map = [&](CUtensorMap* m, const void* p, int heads, int64_t ld) {
+    auto map = [&](CUtensorMap* m, const void* p, int heads, int64_t ld, uint32_t rows) {
+        const uint32_t box[4] = {64, 1, rows, 1};
         const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)heads, (uint64_t)a.S, (uint64_t)a.Z};
         const uint64_t strides[3] = {(uint64_t)a.D * 2, (uint64_t)ld * 2, (uint64_t)a.S * ld * 2};
         return zg::tensor_map_bf16(m, p, 4, dims, strides, box, true);
     };
-    if (!map(&tq, a.q, a.H, a.ldq) || !map(&tk, a.k, a.K, a.ldk) || !map(&tv, a.v, a.K, a.ldv))
+    if (!map(&tq, a.q, a.H, a.ldq, 128) || !map(&tk, a.k, a.K, a.ldk, W::KEYS) || !map(&tv, a.v, a.K, a.ldv, W::KEYS))
         return zg::fail(ZG_ERR_CUDA, "zg_window_attention: tensor maps");
     if (cudaFuncSetAttribute(window_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM) !=
         cudaSuccess)
@@ -718,8 +869,8 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
 
 namespace zg {
 
-// Timed-out waits of the tensor-core kernel (codes 101-108, 110-112) or its
-// shared memory not 1024-aligned (109); 0 = none.
+// Timed-out waits of the tensor-core kernel (codes 101-109, 111-113) or its
+// shared memory not 1024-aligned (110); 0 = none.
 int window_error_word(int clear) { return ptx_error_word(clear); }
 
 }  // namespace zg

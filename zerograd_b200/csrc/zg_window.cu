@@ -8,8 +8,6 @@
 // zeros.  4 D flops for each visible (i, j) and head.
 #include <math.h>
 
-#include <type_traits>
-
 #include "zg_ptx.cuh"
 #include "zg_tc.cuh"
 
@@ -36,28 +34,6 @@ __device__ __forceinline__ float max_nan(float x, float y) {
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
     return m;
-}
-
-// 2^y of two values on the FMA pipe, for y in [-120, 120]: y = n + f with n the
-// nearest whole number (by adding and taking off 1.5 * 2^23), 2^f by a
-// polynomial of degree 4 fitted to the relative error on [-1/2, 1/2] (2.7e-6,
-// 2^-18.5), n added to the exponent.  The special-function pipe has 16 results a
-// clock and SM, an eighth of the FMA pipe's rate: part of a row's weights
-// are formed here.
-__device__ __forceinline__ float2 exp2_fma(float2 y) {
-    const float2 one = make_float2(1.f, 1.f), magic = make_float2(12582912.f, 12582912.f);
-    y.x = fmaxf(y.x, -120.f);
-    y.y = fmaxf(y.y, -120.f);
-    const float2 t = ffma2_tc(y, one, magic);
-    const float2 n = ffma2_tc(t, one, make_float2(-12582912.f, -12582912.f));
-    const float2 f = ffma2_tc(n, make_float2(-1.f, -1.f), y);
-    float2 p = make_float2(0.00957010127604f, 0.00957010127604f);
-    p = ffma2_tc(p, f, make_float2(0.05591785907745f, 0.05591785907745f));
-    p = ffma2_tc(p, f, make_float2(0.24024744331837f, 0.24024744331837f));
-    p = ffma2_tc(p, f, make_float2(0.69312179088593f, 0.69312179088593f));
-    p = ffma2_tc(p, f, make_float2(0.99999928474426f, 0.99999928474426f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // The length of sequence z; -1 when it is not one of [0, S].
@@ -358,7 +334,6 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 // ever touched.
 // ---------------------------------------------------------------------------
 constexpr int WT_THREADS = 384;
-constexpr int WT_POLY = 3;   // every third pair of weights comes from the polynomial
 
 template <int DP>
 struct WtShape {
@@ -711,8 +686,20 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     }
                     return true;
                 };
-                if (j0 + W::KEYS - 1 <= row0 && (j0 > row0 + 31 - a.window || j0 + W::KEYS <= a.sinks)) {
-                    // every row of this warp sees all of the block: its scores stay in registers
+                // whether every row of this warp sees all of the block, or any row any of keys jc ..
+                const bool full = j0 + W::KEYS - 1 <= row0 && (j0 > row0 + 31 - a.window || j0 + W::KEYS <= a.sinks);
+                auto seen = [&](int jc, int keys) {
+                    return jc <= row0 + 31 && (jc + keys - 1 > row0 - a.window || jc < a.sinks);
+                };
+                if (W::KEYS == 64 && !seen(j0, 64)) {
+                    mbar_arrive(&c.s_read[t]);
+                    uint32_t zero[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) zero[e] = 0u;
+                    tmem_st16u(pc, zero);
+                    tmem_st16u(pc + 16, zero);
+                } else if (full || W::KEYS == 64) {
+                    // a row's scores stay in its thread's registers
                     uint32_t r[W::KEYS / 32][32];
 #pragma unroll
                     for (int q = 0; q < W::KEYS / 32; ++q) tmem_ld32_nowait(sc + 32 * q, r[q]);
@@ -723,6 +710,15 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     // asked now, used behind the maximum: an answer takes some 250 clocks
                     // behind the exponentials in the same queue
                     const bool pv_seen = !first && mbar_test_wait(&c.pv_done[t], (nb - 1) & 1);
+                    if (W::KEYS == 64 && !full) {
+                        // keys that the row does not see score -inf
+#pragma unroll
+                        for (int q = 0; q < W::KEYS / 32; ++q) {
+                            const uint32_t on = seen_bits(a, i, x.n, j0 + 32 * q);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) r[q][e] = on >> e & 1 ? r[q][e] : 0xff800000u;
+                        }
+                    }
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int q = 0; q < W::KEYS / 32; q += 2)
@@ -731,7 +727,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             mx4[e % 4] = max_nan(mx4[e % 4], max_nan(__uint_as_float(r[q][e]), __uint_as_float(r[q + 1][e])));
                     const float mx = max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3])) * a.scale;
                     if (!(ok = settle(mx, pv_seen))) break;
-                    const float2 base2 = make_float2(-m, -m);
+                    const float base = m == -INFINITY ? 0.f : m;
+                    const float2 base2 = make_float2(-base, -base);
 #pragma unroll
                     for (int q = 0; q < W::KEYS / 32; ++q) {
                         uint32_t pk[16];
@@ -739,8 +736,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         for (int e = 0; e < 16; ++e) {
                             const float2 y = ffma2_tc(
                                 make_float2(__uint_as_float(r[q][2 * e]), __uint_as_float(r[q][2 * e + 1])), scale2, base2);
-                            const float2 w = e % WT_POLY == WT_POLY - 1 ? exp2_fma(y)
-                                                                        : make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            const float2 w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
                             sum[e & 1] = ffma2_tc(w, one2, sum[e & 1]);
                             const __nv_bfloat162 v = __floats2bfloat162_rn(w.x, w.y);
                             pk[e] = *reinterpret_cast<const uint32_t*>(&v);
@@ -748,15 +744,15 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         tmem_st16u(pc + 16 * q, pk);
                     }
                 } else {
-                    // The mask cuts the block: 32 keys at a time, read twice, those that no
-                    // row of the warp sees passed over.  Little code, as it runs seldom: the
-                    // two softmax groups' instructions share a cache.
-                    auto seen = [&](int jc) { return jc <= row0 + 31 && (jc + 31 > row0 - a.window || jc < a.sinks); };
+                    // The mask cuts a block of 128: 32 keys at a time, read twice, those that no
+                    // row of the warp sees passed over.  (With the mask in the path above D = 64
+                    // was 10% slower; two paths of 128 registers each spill.  At D = 128, with
+                    // 64, one path with the mask in it is 7% faster under a window of 1024.)
                     float mx = -INFINITY;
 #pragma unroll 1
                     for (int q = 0; q < W::KEYS / 32; ++q) {
                         const int jc = j0 + 32 * q;
-                        if (!seen(jc)) continue;
+                        if (!seen(jc, 32)) continue;
                         float v[32];
                         tmem_ld32(sc + 32 * q, v);
                         const uint32_t on = seen_bits(a, i, x.n, jc);
@@ -770,7 +766,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     for (int q = 0; q < W::KEYS / 32; ++q) {
                         const int jc = j0 + 32 * q;
                         uint32_t pk[16];
-                        if (seen(jc)) {
+                        if (seen(jc, 32)) {
                             float v[32];
                             tmem_ld32(sc + 32 * q, v);
                             const uint32_t on = seen_bits(a, i, x.n, jc);

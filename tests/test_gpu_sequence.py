@@ -362,3 +362,19 @@ def test_under_vmap(cuda):
     with pytest.raises(NotImplementedError):
         torch.func.vmap(lambda c: zg.paged_attention(x[0, :, 0, :H], c, c, table[0], lengths))(
             torch.stack([kp, kp]))
+
+
+def test_views_of_a_fused_projection_are_not_copied(cuda):
+    """Rows with a pitch, also of single tokens and through a transposed batch
+    of length one, reach the kernels as they are; other strides are copied."""
+    from zerograd_b200 import _sequence
+
+    x = torch.arange(4 * 6 * 5 * 8, device=cuda, dtype=F32).reshape(4, 6, 5, 8)
+    for t, pitch in ((x[:, :, :2], 40), (x[:, :1, :2], 240), (x[:1, :, 1:3], 40), (x[0, 0, 1:3], 16), (x[:, 2:3, 4:], 240),
+                     (x.reshape(24, 5, 8)[:, :3], 40), (x[::2, :, :2], None), (x[:, ::2, :2], 80),
+                     (x[:, :, ::2], None), (x[..., :4], None), (x[:1].expand(3, 6, 5, 8)[:, :, :2], None),
+                     (x.transpose(0, 1), None), (x[:, :, 1:2, :3], 40)):
+        y, ld = _sequence._pitched(t)
+        assert (y.data_ptr() == t.data_ptr()) == (pitch is not None), tuple(t.shape)
+        assert ld == (pitch if pitch is not None else t.shape[-2] * t.shape[-1])
+        assert torch.equal(y, t)

@@ -27,19 +27,20 @@ import math
 import torch
 
 from . import _lib as L
-from ._block import _as, _row_pitch
+from ._block import _as
 from ._ops import _NS, _movedim0
 
 _INT_MAX = 2 ** 31 - 1
 _POSITION_CODES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _no_transform = torch._C._functorch.peek_interpreter_stack
+_no_mode = torch._C._len_torch_dispatch_stack
 
 
 def _plain_call(*ts) -> bool:
     """True when a call needs none of what the dispatcher adds (vmap, an
     autograd error, a tracing mode): the op is then launched without it,
     which a single token's call notices (about 20 us of host time)."""
-    if _no_transform() is not None or torch._C._len_torch_dispatch_stack() or torch.compiler.is_compiling():
+    if _no_transform() is not None or _no_mode() or torch.compiler.is_compiling():
         return False
     grad = torch.is_grad_enabled()
     for t in ts:
@@ -49,9 +50,10 @@ def _plain_call(*ts) -> bool:
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
-    """The entry point on `dev`'s current stream (the last argument), with
+    """The entry point on `dev`'s current stream (its last argument), with
     `dev` current while it is called."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
         L.call(name, *args, L.stream_ptr(dev))
     else:
         with torch.cuda.device(dev):
@@ -62,20 +64,35 @@ def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
     """Whole numbers as contiguous int32; wider ones that int32 cannot hold
     become -1 or the largest, which the kernels refuse as they would the
     number itself."""
-    if t.dtype == torch.int32:
-        return t.contiguous()
-    if t.dtype != torch.int64:
+    if t.dtype is torch.int32:
+        return t if t.is_contiguous() else t.contiguous()
+    if t.dtype is not torch.int64:
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
     return t.clamp(-1, _INT_MAX).to(torch.int32).contiguous()
 
 
 def _pitched(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """`t` [..., S, H, D] with its row pitch, copied if its rows have none."""
-    ld = _row_pitch(t)
-    if ld is None:
-        t = t.contiguous()
-        ld = int(t.shape[-2]) * int(t.shape[-1])
-    return t, ld
+    """`t` [..., heads, D] with the elements between its consecutive rows (all
+    leading axes as one; heads contiguous, as in a view of a fused
+    projection), copied if its rows lie otherwise."""
+    shape, stride = t.shape, t.stride()
+    H, D = shape[-2], shape[-1]
+    ld, rows = 0, 1
+    if (stride[-1] == 1 or D == 1) and (stride[-2] == D or H == 1):
+        for d in range(len(shape) - 3, -1, -1):
+            n = shape[d]
+            if n != 1:
+                if rows == 1:
+                    ld = stride[d]
+                elif stride[d] != ld * rows:
+                    ld = -1
+                    break
+                rows *= n
+        if rows == 1:
+            return t, H * D
+        if ld >= H * D:
+            return t, ld
+    return t.contiguous(), H * D
 
 
 def _span(window: int | None, sinks: int) -> tuple[int, int]:
@@ -114,9 +131,9 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
     qo = torch.empty(q.shape, dtype=dt, device=dev)
     ko = torch.empty(k.shape, dtype=dt, device=dev)
     widths = (ctypes.c_int32 * len(axes))(*axes)
-    _call(dev, "zg_rotary", L.ptr(q), ldq, L.ptr(k), ldk, L.ptr(positions), _POSITION_CODES[positions.dtype],
+    _call(dev, "zg_rotary", q.data_ptr(), ldq, k.data_ptr(), ldk, positions.data_ptr(), _POSITION_CODES[positions.dtype],
           math.prod(tokens), math.prod(positions.shape[:-1]), H, K, D, len(axes), widths, base, int(interleaved),
-          int(joint), int(inverse), code, L.ptr(qo), L.ptr(ko))
+          int(joint), int(inverse), code, qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -190,8 +207,8 @@ def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
         lengths = _int32(lengths, "lengths")
     (q, ldq), (k, ldk), (v, ldv) = _pitched(q), _pitched(_as(k, dt)), _pitched(_as(v, dt))
     o = torch.empty(q.shape, dtype=dt, device=dev)
-    _call(dev, "zg_window_attention", L.ptr(q), ldq, L.ptr(k), ldk, L.ptr(v), ldv, L.ptr(lengths), Z, S, H, K, D,
-          window, sinks, code, L.ptr(o))
+    _call(dev, "zg_window_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, L.ptr(lengths), Z, S,
+          H, K, D, window, sinks, code, o.data_ptr())
     return o
 
 
@@ -269,9 +286,9 @@ def launch_append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.T
         counts = _int32(counts, "counts")
     (k, ldk), (v, ldv) = _pitched(k), _pitched(v)
     new = torch.empty(lead, dtype=torch.int32, device=dev)
-    _call(dev, "zg_append_pages", L.ptr(k_pages), L.ptr(v_pages), N, page, K, D, L.ptr(k), ldk, L.ptr(v), ldv,
-          math.prod(lead), int(k.shape[-3]), L.ptr(table), int(table.shape[-1]), L.ptr(had), L.ptr(counts),
-          L.dtype_code(k_pages.dtype), L.ptr(new))
+    _call(dev, "zg_append_pages", k_pages.data_ptr(), v_pages.data_ptr(), N, page, K, D, k.data_ptr(), ldk, v.data_ptr(), ldv,
+          math.prod(lead), int(k.shape[-3]), table.data_ptr(), int(table.shape[-1]), had.data_ptr(), L.ptr(counts),
+          L.dtype_code(k_pages.dtype), new.data_ptr())
     return new
 
 
@@ -344,8 +361,8 @@ def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         rows, ldq = rows.clone(memory_format=torch.contiguous_format), H * D
     nbytes = L.query("zg_paged_attention_workspace_size", B, H, K, D, M, page, window, sinks, code)
     ws = L.workspace(nbytes, dev) if nbytes else None
-    _call(dev, "zg_paged_attention", L.ptr(rows), ldq, L.ptr(k_pages), L.ptr(v_pages), N, page, L.ptr(table), M,
-          L.ptr(had), B, H, K, D, window, sinks, code, L.ptr(o), L.ptr(ws), nbytes)
+    _call(dev, "zg_paged_attention", rows.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), N, page, table.data_ptr(), M,
+          had.data_ptr(), B, H, K, D, window, sinks, code, o.data_ptr(), L.ptr(ws), nbytes)
     return o
 
 

@@ -204,12 +204,20 @@ extern "C" int zg_rotary(const void* q, int64_t ldq, const void* k, int64_t ldk,
     if (!positions || (H && (!q || !q_out)) || (K && (!k || !k_out)))
         return zg::fail(ZG_ERR_INVALID, "zg_rotary: null pointer");
     a.pairs = (int)(width / 2);
-    for (int i = 0, p = 0; i < A; ++i)
-        for (int j = 0; j < axes[i] / 2; ++j, ++p) {
-            const double e = joint ? (double)p / a.pairs : (double)j / (axes[i] / 2);
-            a.turns[p] = pow(base, -e) / 6.283185307179586476925286766559;
+    // base^(-j/n) by repeated products in the host's 64-bit mantissas: at most
+    // 127 roundings of 2^-64, below one of the doubles they end in
+    const long double start = 1.0L / 6.283185307179586476925286766559005768L;
+    long double f = start, step = powl((long double)base, -1.0L / a.pairs);
+    for (int i = 0, p = 0; i < A; ++i) {
+        if (!joint) {
+            f = start;
+            step = powl((long double)base, -2.0L / axes[i]);
+        }
+        for (int j = 0; j < axes[i] / 2; ++j, ++p, f *= step) {
+            a.turns[p] = (double)f;
             a.axis[p] = (uint8_t)i;
         }
+    }
     a.q = q; a.k = k; a.pos = positions; a.q_out = q_out; a.k_out = k_out;
     a.ldq = ldq; a.ldk = ldk; a.T = T; a.pos_rows = pos_rows;
     a.H = H; a.K = K; a.D = D; a.A = A; a.pos_type = pos_type; a.interleaved = interleaved != 0;

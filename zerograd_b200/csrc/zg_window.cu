@@ -8,6 +8,8 @@
 // zeros.  4 D flops for each visible (i, j) and head.
 #include <math.h>
 
+#include <type_traits>
+
 #include "zg_ptx.cuh"
 #include "zg_tc.cuh"
 
@@ -99,30 +101,37 @@ __device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h
 // ---------------------------------------------------------------------------
 // FMA path: float32, and bf16 shapes that the tensor cores do not take.
 //
-// A block has 64 query rows of one head and walks over the tiles of 64 keys
+// A block has 32 query rows of one head and walks over the tiles of 64 keys
 // that any of them sees, q, k, v and the weights in shared memory as float32.
-// 256 threads as 16 x 16: thread (ty, tx) has the scores of rows ty + 16 i
-// and keys tx + 16 j, and the outputs of the same rows in columns
-// 4 tx + 64 c.  Rows are DP + 4 floats apart, so that the 16-byte reads of
-// neighbouring rows fall into different banks.
+// 128 threads as 8 x 16: thread (ty, tx) has the scores of rows ty + 8 i
+// and keys tx + 16 j, and the outputs of the same rows in column pairs
+// 2 tx + 32 c.  Both products are in packed pairs (two FMAs an instruction):
+// of the scores the even and the odd columns' sums apart, of the outputs two
+// columns.  Rows are DP + 4 floats apart, so that the 16-byte reads of
+// neighbouring rows fall into different banks.  Float32 rows come by cp.async,
+// the next tile's keys under this one's second product and its values under
+// the next first one; others are converted on the way, a tile's words in
+// flight together.
 // ---------------------------------------------------------------------------
-constexpr int WF_M = 64, WF_N = 64, WF_THREADS = 256, WF_PP = WF_N + 4;
+constexpr int WF_M = 32, WF_N = 64, WF_THREADS = 128, WF_PP = WF_N + 4;
 
 template <int DP>
 constexpr size_t wf_smem() {
-    return (size_t)(3 * 64 * (DP + 4) + WF_M * WF_PP) * sizeof(float);
+    return (size_t)((WF_M + 2 * WF_N) * (DP + 4) + WF_M * WF_PP) * sizeof(float);
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(WF_THREADS) window_fma_kernel(const WindowArgs a, int q_tiles, int vec) {
-    constexpr int PITCH = DP + 4, NC = DP / 64;
+__global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) window_fma_kernel(const WindowArgs a, int q_tiles, int vec) {
+    constexpr int PITCH = DP + 4, NC = DP / 32;
     extern __shared__ __align__(16) float sm[];
-    float *qs = sm, *ks = qs + 64 * PITCH, *vs = ks + 64 * PITCH, *ps = vs + 64 * PITCH;
+    float *qs = sm, *ks = qs + WF_M * PITCH, *vs = ks + WF_N * PITCH, *ps = vs + WF_N * PITCH;
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    // the tiles that see the most keys first
-    const int qt = q_tiles - 1 - (int)(blockIdx.x % q_tiles);
-    const int64_t zh = blockIdx.x / q_tiles;
-    const int z = (int)(zh / a.H), h = (int)(zh % a.H), kh = h / a.G;
+    // the tiles that see the most keys first, of all heads: 2048 tokens of 8
+    // heads of 128 are 256 blocks of 1 to 32 tiles (head by head the SMs
+    // were busy for 61% of the time)
+    const int heads = a.Z * a.H;
+    const int qt = q_tiles - 1 - (int)(blockIdx.x / heads), zh = (int)(blockIdx.x % heads);
+    const int z = zh / a.H, h = zh % a.H, kh = h / a.G;
     const int n = length_of(a, z), i0 = qt * WF_M;
     T* o = static_cast<T*>(a.o) + ((int64_t)z * a.S * a.H + h) * a.D;
     const int64_t ldo = (int64_t)a.H * a.D;
@@ -137,74 +146,104 @@ __global__ void __launch_bounds__(WF_THREADS) window_fma_kernel(const WindowArgs
     const T* k = static_cast<const T*>(a.k) + (int64_t)z * a.S * a.ldk + (int64_t)kh * a.D;
     const T* v = static_cast<const T*>(a.v) + (int64_t)z * a.S * a.ldv + (int64_t)kh * a.D;
 
-    auto load = [&](float* dst, const T* src, int64_t ld, int r0) {  // 64 rows from r0, zeros past n and D
-        if (vec) {
-            for (int x = threadIdx.x; x < 64 * (DP / 4); x += WF_THREADS) {
-                const int r = x / (DP / 4), d = x % (DP / 4) * 4;
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r0 + r < n && d < a.D) {
-                    const T* p = src + (r0 + r) * ld + d;
-                    if constexpr (sizeof(T) == 4) {
-                        f = *reinterpret_cast<const float4*>(p);
-                    } else {
-                        const uint2 u = *reinterpret_cast<const uint2*>(p);
-                        f = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u),
-                                        __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-                    }
-                }
-                *reinterpret_cast<float4*>(dst + r * PITCH + d) = f;
+    // ROWS rows from r0, zeros past n and D
+    auto load = [&](auto rows, float* dst, const T* src, int64_t ld, int r0) {
+        constexpr int ROWS = decltype(rows)::value;
+        constexpr int WORDS = DP / 4, EACH = ROWS * WORDS / WF_THREADS;  // 16-byte words of a row, words of a thread
+        if (sizeof(T) == 4 && vec) {
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int x = threadIdx.x + e * WF_THREADS, r = x / WORDS, d = x % WORDS * 4;
+                const bool on = r0 + r < n && d < a.D;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * PITCH + d)),
+                             "l"(on ? src + (r0 + r) * ld + d : src), "r"(on ? 16 : 0)
+                             : "memory");
+            }
+        } else if (vec) {
+            uint2 u[EACH];
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int x = threadIdx.x + e * WF_THREADS, r = x / WORDS, d = x % WORDS * 4;
+                u[e] = r0 + r < n && d < a.D ? *reinterpret_cast<const uint2*>(src + (r0 + r) * ld + d) : make_uint2(0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const int x = threadIdx.x + e * WF_THREADS, r = x / WORDS, d = x % WORDS * 4;
+                *reinterpret_cast<float4*>(dst + r * PITCH + d) =
+                    make_float4(__uint_as_float(u[e].x << 16), __uint_as_float(u[e].x & 0xffff0000u),
+                                __uint_as_float(u[e].y << 16), __uint_as_float(u[e].y & 0xffff0000u));
             }
         } else {
-            for (int x = threadIdx.x; x < 64 * DP; x += WF_THREADS) {
+#pragma unroll 8
+            for (int x = threadIdx.x; x < ROWS * DP; x += WF_THREADS) {
                 const int r = x / DP, d = x % DP;
                 dst[r * PITCH + d] = r0 + r < n && d < a.D ? zg_to_float(src[(r0 + r) * ld + d]) : 0.f;
             }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    load(qs, q, a.ldq, i0);
+    const std::integral_constant<int, WF_M> q_rows{};
+    const std::integral_constant<int, WF_N> k_rows{};
+    load(q_rows, qs, q, a.ldq, i0);
 
-    float x[4][4 * NC], m[4], l[4];
+    const float2 zero2 = make_float2(0.f, 0.f);
+    float2 x[4][NC];
+    float m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4 * NC; ++c) x[i][c] = 0.f;
+        for (int c = 0; c < NC; ++c) x[i][c] = zero2;
     }
     const int last = i0 + WF_M < n ? i0 + WF_M : n;  // rows [i0, last)
     const int kt_end = (last + WF_N - 1) / WF_N;
     const int w0 = i0 - a.window + 1 > 0 ? (i0 - a.window + 1) / WF_N : 0;  // the window's first tile
     int sink_end = (a.sinks + WF_N - 1) / WF_N;                              // tiles that hold sinks
     if (sink_end > w0) sink_end = w0;
-    for (int kt = sink_end > 0 ? 0 : w0; kt < kt_end; kt = kt + 1 < sink_end || kt >= w0 ? kt + 1 : w0) {
+    auto next = [&](int kt) { return kt + 1 < sink_end || kt >= w0 ? kt + 1 : w0; };
+    int kt = sink_end > 0 ? 0 : w0;
+    load(k_rows, ks, k, a.ldk, kt * WF_N);
+    for (; kt < kt_end; kt = next(kt)) {
         const int j0 = kt * WF_N;
-        __syncthreads();  // the last tile has been read
-        load(ks, k, a.ldk, j0);
-        load(vs, v, a.ldv, j0);
+        load(k_rows, vs, v, a.ldv, j0);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
         __syncthreads();
-        float s[4][4];
+        float2 s2[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+            for (int j = 0; j < 4; ++j) s2[i][j] = zero2;
 #pragma unroll 4
         for (int d = 0; d < DP; d += 4) {
             float4 qv[4], kv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 16 * i) * PITCH + d);
+                qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * PITCH + d);
                 kv[i] = *reinterpret_cast<const float4*>(ks + (tx + 16 * i) * PITCH + d);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    s[i][j] = fmaf(qv[i].x, kv[j].x,
-                                   fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
+                for (int j = 0; j < 4; ++j) {
+                    s2[i][j] = ffma2_tc(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+                    s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+                }
         }
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
+        __syncthreads();
+        if (next(kt) < kt_end)
+            load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
+        else
+            asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int qi = i0 + ty + 16 * i;
+            const int qi = i0 + ty + 8 * i;
             float t = m[i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -222,48 +261,45 @@ __global__ void __launch_bounds__(WF_THREADS) window_fma_kernel(const WindowArgs
             for (int j = 0; j < 4; ++j) {
                 const float p = exp2f(s[i][j] - base);
                 l[i] += p;
-                ps[(ty + 16 * i) * WF_PP + tx + 16 * j] = p;
+                ps[(ty + 8 * i) * WF_PP + tx + 16 * j] = p;
             }
 #pragma unroll
-            for (int e = 0; e < 4 * NC; ++e) x[i][e] *= c;
+            for (int e = 0; e < NC; ++e) x[i][e] = ffma2_tc(x[i][e], make_float2(c, c), zero2);
         }
         __syncwarp();  // a row's weights are written and read by the same half warp
 #pragma unroll 2
         for (int j = 0; j < WF_N; j += 4) {
             float4 pv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 16 * i) * WF_PP + j);
+            for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 8 * i) * WF_PP + j);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
-                    const float4 vv = *reinterpret_cast<const float4*>(vs + (j + e) * PITCH + 64 * c + 4 * tx);
+                    const float2 vv = *reinterpret_cast<const float2*>(vs + (j + e) * PITCH + 32 * c + 2 * tx);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float p = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
-                        x[i][4 * c] = fmaf(p, vv.x, x[i][4 * c]);
-                        x[i][4 * c + 1] = fmaf(p, vv.y, x[i][4 * c + 1]);
-                        x[i][4 * c + 2] = fmaf(p, vv.z, x[i][4 * c + 2]);
-                        x[i][4 * c + 3] = fmaf(p, vv.w, x[i][4 * c + 3]);
+                        x[i][c] = ffma2_tc(make_float2(p, p), vv, x[i][c]);
                     }
                 }
             }
         }
-        __syncwarp();
+        __syncthreads();  // the values have been read
     }
     unsigned redo = 0;  // bit i: row i of this half warp is not finite
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int f = 8; f > 0; f >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], f);
-        const int qi = i0 + ty + 16 * i;
+        const int qi = i0 + ty + 8 * i;
         bool fine = true;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = 64 * c + 4 * tx + e;
-                const float y = qi < n ? x[i][4 * c + e] / l[i] : 0.f;
+            for (int e = 0; e < 2; ++e) {
+                const int d = 32 * c + 2 * tx + e;
+                const float y = qi < n ? (e ? x[i][c].y : x[i][c].x) / l[i] : 0.f;
                 if (d < a.D) {
                     fine = fine && isfinite(y);
                     if (qi < a.S) o[qi * ldo + d] = zg_from_float<T>(y);
@@ -278,7 +314,7 @@ __global__ void __launch_bounds__(WF_THREADS) window_fma_kernel(const WindowArgs
         for (int i = 0; i < 4; ++i)
             if (rows >> i & 1) {
                 __syncwarp();  // the row's first values are written before these
-                window_row<T>(a, z, i0 + (int)(threadIdx.x / 32) * 2 + t + 16 * i, h);
+                window_row<T>(a, z, i0 + (int)(threadIdx.x / 32) * 2 + t + 8 * i, h);
             }
     }
 }
@@ -301,8 +337,11 @@ template <typename T>
 int launch_window_any(const WindowArgs& a, cudaStream_t st) {
     auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     const int vec = a.D % 4 == 0 && a.ldq % 4 == 0 && a.ldk % 4 == 0 && a.ldv % 4 == 0 && al(a.q) && al(a.k) && al(a.v);
-    return a.D <= 64    ? launch_window_fma<T, 64>(a, vec, st)
-           : a.D <= 128 ? launch_window_fma<T, 128>(a, vec, st) : launch_window_fma<T, 256>(a, vec, st);
+    return a.D <= 32    ? launch_window_fma<T, 32>(a, vec, st)
+           : a.D <= 64  ? launch_window_fma<T, 64>(a, vec, st)
+           : a.D <= 96  ? launch_window_fma<T, 96>(a, vec, st)
+           : a.D <= 128 ? launch_window_fma<T, 128>(a, vec, st)
+           : a.D <= 192 ? launch_window_fma<T, 192>(a, vec, st) : launch_window_fma<T, 256>(a, vec, st);
 }
 
 // ---------------------------------------------------------------------------

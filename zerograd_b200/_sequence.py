@@ -27,7 +27,6 @@ import math
 import torch
 
 from . import _lib as L
-from ._block import _as
 from ._ops import _NS, _movedim0
 
 _INT_MAX = 2 ** 31 - 1
@@ -44,9 +43,21 @@ def _plain_call(*ts) -> bool:
         return False
     grad = torch.is_grad_enabled()
     for t in ts:
-        if t is not None and (type(t) is not torch.Tensor or (grad and t.requires_grad)):
+        if type(t) is not torch.Tensor:
+            if t is not None:
+                return False
+        elif grad and t.requires_grad:
             return False
     return True
+
+
+def _device(*ts) -> torch.device:
+    """The CUDA device that all of the tensors (or None) are on."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and (t.device != dev or not t.is_cuda):
+            return L.require_cuda(*ts)
+    return dev
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
@@ -65,7 +76,7 @@ def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
     become -1 or the largest, which the kernels refuse as they would the
     number itself."""
     if t.dtype is torch.int32:
-        return t if t.is_contiguous() else t.contiguous()
+        return t.contiguous()
     if t.dtype is not torch.int64:
         raise TypeError(f"{what} must be int32 or int64, got {t.dtype}")
     return t.clamp(-1, _INT_MAX).to(torch.int32).contiguous()
@@ -112,28 +123,27 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
     """q [..., S, H, D] and k [..., S, K, D] turned by `positions`
     [pos.., S, A], whose leading axes are the last ones of q's (none: shared
     by all); outputs contiguous."""
-    dev = L.require_cuda(q, k, positions)
-    if q.ndim < 3 or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+    dev = _device(q, k, positions)
+    qs, ks, ps = q.shape, k.shape, positions.shape
+    tokens = qs[:-2]
+    if len(qs) < 3 or len(ks) != len(qs) or ks[:-2] != tokens or qs[-1] != ks[-1]:
         raise ValueError("q and k must be [..., S, H, D] and [..., S, K, D] with the same leading axes and D")
-    tokens = tuple(q.shape[:-2])
-    if (positions.ndim < 2 or positions.shape[-1] != len(axes) or positions.ndim - 1 > len(tokens)
-            or tuple(positions.shape[:-1]) != tokens[len(tokens) - (positions.ndim - 1):]):
-        raise ValueError(f"positions of shape {tuple(positions.shape)} do not give {len(axes)} axes for the tokens "
-                         f"{tokens}")
-    if positions.dtype not in _POSITION_CODES:
+    if len(ps) < 2 or ps[-1] != len(axes) or len(ps) - 1 > len(tokens) or ps[:-1] != tokens[len(tokens) - len(ps) + 1:]:
+        raise ValueError(f"positions of shape {tuple(ps)} do not give {len(axes)} axes for the tokens {tuple(tokens)}")
+    pos_code = _POSITION_CODES.get(positions.dtype)
+    if pos_code is None:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
     dt = q.dtype
     code = L.dtype_code(dt)
-    H, D = int(q.shape[-2]), int(q.shape[-1])
-    K = int(k.shape[-2])
-    (q, ldq), (k, ldk) = _pitched(q), _pitched(_as(k, dt))
+    if k.dtype is not dt:
+        k = k.to(dt)
+    (q, ldq), (k, ldk) = _pitched(q), _pitched(k)
     positions = positions.contiguous()
-    qo = torch.empty(q.shape, dtype=dt, device=dev)
-    ko = torch.empty(k.shape, dtype=dt, device=dev)
+    qo, ko = q.new_empty(qs), k.new_empty(ks)
     widths = (ctypes.c_int32 * len(axes))(*axes)
-    _call(dev, "zg_rotary", q.data_ptr(), ldq, k.data_ptr(), ldk, positions.data_ptr(), _POSITION_CODES[positions.dtype],
-          math.prod(tokens), math.prod(positions.shape[:-1]), H, K, D, len(axes), widths, base, int(interleaved),
-          int(joint), int(inverse), code, qo.data_ptr(), ko.data_ptr())
+    _call(dev, "zg_rotary", q.data_ptr(), ldq, k.data_ptr(), ldk, positions.data_ptr(), pos_code, math.prod(tokens),
+          positions.numel() // len(axes), qs[-2], ks[-2], qs[-1], len(axes), widths, base, interleaved, joint,
+          inverse, code, qo.data_ptr(), ko.data_ptr())
     return qo, ko
 
 
@@ -178,6 +188,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes, base
     goes through.  q and k may be views of one fused projection; outputs are
     contiguous.  D of q and k, and their leading axes, are the same."""
     axes = [int(a) for a in axes]
+    if not axes:
+        raise ValueError("axes must name the columns of one axis at least")
     args = (q, k, positions, axes, float(base), bool(interleaved), bool(joint), bool(inverse))
     return launch_rotary(*args) if _plain_call(q, k, positions) else _rotary_op(*args)
 
@@ -189,26 +201,29 @@ def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
                             window: int, sinks: int) -> torch.Tensor:
     """q [..., S, H, D], k and v [..., S, K, D], lengths [...] or None;
     window 0: none."""
-    dev = L.require_cuda(q, k, v, lengths)
-    if q.ndim < 3 or k.shape != v.shape or k.ndim != q.ndim or q.shape[:-2] != k.shape[:-2] \
-            or q.shape[-1] != k.shape[-1]:
+    dev = _device(q, k, v, lengths)
+    qs, ks = q.shape, k.shape
+    lead = qs[:-3]
+    if len(qs) < 3 or ks != v.shape or len(ks) != len(qs) or ks[:-2] != qs[:-2] or qs[-1] != ks[-1]:
         raise ValueError("q must be [..., S, H, D], k and v [..., S, K, D] with the same leading axes and D")
     dt = q.dtype
     code = L.dtype_code(dt)
-    S, H, D = (int(d) for d in q.shape[-3:])
-    K = int(k.shape[-2])
+    S, H, D = qs[-3:]
+    K = ks[-2]
     if K < 1 or H % K:
         raise ValueError(f"{H} query heads are not a multiple of {K} key heads")
-    Z = math.prod(q.shape[:-3])
     if lengths is not None:
-        if tuple(lengths.shape) != tuple(q.shape[:-3]):
-            raise ValueError(f"lengths of shape {tuple(lengths.shape)} do not match the sequences "
-                             f"{tuple(q.shape[:-3])}")
+        if lengths.shape != lead:
+            raise ValueError(f"lengths of shape {tuple(lengths.shape)} do not match the sequences {tuple(lead)}")
         lengths = _int32(lengths, "lengths")
-    (q, ldq), (k, ldk), (v, ldv) = _pitched(q), _pitched(_as(k, dt)), _pitched(_as(v, dt))
-    o = torch.empty(q.shape, dtype=dt, device=dev)
-    _call(dev, "zg_window_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, L.ptr(lengths), Z, S,
-          H, K, D, window, sinks, code, o.data_ptr())
+    if k.dtype is not dt:
+        k = k.to(dt)
+    if v.dtype is not dt:
+        v = v.to(dt)
+    (q, ldq), (k, ldk), (v, ldv) = _pitched(q), _pitched(k), _pitched(v)
+    o = q.new_empty(qs)
+    _call(dev, "zg_window_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+          None if lengths is None else lengths.data_ptr(), math.prod(lead), S, H, K, D, window, sinks, code, o.data_ptr())
     return o
 
 
@@ -249,22 +264,21 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 # -------------------------------------------------------------- paged cache
 
 
-def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int]:
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> torch.Size:
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:
         raise ValueError("key and value pages must share one [pages, page size, K, D] shape and type")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("key and value pages must be contiguous")
-    L.dtype_code(k_pages.dtype)
-    N, page, K, D = (int(d) for d in k_pages.shape)
-    if page < 1 or K < 1 or D < 1:
-        raise ValueError(f"pages of shape {tuple(k_pages.shape)} hold nothing")
-    return N, page, K, D
+    if shape[1] < 1 or shape[2] < 1 or shape[3] < 1:
+        raise ValueError(f"pages of shape {tuple(shape)} hold nothing")
+    return shape
 
 
-def _table(page_table: torch.Tensor, lengths: torch.Tensor, lead: tuple) -> tuple[torch.Tensor, torch.Tensor]:
-    if page_table.ndim < 1 or tuple(page_table.shape[:-1]) != lead or tuple(lengths.shape) != lead:
+def _table(page_table: torch.Tensor, lengths: torch.Tensor, lead: torch.Size) -> tuple[torch.Tensor, torch.Tensor]:
+    if page_table.ndim < 1 or page_table.shape[:-1] != lead or lengths.shape != lead:
         raise ValueError(f"a page table of shape {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} do not "
-                         f"match the sequences {lead}")
+                         f"match the sequences {tuple(lead)}")
     return _int32(page_table, "the page table"), _int32(lengths, "lengths")
 
 
@@ -272,23 +286,26 @@ def launch_append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.T
                         page_table: torch.Tensor, lengths: torch.Tensor,
                         counts: torch.Tensor | None) -> torch.Tensor:
     """k and v [..., S, K, D] into the pages of the sequences [...]."""
-    dev = L.require_cuda(k_pages, v_pages, k, v, page_table, lengths, counts)
+    dev = _device(k_pages, v_pages, k, v, page_table, lengths, counts)
     N, page, K, D = _pool(k_pages, v_pages)
-    if k.ndim < 3 or k.shape != v.shape or tuple(k.shape[-2:]) != (K, D):
-        raise ValueError(f"new keys and values must be [..., S, {K}, {D}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype != k_pages.dtype or v.dtype != k_pages.dtype:
-        raise TypeError(f"new keys and values must have the pages' type {k_pages.dtype}")
-    lead = tuple(k.shape[:-3])
+    ks = k.shape
+    if len(ks) < 3 or ks != v.shape or ks[-2] != K or ks[-1] != D:
+        raise ValueError(f"new keys and values must be [..., S, {K}, {D}], got {tuple(ks)} and {tuple(v.shape)}")
+    dt = k_pages.dtype
+    code = L.dtype_code(dt)
+    if k.dtype is not dt or v.dtype is not dt:
+        raise TypeError(f"new keys and values must have the pages' type {dt}")
+    lead = ks[:-3]
     table, had = _table(page_table, lengths, lead)
     if counts is not None:
-        if tuple(counts.shape) != lead:
-            raise ValueError(f"counts of shape {tuple(counts.shape)} do not match the sequences {lead}")
+        if counts.shape != lead:
+            raise ValueError(f"counts of shape {tuple(counts.shape)} do not match the sequences {tuple(lead)}")
         counts = _int32(counts, "counts")
     (k, ldk), (v, ldv) = _pitched(k), _pitched(v)
-    new = torch.empty(lead, dtype=torch.int32, device=dev)
-    _call(dev, "zg_append_pages", k_pages.data_ptr(), v_pages.data_ptr(), N, page, K, D, k.data_ptr(), ldk, v.data_ptr(), ldv,
-          math.prod(lead), int(k.shape[-3]), table.data_ptr(), int(table.shape[-1]), had.data_ptr(), L.ptr(counts),
-          L.dtype_code(k_pages.dtype), new.data_ptr())
+    new = had.new_empty(lead)
+    _call(dev, "zg_append_pages", k_pages.data_ptr(), v_pages.data_ptr(), N, page, K, D, k.data_ptr(), ldk, v.data_ptr(),
+          ldv, math.prod(lead), ks[-3], table.data_ptr(), table.shape[-1], had.data_ptr(),
+          None if counts is None else counts.data_ptr(), code, new.data_ptr())
     return new
 
 
@@ -343,26 +360,27 @@ def append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
 def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                            lengths: torch.Tensor, window: int, sinks: int) -> torch.Tensor:
     """q [..., H, D] over the pages of the sequences [...]; window 0: none."""
-    dev = L.require_cuda(q, k_pages, v_pages, page_table, lengths)
+    dev = _device(q, k_pages, v_pages, page_table, lengths)
     N, page, K, D = _pool(k_pages, v_pages)
-    if q.ndim < 2 or int(q.shape[-1]) != D or int(q.shape[-2]) < 1 or int(q.shape[-2]) % K:
-        raise ValueError(f"q of shape {tuple(q.shape)} is not [..., H, {D}] with H a multiple of {K} key heads")
-    if q.dtype != k_pages.dtype:
-        raise TypeError(f"q must have the pages' type {k_pages.dtype}, got {q.dtype}")
-    lead = tuple(q.shape[:-2])
+    qs, dt = q.shape, k_pages.dtype
+    if len(qs) < 2 or qs[-1] != D or qs[-2] < 1 or qs[-2] % K:
+        raise ValueError(f"q of shape {tuple(qs)} is not [..., H, {D}] with H a multiple of {K} key heads")
+    if q.dtype is not dt:
+        raise TypeError(f"q must have the pages' type {dt}, got {q.dtype}")
+    lead, H = qs[:-2], qs[-2]
     table, had = _table(page_table, lengths, lead)
-    H, B, M = int(q.shape[-2]), math.prod(lead), int(table.shape[-1])
-    code = L.dtype_code(q.dtype)
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    B, M = math.prod(lead), table.shape[-1]
+    code = L.dtype_code(dt)
+    o = q.new_empty(qs)
     if B == 0:
         return o
-    rows, ldq = _pitched(q if q.ndim > 2 else q.unsqueeze(0))
+    rows, ldq = _pitched(q)
     if rows.data_ptr() % 4 or ldq % 2:
         rows, ldq = rows.clone(memory_format=torch.contiguous_format), H * D
     nbytes = L.query("zg_paged_attention_workspace_size", B, H, K, D, M, page, window, sinks, code)
     ws = L.workspace(nbytes, dev) if nbytes else None
-    _call(dev, "zg_paged_attention", rows.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), N, page, table.data_ptr(), M,
-          had.data_ptr(), B, H, K, D, window, sinks, code, o.data_ptr(), L.ptr(ws), nbytes)
+    _call(dev, "zg_paged_attention", rows.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), N, page,
+          table.data_ptr(), M, had.data_ptr(), B, H, K, D, window, sinks, code, o.data_ptr(), L.ptr(ws), nbytes)
     return o
 
 

@@ -100,10 +100,10 @@ struct PagedArgs {
     const void *q, *kp, *vp;
     const int32_t *table, *lengths;
     void* o;
-    float* part;  // splits > 1: per unit and split, m [R], l [R], then R rows of sums
+    float* part;  // splits > 1 without a cluster: per unit and split, m [R], l [R], then R rows of sums
     int64_t ldq, n_pages;
     int page, max_pages, H, K, D, G, row_tiles, R;  // R: query rows of a unit (heads that share a key head)
-    int window, sinks, chunk, splits;
+    int window, sinks, chunk, splits, cluster;  // cluster: a unit's splits are a cluster, which joins them
     float scale;  // log2(e) / sqrt(D)
 };
 
@@ -125,18 +125,25 @@ __device__ __forceinline__ Seen seen_by(const PagedArgs& a, int b) {
     return Seen{w + s, s, n - w - s};
 }
 
-// The place (page * page size + slot) of visible position t, -1 past `end`
-// or, with bad set, where the table names no page.
-__device__ __forceinline__ int place_of(const PagedArgs& a, const Seen& v, const int32_t* row, int t, int end,
-                                        bool& bad) {
-    if (t >= end) return -1;
+// A position's entry of the page table, read one tile before it is used: the
+// read takes as long as a row's own.  off < 0: no position.
+struct Entry {
+    int id, off;
+};
+__device__ __forceinline__ Entry entry_of(const PagedArgs& a, const Seen& v, const int32_t* row, int t, bool on) {
+    if (!on) return Entry{0, -1};
     const int tok = v.token(t), p = tok / a.page;
-    const int32_t id = row[p];
-    if (id < 0 || id >= a.n_pages) {
+    return Entry{row[p], tok - p * a.page};
+}
+// Its place (page * page size + slot); -1 where there is no position or, with
+// bad set, where the table names no page.
+__device__ __forceinline__ int place_of(const PagedArgs& a, const Entry& e, bool& bad) {
+    if (e.off < 0) return -1;
+    if (e.id < 0 || e.id >= a.n_pages) {
         bad = true;
         return -1;
     }
-    return id * a.page + (tok - p * a.page);
+    return e.id * a.page + e.off;
 }
 
 __device__ __forceinline__ uint32_t shared_u32(const void* p) {
@@ -157,14 +164,29 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// Joins the warps' (m, l, sums) of one unit in shared memory, in warp order,
-// and writes the output (one split) or this split's partial.
-// ms, ls [PG_WARPS][R]; os [PG_WARPS][R][pitch].
+// The float at `p` of this block's shared memory in block `rank` of the cluster.
+__device__ __forceinline__ float cluster_float(const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+constexpr int PG_CLUSTER = 8;  // splits that are joined in a cluster, at most
+
+// Joins the warps' (m, l, sums) of one unit in shared memory, in warp order;
+// then writes the output (one split), or this split's partial, or joins the
+// splits of a cluster, in split order, each block a part of the outputs.
+// ms, ls [PG_WARPS][R] (the joined ones in the first R); os [PG_WARPS][R][pitch].
 template <typename T>
-__device__ __forceinline__ void join_warps(const PagedArgs& a, const float* ms, const float* ls, const float* os,
-                                           int pitch, int rows, int b, int h0, int64_t unit, int split, bool bad,
-                                           bool none) {
-    float* part = a.splits > 1 ? a.part + (unit * a.splits + split) * part_floats(a.R, a.D) : nullptr;
+__device__ __forceinline__ void join_warps(const PagedArgs& a, float* ms, float* ls, float* os, int pitch, int rows,
+                                           int b, int h0, int64_t unit, int split, bool bad, bool none) {
+    float* part = a.splits > 1 && !a.cluster ? a.part + (unit * a.splits + split) * part_floats(a.R, a.D) : nullptr;
+    T* out = static_cast<T*>(a.o) + ((int64_t)b * a.H + h0) * a.D;
     for (int i = threadIdx.x; i < rows * a.D; i += PG_WARPS * 32) {
         const int r = i / a.D, d = i - r * a.D;
         float M = -INFINITY;
@@ -179,16 +201,56 @@ __device__ __forceinline__ void join_warps(const PagedArgs& a, const float* ms, 
             x = fmaf(os[(w * a.R + r) * pitch + d], f, x);
         }
         if (bad) l = __int_as_float(0x7fffffff);
-        if (part) {
+        if (a.cluster) {
+            os[r * pitch + d] = x;  // read by this thread alone
+        } else if (part) {
             if (d == 0) {
                 part[r] = M;
                 part[a.R + r] = l;
             }
             part[2 * a.R + r * pad4(a.D) + d] = x;
         } else {
-            static_cast<T*>(a.o)[((int64_t)b * a.H + h0 + r) * a.D + d] = zg_from_float<T>(none ? 0.f : x / l);
+            out[i] = zg_from_float<T>(none ? 0.f : x / l);
         }
     }
+    if (!a.cluster) return;
+    // the row's maximum and sum over the warps, by one warp's lanes (R <= 16)
+    __syncthreads();
+    if (threadIdx.x < a.R) {
+        const int r = threadIdx.x;
+        float M = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[w * a.R + r]);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < PG_WARPS; ++w) l = fmaf(ls[w * a.R + r], exp2_fast(ms[w * a.R + r] - base), l);
+        ms[r] = M;  // read by this thread alone
+        ls[r] = bad ? __int_as_float(0x7fffffff) : l;
+    }
+    cluster_sync_all();
+    for (int i = split * PG_WARPS * 32 + threadIdx.x; i < rows * a.D; i += a.splits * PG_WARPS * 32) {
+        const int r = i / a.D, d = i - r * a.D;
+        float m[PG_CLUSTER], l[PG_CLUSTER], x[PG_CLUSTER], M = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < PG_CLUSTER; ++s)
+            if (s < a.splits) {
+                m[s] = cluster_float(ms + r, s);
+                l[s] = cluster_float(ls + r, s);
+                x[s] = cluster_float(os + r * pitch + d, s);
+                M = fmaxf(M, m[s]);
+            }
+        const float base = M == -INFINITY ? 0.f : M;
+        float num = 0.f, den = 0.f;
+#pragma unroll
+        for (int s = 0; s < PG_CLUSTER; ++s)
+            if (s < a.splits) {
+                const float f = exp2_fast(m[s] - base);
+                num = fmaf(x[s], f, num);
+                den = fmaf(l[s], f, den);
+            }
+        out[i] = zg_from_float<T>(none ? 0.f : num / den);
+    }
+    cluster_sync_all();  // no block leaves while another reads its memory
 }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -238,7 +300,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     const Seen see = seen_by(a, b);
     const int c0 = split * a.chunk;
     const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;  // this split: [c0, end)
-    if (c0 >= see.vis && a.splits > 1) return;  // nothing here; the join knows by the length
+    if (c0 >= see.vis && a.splits > 1 && !a.cluster) return;  // nothing here; the join knows by the length
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + 15) / 16 : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -248,9 +310,10 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     const int64_t token_pitch = (int64_t)a.K * a.D;
     bool bad = false;
 
-    // lanes 0..15: the place of each row of this warp's tile i
-    auto places = [&](int i) {
-        return i < tiles && lane < 16 ? place_of(a, see, table, c0 + (warp + PG_WARPS * i) * 16 + lane, end, bad) : -1;
+    // lanes 0..15: the table's entry for each row of this warp's tile i
+    auto entries = [&](int i) {
+        const int t = c0 + (warp + PG_WARPS * i) * 16 + lane;
+        return entry_of(a, see, table, t, i < tiles && lane < 16 && t < end);
     };
     auto fetch = [&](int stage, int place) {
         const uint32_t kd = shared_u32(ring + stage * 2 * TILE), vd = kd + TILE;
@@ -266,13 +329,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
         }
     };
 
-    int place = places(0);
+    Entry entry = entries(0);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-        const int next = places(s + 1);
-        if (s < tiles) fetch(s, place);
+        const Entry next = entries(s + 1);
+        if (s < tiles) fetch(s, place_of(a, entry, bad));
         copy_commit();
-        place = next;
+        entry = next;
     }
 
     // queries as the rows of A: (row, k) = (lane / 4 [+ 8], 2 (lane % 4) [+ 8]) in k-steps of 16
@@ -298,10 +361,10 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
         copy_wait<STAGES - 2>();
         __syncwarp();  // every lane's copies of tile i have landed, and tile i-1 has been read
         {
-            const int next = places(i + STAGES);
-            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place);
+            const Entry next = entries(i + STAGES);
+            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
             copy_commit();
-            place = next;
+            entry = next;
         }
         const uint32_t kt = shared_u32(ring + (i % STAGES) * 2 * TILE), vt = kt + TILE;
         float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -394,13 +457,15 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 // a PARTS-th of the columns), then every lane takes the columns lane + 32 i
 // of the sums.  GT query heads at a time; the same ring of tiles as above,
 // its rows kept as they are stored, 16 bytes apart from the next one's banks.
+constexpr int PG_FMA_STAGES = 2;  // three blocks an SM (two with 3: a batch of 64 x 1000 in float32 34.2 us, not 32.6)
+
 template <typename T, int PARTS, int GT>
 __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArgs a, int vec) {
-    constexpr int TT = 32 / PARTS, STAGES = 3, NI = PARTS, DMAX = 32 * PARTS;
+    constexpr int TT = 32 / PARTS, STAGES = PG_FMA_STAGES, NI = PARTS, DMAX = 32 * PARTS;
     constexpr int PITCH = DMAX * (int)sizeof(T) + 16, TILE = TT * PITCH;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float ms[PG_WARPS * GT], ls[PG_WARPS * GT];
-    __shared__ __align__(16) float qs[GT][DMAX];
+    __shared__ __align__(16) float qs[GT][36 * PARTS];  // parts of 32 columns, 4 banks apart
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t unit = blockIdx.x / a.splits;
     const int split = (int)(blockIdx.x % a.splits);
@@ -411,7 +476,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
     const Seen see = seen_by(a, b);
     const int c0 = split * a.chunk;
     const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;
-    if (c0 >= see.vis && a.splits > 1) return;
+    if (c0 >= see.vis && a.splits > 1 && !a.cluster) return;
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + TT - 1) / TT : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -423,47 +488,49 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
 
     for (int i = threadIdx.x; i < GT * DMAX; i += PG_WARPS * 32) {
         const int r = i / DMAX, d = i % DMAX;
-        qs[r][d] = r < rows && d < a.D ? zg_to_float(static_cast<const T*>(a.q)[b * a.ldq + (int64_t)(h0 + r) * a.D + d]) * a.scale : 0.f;
+        qs[r][d / 32 * 36 + d % 32] = r < rows && d < a.D ? zg_to_float(static_cast<const T*>(a.q)[b * a.ldq + (int64_t)(h0 + r) * a.D + d]) * a.scale : 0.f;
     }
     // the columns past D stay zero in every stage
     for (int i = lane; i < STAGES * 2 * TILE / 4; i += 32) reinterpret_cast<uint32_t*>(ring)[i] = 0u;
     __syncthreads();
 
-    auto places = [&](int i) {
-        return i < tiles && lane < TT ? place_of(a, see, table, c0 + (warp + PG_WARPS * i) * TT + lane, end, bad) : -1;
+    auto entries = [&](int i) {
+        const int t = c0 + (warp + PG_WARPS * i) * TT + lane;
+        return entry_of(a, see, table, t, i < tiles && lane < TT && t < end);
     };
-    const int words = vec ? a.D * (int)sizeof(T) / 16 : a.D;  // of a row
     auto fetch = [&](int stage, int place) {
         uint8_t* kd = ring + stage * 2 * TILE;
         uint8_t* vd = kd + TILE;
-        int r = lane / words, c = lane - r * words;
-        for (int i = 0; i < TT * words; i += 32) {
-            const int at = __shfl_sync(0xffffffffu, place, r < TT ? r : 0);
-            if (r < TT) {
+        if (vec) {
+            // 16-byte words of the padded rows, zeros behind D
+            constexpr int N = 16 / sizeof(T), WORDS = DMAX / N;
+#pragma unroll
+            for (int it = 0; it < TT * WORDS / 32; ++it) {
+                const int i = it * 32 + lane, r = i / WORDS, c = i % WORDS;
+                const int at = __shfl_sync(0xffffffffu, place, r);
+                const bool on = at >= 0 && c * N < a.D;
+                const int64_t off = on ? at * token_pitch + c * N : 0;
+                copy16(shared_u32(kd + r * PITCH + c * 16), kp + off, on ? 16 : 0);
+                copy16(shared_u32(vd + r * PITCH + c * 16), vp + off, on ? 16 : 0);
+            }
+        } else {
+            for (int r = 0; r < TT; ++r) {
+                const int at = __shfl_sync(0xffffffffu, place, r);
                 const int64_t off = at >= 0 ? at * token_pitch : 0;
-                if (vec) {
-                    constexpr int N = 16 / sizeof(T);
-                    copy16(shared_u32(kd + r * PITCH + c * 16), kp + off + (at >= 0 ? c * N : 0), at >= 0 ? 16 : 0);
-                    copy16(shared_u32(vd + r * PITCH + c * 16), vp + off + (at >= 0 ? c * N : 0), at >= 0 ? 16 : 0);
-                } else {
+                for (int c = lane; c < a.D; c += 32) {
                     reinterpret_cast<T*>(kd + r * PITCH)[c] = at >= 0 ? kp[off + c] : zg_from_float<T>(0.f);
                     reinterpret_cast<T*>(vd + r * PITCH)[c] = at >= 0 ? vp[off + c] : zg_from_float<T>(0.f);
                 }
             }
-            c += 32;
-            while (c >= words) {
-                c -= words;
-                ++r;
-            }
         }
     };
-    int place = places(0);
+    Entry entry = entries(0);
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-        const int next = places(s + 1);
-        if (s < tiles) fetch(s, place);
+        const Entry next = entries(s + 1);
+        if (s < tiles) fetch(s, place_of(a, entry, bad));
         copy_commit();
-        place = next;
+        entry = next;
     }
     float o[GT][NI], m[GT], l[GT];
 #pragma unroll
@@ -478,10 +545,10 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
         copy_wait<STAGES - 2>();
         __syncwarp();
         {
-            const int next = places(i + STAGES);
-            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place);
+            const Entry next = entries(i + STAGES);
+            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
             copy_commit();
-            place = next;
+            entry = next;
         }
         const uint8_t* kt = ring + (i % STAGES) * 2 * TILE;
         const uint8_t* vt = kt + TILE;
@@ -502,7 +569,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
             }
 #pragma unroll
             for (int g = 0; g < GT; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&qs[g][part * 32 + d]);
+                const float4 x = *reinterpret_cast<const float4*>(&qs[g][part * 36 + d]);
                 s[g] = fmaf(kv[0], x.x, fmaf(kv[1], x.y, fmaf(kv[2], x.z, fmaf(kv[3], x.w, s[g]))));
             }
         }
@@ -566,6 +633,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
     const int kh = h / a.G, rt = h % a.G / a.R, r = h % a.G % a.R;
     const int64_t unit = ((int64_t)b * a.K + kh) * a.row_tiles + rt;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched before the splits' kernel has ended
     const int vis = seen_by(a, b).vis;
     const int n = vis > 0 ? (vis + a.chunk - 1) / a.chunk : 0;
     const int64_t pf = part_floats(a.R, a.D);
@@ -613,10 +681,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     static_cast<T*>(a.o)[((int64_t)b * a.H + h) * a.D + d] = zg_from_float<T>(out);
 }
 
+constexpr int PG_MIN_CHUNK = 128;
+
 // How a call is cut: R query rows of a unit, and the units' splits.
 struct PagedPlan {
     int R, row_tiles, chunk, splits;
-    bool mma;
+    bool mma, cluster;
 };
 
 PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window, int sinks, int dtype) {
@@ -629,23 +699,35 @@ PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window
     if (window > 0 && (int64_t)window + sinks < vis) vis = (int64_t)window + sinks;
     if (vis < 1) vis = 1;
     const int64_t units = B * K * p.row_tiles;
-    // Two blocks run on each of 148 SMs.  One sequence: as many splits as
-    // fill them once.  A batch: four times that, so that sequences of
-    // different lengths, cut into pieces of one length, even out.
-    const int64_t want = 2 * 148 * (B == 1 ? 1 : 4);
-    int64_t splits = want / units;
-    if (splits < 1) splits = 1;
+    // Two blocks run on each of 148 SMs (three of the FMA path): as many splits
+    // as fill them once.  (Four times as many, so that a batch of 64 sequences
+    // of different lengths evens out, was 126 us instead of 81: a block costs
+    // its pipeline's filling and its part in the join.)  Up to PG_CLUSTER
+    // splits are a cluster, which joins them by itself.  Of more than that,
+    // where a kernel of its own joins them, a batch takes half as many again:
+    // 8 sequences of up to 30000 tokens 29.5 -> 27.1 us; one sequence, whose
+    // pieces are all of one length, does not (53 -> 72 us).
+    const int per_sm = p.mma ? 2 : 3;
+    int64_t splits = (per_sm * 148 + units - 1) / units;
+    if (splits > PG_CLUSTER && B > 1) splits = ((per_sm + 1) * 148 + units - 1) / units;
     if (splits > 128) splits = 128;
     int64_t chunk = (vis + splits - 1) / splits;
-    if (chunk < 256) chunk = 256;  // less would be the pipeline's filling and the join
+    if (chunk < PG_MIN_CHUNK) chunk = PG_MIN_CHUNK;  // less would be the pipeline's filling and the join
     chunk = (chunk + 63) / 64 * 64;
     p.chunk = (int)(chunk > INT32_MAX ? INT32_MAX / 64 * 64 : chunk);
     p.splits = (int)((vis + p.chunk - 1) / p.chunk);
+    p.cluster = p.splits > 1 && p.splits <= PG_CLUSTER;
+    if (p.cluster) {
+        // two, four or eight blocks, of equal shares
+        const int size = p.splits <= 2 ? 2 : p.splits <= 4 ? 4 : 8;
+        p.chunk = (int)(((vis + size - 1) / size + 63) / 64 * 64);
+        p.splits = size;
+    }
     return p;
 }
 
 size_t paged_workspace(const PagedPlan& p, int64_t B, int K, int D) {
-    return p.splits > 1 ? (size_t)(B * K * p.row_tiles * p.splits * part_floats(p.R, D)) * sizeof(float) : 0;
+    return p.splits > 1 && !p.cluster ? (size_t)(B * K * p.row_tiles * p.splits * part_floats(p.R, D)) * sizeof(float) : 0;
 }
 
 bool paged_sizes_ok(int64_t n_pages, int page, int64_t B, int H, int K, int D, int max_pages) {
@@ -659,24 +741,40 @@ int set_smem(F* f, size_t bytes) {
     return ZG_OK;
 }
 
+template <typename... P, typename... A>
+int launch_split(void (*f)(P...), const PagedArgs& a, int64_t blocks, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)blocks);
+    c.blockDim = dim3(PG_WARPS * 32);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)a.splits;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = a.cluster ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&c, f, args...);
+    if (e != cudaSuccess) return zg::fail(ZG_ERR_CUDA, "zg_paged_attention: %s", cudaGetErrorString(e));
+    return zg::check_launch("zg_paged_attention");
+}
+
 template <int DP, int STAGES>
 int launch_mma(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
     const size_t smem = (size_t)PG_WARPS * STAGES * 2 * 16 * DP * 2;
     if (int rc = set_smem(paged_mma_kernel<DP, STAGES>, smem)) return rc;
     zg::LaunchTimer zg_lt_("paged_attention", st);
-    paged_mma_kernel<DP, STAGES><<<(unsigned)blocks, PG_WARPS * 32, smem, st>>>(a);
-    return zg::check_launch("zg_paged_attention");
+    return launch_split(paged_mma_kernel<DP, STAGES>, a, blocks, smem, st, a);
 }
 
 template <typename T, int PARTS, int GT>
 int launch_fma(const PagedArgs& a, int vec, int64_t blocks, cudaStream_t st) {
-    const size_t ring = (size_t)PG_WARPS * 3 * 2 * (32 / PARTS) * (32 * PARTS * sizeof(T) + 16);
+    const size_t ring = (size_t)PG_WARPS * PG_FMA_STAGES * 2 * (32 / PARTS) * (32 * PARTS * sizeof(T) + 16);
     const size_t out = (size_t)PG_WARPS * GT * 32 * PARTS * sizeof(float);
     const size_t smem = ring > out ? ring : out;
     if (int rc = set_smem(paged_fma_kernel<T, PARTS, GT>, smem)) return rc;
     zg::LaunchTimer zg_lt_("paged_attention_fma", st);
-    paged_fma_kernel<T, PARTS, GT><<<(unsigned)blocks, PG_WARPS * 32, smem, st>>>(a, vec);
-    return zg::check_launch("zg_paged_attention");
+    return launch_split(paged_fma_kernel<T, PARTS, GT>, a, blocks, smem, st, a, vec);
 }
 
 template <typename T, int PARTS>
@@ -762,7 +860,7 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
     const int n = 16 / (int)zg::dtype_size(dtype);
     const int vec = D % n == 0 && aligned16(k_pages) && aligned16(v_pages);
     PagedArgs a{q, k_pages, v_pages, table, lengths, o, static_cast<float*>(workspace), ldq, n_pages, page, max_pages,
-                H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.chunk, p.splits,
+                H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.chunk, p.splits, p.cluster,
                 (float)(1.4426950408889634 / sqrt((double)D))};
     cudaStream_t st = zg::as_stream(stream);
     int rc;
@@ -776,11 +874,18 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
         rc = dtype == ZG_BF16 ? launch_fma_any<__nv_bfloat16>(a, vec, blocks, st)
                               : launch_fma_any<float>(a, vec, blocks, st);
     }
-    if (rc != ZG_OK || p.splits == 1) return rc;
+    if (rc != ZG_OK || p.splits == 1 || p.cluster) return rc;
     zg::LaunchTimer zg_lt_("paged_join", st);
-    if (dtype == ZG_BF16)
-        paged_join_kernel<__nv_bfloat16><<<(unsigned)(B * H), 256, 0, st>>>(a);
-    else
-        paged_join_kernel<float><<<(unsigned)(B * H), 256, 0, st>>>(a);
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(B * H));
+    c.blockDim = dim3(256);
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&c, dtype == ZG_BF16 ? paged_join_kernel<__nv_bfloat16> : paged_join_kernel<float>, a);
+    if (e != cudaSuccess) return zg::fail(ZG_ERR_CUDA, "zg_paged_attention: %s", cudaGetErrorString(e));
     return zg::check_launch("zg_paged_attention");
 }

@@ -16,12 +16,12 @@
 // the reduced angle goes to sincospif.
 #include <math.h>
 
-#include "zg_common.cuh"
+#include "zg_ptx.cuh"
 
 namespace {
 
 constexpr int RO_MAX_PAIRS = 128;  // D <= 256
-constexpr int RO_THREADS = 256;
+constexpr int RO_THREADS = 128;
 
 enum { RO_POS_I32 = 0, RO_POS_I64 = 1, RO_POS_F32 = 2 };
 
@@ -35,15 +35,25 @@ struct RotaryArgs {
     uint8_t axis[RO_MAX_PAIRS];
 };
 
-__device__ __forceinline__ float2 rotary_angle(const RotaryArgs& a, int64_t token, int p) {
-    const int64_t at = (token % a.pos_rows) * a.A + a.axis[p];
-    const double x = a.pos_type == RO_POS_I64   ? (double)static_cast<const int64_t*>(a.pos)[at]
-                     : a.pos_type == RO_POS_I32 ? (double)static_cast<const int32_t*>(a.pos)[at]
-                                                : (double)static_cast<const float*>(a.pos)[at];
-    const double t = x * a.turns[p];
-    float s, c;
-    sincospif((float)(2.0 * (t - rint(t))), &s, &c);
-    return make_float2(c, s * a.sign);
+// (cos, sin) of every pair p of the block's nt tokens from t0, handed to
+// put(token, p, cos, sin).  The row of a position table that repeats is found
+// once a block (a 64-bit remainder costs some hundred instructions).
+template <typename F>
+__device__ __forceinline__ void rotary_angles(const RotaryArgs& a, int64_t t0, int nt, F put) {
+    const int64_t row0 = t0 % a.pos_rows;
+    for (int i = threadIdx.x; i < nt * a.pairs; i += RO_THREADS) {
+        const int tt = i / a.pairs, p = i - tt * a.pairs;
+        int64_t row = row0 + tt;
+        while (row >= a.pos_rows) row -= a.pos_rows;
+        const int64_t at = row * a.A + a.axis[p];
+        const double x = a.pos_type == RO_POS_I64   ? (double)static_cast<const int64_t*>(a.pos)[at]
+                         : a.pos_type == RO_POS_I32 ? (double)static_cast<const int32_t*>(a.pos)[at]
+                                                    : (double)static_cast<const float*>(a.pos)[at];
+        const double t = x * a.turns[p];
+        float s, c;
+        sincospif((float)(2.0 * (t - rint(t))), &s, &c);
+        put(tt, p, c, s * a.sign);
+    }
 }
 
 // Sixteen bytes of T as floats, and back.
@@ -73,55 +83,85 @@ struct Vec16 {
 
 // Rows of 16-byte words.  An item is one word of an interleaved head, or two
 // words (the pairs' two columns) of a head in halves; the unturned columns
-// behind the pairs are items of one word, copied.
+// behind the pairs are items of one word, copied.  A thread has RO_ITEMS
+// items' words on the way at a time, the first ones while the block forms its
+// angles.  336 MB of bf16 (two videos of 16384 tokens, 16 + 4 heads of 128):
+// 66 us, 5.1 TB/s; with the angles read one by one, lanes 64 bytes apart in
+// shared memory, 74 us (the reads of four lanes met in a bank); persistent
+// blocks that fetch a group of tokens ahead by cp.async, 84 us (an SM's
+// instructions, not its reads in flight, are what is left).
+constexpr int RO_ITEMS = 4;
+
 template <typename T, bool IL>
 __global__ void __launch_bounds__(RO_THREADS) rotary_vec_kernel(const __grid_constant__ RotaryArgs a) {
     constexpr int N = Vec16<T>::N;
-    extern __shared__ float2 cs[];  // [tokens][pairs]
+    // An item's angles two by two, (cos, cos, sin, sin), those of neighbouring
+    // items of a head side by side: [tokens][EACH / 2][turned], EACH its pairs.
+    constexpr int EACH = IL ? N / 2 : N;
+    extern __shared__ float4 table[];
     const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
     const int nt = (int)(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
-    for (int i = threadIdx.x; i < nt * a.pairs; i += RO_THREADS)
-        cs[i] = rotary_angle(a, t0 + i / a.pairs, i % a.pairs);
-    __syncthreads();
     const int turned = IL ? 2 * a.pairs / N : a.pairs / N;  // items of a head that are turned
     const int per_head = turned + (a.D - 2 * a.pairs) / N;
     const int per_token = per_head * (a.H + a.K);
-    for (int i = threadIdx.x; i < nt * per_token; i += RO_THREADS) {
-        const int tt = i / per_token, r = i - tt * per_token;
-        const int hh = r / per_head, c = r - hh * per_head;
-        const int64_t token = t0 + tt;
-        const bool is_q = hh < a.H;
-        const int h = is_q ? hh : hh - a.H;
-        const T* x = static_cast<const T*>(is_q ? a.q : a.k) + token * (is_q ? a.ldq : a.ldk) + (int64_t)h * a.D;
-        T* y = static_cast<T*>(is_q ? a.q_out : a.k_out) + (token * (is_q ? a.H : a.K) + h) * a.D;
-        const float2* w = cs + tt * a.pairs;
-        if (c >= turned) {
-            const int col = 2 * a.pairs + (c - turned) * N;
-            *reinterpret_cast<uint4*>(y + col) = *reinterpret_cast<const uint4*>(x + col);
-        } else if constexpr (IL) {
-            float v[N];
-            Vec16<T>::unpack(*reinterpret_cast<const uint4*>(x + c * N), v);
+    bool angles = false;
+    for (int i0 = 0; i0 < nt * per_token; i0 += RO_ITEMS * RO_THREADS) {
+        uint4 u[RO_ITEMS], z[IL ? 1 : RO_ITEMS];
+        int tt[RO_ITEMS], col[RO_ITEMS];  // token of the block, first column; col < 0: no item
+        T* y[RO_ITEMS];
 #pragma unroll
-            for (int e = 0; e < N / 2; ++e) {
-                const float2 f = w[c * (N / 2) + e];
-                const float u = v[2 * e], z = v[2 * e + 1];
-                v[2 * e] = u * f.x - z * f.y;
-                v[2 * e + 1] = u * f.y + z * f.x;
-            }
-            *reinterpret_cast<uint4*>(y + c * N) = Vec16<T>::pack(v);
-        } else {
-            float u[N], z[N];
-            Vec16<T>::unpack(*reinterpret_cast<const uint4*>(x + c * N), u);
-            Vec16<T>::unpack(*reinterpret_cast<const uint4*>(x + a.pairs + c * N), z);
+        for (int e = 0; e < RO_ITEMS; ++e) {
+            const int i = i0 + e * RO_THREADS + threadIdx.x;
+            col[e] = -1;
+            if (i >= nt * per_token) continue;
+            tt[e] = i / per_token;
+            const int r = i - tt[e] * per_token, hh = r / per_head, c = r - hh * per_head;
+            const int64_t token = t0 + tt[e];
+            const bool is_q = hh < a.H;
+            const int h = is_q ? hh : hh - a.H;
+            const T* x = static_cast<const T*>(is_q ? a.q : a.k) + token * (is_q ? a.ldq : a.ldk) + (int64_t)h * a.D;
+            y[e] = static_cast<T*>(is_q ? a.q_out : a.k_out) + (token * (is_q ? a.H : a.K) + h) * a.D;
+            col[e] = c < turned ? c * N : 2 * a.pairs + (c - turned) * N;
+            u[e] = *reinterpret_cast<const uint4*>(x + col[e]);
+            if constexpr (!IL)
+                if (c < turned) z[e] = *reinterpret_cast<const uint4*>(x + a.pairs + col[e]);
+        }
+        if (!angles) {
+            rotary_angles(a, t0, nt, [&](int token, int p, float cosine, float sine) {
+                float* at = reinterpret_cast<float*>(table + (token * (EACH / 2) + p % EACH / 2) * turned + p / EACH);
+                at[p & 1] = cosine;
+                at[2 + (p & 1)] = sine;
+            });
+            __syncthreads();
+            angles = true;
+        }
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float2 f = w[c * N + e];
-                const float p = u[e], s = z[e];
-                u[e] = p * f.x - s * f.y;
-                z[e] = p * f.y + s * f.x;
+        for (int e = 0; e < RO_ITEMS; ++e) {
+            if (col[e] < 0) continue;
+            if (col[e] >= (IL ? 2 * a.pairs : a.pairs)) {
+                *reinterpret_cast<uint4*>(y[e] + col[e]) = u[e];
+                continue;
             }
-            *reinterpret_cast<uint4*>(y + c * N) = Vec16<T>::pack(u);
-            *reinterpret_cast<uint4*>(y + a.pairs + c * N) = Vec16<T>::pack(z);
+            const float4* w = table + tt[e] * (EACH / 2) * turned + col[e] / N;
+            float p[N], s[N];
+            Vec16<T>::unpack(u[e], p);
+            if constexpr (!IL) Vec16<T>::unpack(z[e], s);
+#pragma unroll
+            for (int f = 0; f < EACH; f += 2) {
+                const float4 g = w[f / 2 * turned];
+                const float2 c = make_float2(g.x, g.y), d = make_float2(g.z, g.w), zero = make_float2(0.f, 0.f);
+                const float2 o = IL ? make_float2(p[2 * f], p[2 * f + 2]) : make_float2(p[f], p[f + 1]);
+                const float2 t = IL ? make_float2(p[2 * f + 1], p[2 * f + 3]) : make_float2(s[f], s[f + 1]);
+                const float2 td = ffma2_tc(t, d, zero);
+                const float2 ra = ffma2_tc(o, c, make_float2(-td.x, -td.y)), rb = ffma2_tc(o, d, ffma2_tc(t, c, zero));
+                if constexpr (IL) {
+                    p[2 * f] = ra.x; p[2 * f + 2] = ra.y; p[2 * f + 1] = rb.x; p[2 * f + 3] = rb.y;
+                } else {
+                    p[f] = ra.x; p[f + 1] = ra.y; s[f] = rb.x; s[f + 1] = rb.y;
+                }
+            }
+            *reinterpret_cast<uint4*>(y[e] + col[e]) = Vec16<T>::pack(p);
+            if constexpr (!IL) *reinterpret_cast<uint4*>(y[e] + a.pairs + col[e]) = Vec16<T>::pack(s);
         }
     }
 }
@@ -132,8 +172,7 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_any_kernel(const __grid_con
     extern __shared__ float2 cs[];
     const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
     const int nt = (int)(a.T - t0 < a.tokens ? a.T - t0 : a.tokens);
-    for (int i = threadIdx.x; i < nt * a.pairs; i += RO_THREADS)
-        cs[i] = rotary_angle(a, t0 + i / a.pairs, i % a.pairs);
+    rotary_angles(a, t0, nt, [&](int token, int p, float c, float s) { cs[token * a.pairs + p] = make_float2(c, s); });
     __syncthreads();
     const int per_head = a.D - a.pairs, per_token = per_head * (a.H + a.K);
     for (int i = threadIdx.x; i < nt * per_token; i += RO_THREADS) {
@@ -162,8 +201,14 @@ int launch_rotary(RotaryArgs& a, cudaStream_t st) {
     auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     const bool vec = a.D % N == 0 && (a.interleaved ? 2 * a.pairs : a.pairs) % N == 0 && a.ldq % N == 0 &&
                      a.ldk % N == 0 && al(a.q) && al(a.k) && al(a.q_out) && al(a.k_out);
-    // up to eight tokens a block, fewer while the grid is short of two blocks per SM
-    a.tokens = 8;
+    // as many tokens a block as its threads have items in flight, fewer while
+    // the grid is short of two blocks per SM
+    const int pairs_of = a.interleaved ? 2 * a.pairs / N : a.pairs / N;
+    const int64_t items = vec ? (int64_t)(pairs_of + (a.D - 2 * a.pairs) / N) * (a.H + a.K)
+                              : (int64_t)(a.D - a.pairs) * (a.H + a.K);
+    a.tokens = (int)(RO_ITEMS * RO_THREADS / items);
+    if (a.tokens > 16) a.tokens = 16;
+    if (a.tokens < 1) a.tokens = 1;
     while (a.tokens > 1 && (a.T + a.tokens - 1) / a.tokens < 2 * 148) a.tokens /= 2;
     const int64_t blocks = (a.T + a.tokens - 1) / a.tokens;
     if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_rotary: too many tokens");

@@ -42,8 +42,8 @@ def rotary_tolerance(want, size, dtype):
     return HALF_STEP[dtype] * want.abs() + size * 2.0 ** -21
 
 
-def window_mask(S, window, sinks):
-    i, j = torch.arange(S)[:, None], torch.arange(S)[None, :]
+def window_mask(S, window, sinks, device="cpu"):
+    i, j = torch.arange(S, device=device)[:, None], torch.arange(S, device=device)[None, :]
     seen = j <= i
     if window is not None:
         seen = seen & ((i - j < window) | (j < sinks))
@@ -69,14 +69,15 @@ def _attend(q, k, v, seen):
 
 
 def window_attention(q, k, v, window=None, sinks=0, lengths=None):
-    """q [Z, S, H, D], k, v [Z, S, K, D] (CPU) -> output and sum w |v|, [Z, S, H, D]."""
+    """q [Z, S, H, D], k, v [Z, S, K, D] -> output and sum w |v|, [Z, S, H, D]."""
     Z, S, H, D = q.shape
-    out, mag = torch.zeros(Z, S, H, D, dtype=torch.float64), torch.zeros(Z, S, H, D, dtype=torch.float64)
+    out = torch.zeros(Z, S, H, D, dtype=torch.float64, device=q.device)
+    mag = torch.zeros_like(out)
     for z in range(Z):
         n = S if lengths is None else int(lengths[z])
         if n == 0:
             continue
-        o, a = _attend(*(t[z, :n].transpose(0, 1) for t in (q, k, v)), window_mask(n, window, sinks))
+        o, a = _attend(*(t[z, :n].transpose(0, 1) for t in (q, k, v)), window_mask(n, window, sinks, q.device))
         out[z, :n], mag[z, :n] = o.transpose(0, 1), a.transpose(0, 1)
     return out, mag
 

@@ -378,3 +378,193 @@ def test_views_of_a_fused_projection_are_not_copied(cuda):
         assert (y.data_ptr() == t.data_ptr()) == (pitch is not None), tuple(t.shape)
         assert ld == (pitch if pitch is not None else t.shape[-2] * t.shape[-1])
         assert torch.equal(y, t)
+
+
+# ------------------------------------------- larger calls, streams, graphs, refusals
+
+
+@pytest.mark.parametrize("Z,S,H,K,D,window,sinks,ragged,dtype", [
+    (2, 1500, 40, 8, 64, None, 0, False, BF),    # several units a CTA, of all lengths
+    (3, 1300, 40, 5, 128, 300, 70, True, BF),
+    (1, 5000, 3, 1, 64, 1000, 4, False, BF),
+    (1, 5000, 3, 1, 128, 4999, 1, False, BF),
+    (150, 130, 4, 2, 64, 60, 1, True, BF),
+    (2, 1500, 6, 6, 96, 500, 2, True, F32),
+])
+def test_window_attention_many_units(cuda, Z, S, H, K, D, window, sinks, ragged, dtype):
+    g = torch.Generator(device=cuda).manual_seed(S + D)
+    x = torch.randn(Z, S, H + 2 * K, D, generator=g, device=cuda).to(dtype)
+    q, k, v = x[:, :, :H], x[:, :, H:H + K], x[:, :, H + K:]
+    lengths = _lengths(Z, S).to(cuda) if ragged else None
+    o = zg.window_attention(q, k, v, window, sinks, lengths)
+    _ok()
+    want, mag = so.window_attention(q, k, v, window, sinks, lengths)
+    so.assert_within(o, want.cpu(), so.attention_tolerance(q, k, want, mag, dtype, S).cpu())
+    for _ in range(20):  # the same bits whatever the order the blocks run in
+        assert torch.equal(zg.window_attention(q, k, v, window, sinks, lengths), o)
+    _ok()
+
+
+@pytest.mark.parametrize("B,L,H,K,D,page,window,dtype", [
+    (1, 70000, 8, 2, 128, 64, None, BF),    # more splits than a cluster holds: a kernel of its own joins them
+    (3, 20000, 4, 1, 64, 16, None, BF),
+    (40, 900, 12, 6, 192, 32, 500, BF),
+    (2, 9000, 10, 1, 96, 16, None, F32),
+    (5, 3000, 3, 3, 200, 8, 2000, F32),
+])
+def test_paged_attention_long(cuda, B, L, H, K, D, page, window, dtype):
+    g = torch.Generator().manual_seed(L + D)
+    lengths = [L - (3 * L * b) // (4 * B) for b in range(B)]
+    kp, vp, table = _pool(lengths, page, K, D, dtype, g)
+    q = _rand((B, H, D), dtype, g)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    want, mag = so.paged_attention(q, kp, vp, table, n, window, 3)
+    args = tuple(t.to(cuda) for t in (q, kp, vp, table, n))
+    o = zg.paged_attention(*args, window, 3)
+    so.assert_within(o, want, so.attention_tolerance(q, kp, want, mag, dtype, L))
+    for _ in range(5):
+        assert torch.equal(zg.paged_attention(*args, window, 3), o)
+
+
+def _step(cuda, dtype=BF, S=200, D=64):
+    """A step's inputs and the call of it."""
+    g = torch.Generator(device=cuda).manual_seed(4)
+    B, H, K, page = 3, 4, 2, 16
+    x = torch.randn(B, S, H + 2 * K, D, generator=g, device=cuda).to(dtype)
+    kp = torch.zeros(3 * 32, page, K, D, device=cuda, dtype=dtype)
+    vp = torch.zeros_like(kp)
+    table = torch.randperm(96, generator=torch.Generator().manual_seed(1)).reshape(3, 32).to(cuda, torch.int32)
+    lengths = torch.tensor([S, 17, 0], dtype=torch.int32, device=cuda)
+    pos = torch.arange(S, device=cuda)[:, None]
+
+    def run():
+        q, k = zg.rotary(x[:, :, :H], x[:, :, H:H + K], pos, (D,))
+        o = zg.window_attention(q, k, x[:, :, H + K:], 50, 2, lengths)
+        n = zg.append_pages(kp, vp, k, x[:, :, H + K:], table, torch.zeros_like(lengths), lengths)
+        return o, n, zg.paged_attention(q[:, 0], kp, vp, table, n)
+
+    return x, kp, run
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (F32, 40)])
+def test_captured_and_replayed(cuda, dtype, D):
+    """The run of them in a CUDA graph, replayed on new values, twice captured
+    at once, gives the bits of the eager calls."""
+    x, kp, run = _step(cuda, dtype, D=D)
+    run()
+    side = torch.cuda.Stream()
+    graphs = []
+    with torch.cuda.stream(side):
+        run()
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = run()
+            graphs.append((graph, out))
+    torch.cuda.synchronize()
+    for seed in (1, 2):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(device=cuda).manual_seed(seed), device=cuda))
+        want = [t.clone() for t in run()]
+        for graph, out in graphs:
+            kp.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+    _ok()
+
+
+def test_on_two_streams_at_once(cuda):
+    x, _, run = _step(cuda, S=300)
+    want = run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    steps = [_step(cuda, S=300) for _ in streams]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for s, (_, _, r) in zip(streams, steps):
+            with torch.cuda.stream(s):
+                outs.append(r())
+    torch.cuda.synchronize()
+    for o in outs:
+        for a, b in zip(o, want):
+            assert torch.equal(a, b)
+
+
+def test_in_inference_mode_and_with_gradients_asked(cuda):
+    """Serving under inference_mode; and an op of tensors that require grad gives
+    its values, but has no backward pass (evolution strategies take no gradients)."""
+    _, _, run = _step(cuda)
+    want = run()
+    with torch.inference_mode():
+        _, _, again = _step(cuda)
+        for a, b in zip(again(), want):
+            assert torch.equal(a, b)
+    q = torch.randn(1, 5, 2, 64, device=cuda, requires_grad=True)
+    o = zg.window_attention(q, q, q)
+    assert torch.equal(o.detach(), zg.window_attention(*[q.detach()] * 3))
+    with pytest.raises(RuntimeError):
+        o.sum().backward()
+
+
+def test_append_is_seen_as_an_in_place_change(cuda):
+    kp = torch.zeros(2, 4, 1, 8, device=cuda)
+    v0 = kp._version
+    t = torch.ones(1, 1, 1, 8, device=cuda)
+    zg.append_pages(kp, torch.zeros_like(kp), t, t, torch.zeros(1, 1, dtype=torch.int32, device=cuda),
+                    torch.zeros(1, dtype=torch.int32, device=cuda))
+    assert kp._version > v0
+
+
+def test_refusals(cuda):
+    q = torch.zeros(2, 5, 4, 64, device=cuda, dtype=BF)
+    k = torch.zeros(2, 5, 2, 64, device=cuda, dtype=BF)
+    pos = torch.zeros(5, 1, dtype=torch.int64, device=cuda)
+    kp = torch.zeros(4, 8, 2, 64, device=cuda, dtype=BF)
+    table = torch.zeros(2, 3, dtype=torch.int32, device=cuda)
+    n = torch.zeros(2, dtype=torch.int32, device=cuda)
+    bad = [
+        (ValueError, lambda: zg.rotary(q, k[:, :3], pos, (64,))),
+        (ValueError, lambda: zg.rotary(q, k, pos, (63,))),
+        (ValueError, lambda: zg.rotary(q, k, pos, ())),
+        (ValueError, lambda: zg.rotary(q, k, pos, (66,))),
+        (ValueError, lambda: zg.rotary(q, k, pos, (32, 32))),
+        (ValueError, lambda: zg.rotary(q, k, pos[:3], (64,))),
+        (ValueError, lambda: zg.rotary(q, k, pos, (64,), base=-1.0)),
+        (ValueError, lambda: zg.rotary(q, k, pos, (64,), base=math.nan)),
+        (TypeError, lambda: zg.rotary(q, k, pos.to(torch.int16), (64,))),
+        (TypeError, lambda: zg.rotary(q.half(), k.half(), pos, (64,))),
+        (ValueError, lambda: zg.window_attention(q, k, k[:, :4])),
+        (ValueError, lambda: zg.window_attention(q[:, :, :3], k, k)),
+        (ValueError, lambda: zg.window_attention(q, k, k, window=0)),
+        (ValueError, lambda: zg.window_attention(q, k, k, window=4, sinks=-1)),
+        (ValueError, lambda: zg.window_attention(q, k, k, lengths=n[:1])),
+        (TypeError, lambda: zg.window_attention(q, k, k, lengths=n.float())),
+        (TypeError, lambda: zg.window_attention(q.double(), k.double(), k.double())),
+        (L.ZgLibraryError, lambda: zg.window_attention(*[torch.zeros(1, 2, 1, 300, device=cuda)] * 3)),
+        (L.ZgLibraryError, lambda: zg.window_attention(q.cpu(), k.cpu(), k.cpu())),
+        (ValueError, lambda: zg.append_pages(kp, kp[:3], k, k, table, n)),
+        (ValueError, lambda: zg.append_pages(kp[:, ::2], kp[:, ::2], k, k, table, n)),
+        (ValueError, lambda: zg.append_pages(kp, kp, q, q, table, n)),
+        (TypeError, lambda: zg.append_pages(kp, kp, k.float(), k.float(), table, n)),
+        (ValueError, lambda: zg.append_pages(kp, kp, k, k, table[:1], n)),
+        (ValueError, lambda: zg.append_pages(kp, kp, k, k, table, n, counts=n[:1])),
+        (TypeError, lambda: zg.append_pages(kp, kp, k, k, table.float(), n)),
+        (ValueError, lambda: zg.paged_attention(q[:, 0, :3], kp, kp, table, n)),
+        (TypeError, lambda: zg.paged_attention(q[:, 0].float(), kp, kp, table, n)),
+        (ValueError, lambda: zg.paged_attention(q[:, 0], kp, kp, table, n[:1])),
+        (ValueError, lambda: zg.paged_attention(q[:, 0], kp, kp, table, n, window=-3)),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+
+
+def test_wide_integers_do_not_wrap(cuda):
+    """A length or page number beyond 32 bits is refused as itself, not as what is left of it."""
+    kp = torch.ones(4, 8, 1, 64, device=cuda, dtype=BF)
+    q = torch.ones(2, 1, 64, device=cuda, dtype=BF)
+    table = torch.zeros(2, 2, dtype=torch.int64, device=cuda)
+    table[1, 0] = 2 ** 32
+    o = zg.paged_attention(q, kp, kp, table, torch.tensor([2 ** 32 + 3, 3], device=cuda))
+    assert torch.isnan(o).all()

@@ -31,15 +31,18 @@ from ._ops import _NS, _movedim0
 
 _INT_MAX = 2 ** 31 - 1
 _POSITION_CODES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-_no_transform = torch._C._functorch.peek_interpreter_stack
-_no_mode = torch._C._len_torch_dispatch_stack
+# what _plain_call asks; without one of them every call takes the dispatcher's way
+_transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", None)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
+_tracing = getattr(torch._C, "_get_tracing_state", None)
+_ask = _transform is not None and _modes is not None and _tracing is not None
 
 
 def _plain_call(*ts) -> bool:
     """True when a call needs none of what the dispatcher adds (vmap, an
     autograd error, a tracing mode): the op is then launched without it,
     which a single token's call notices (about 20 us of host time)."""
-    if _no_transform() is not None or _no_mode() or torch.compiler.is_compiling():
+    if not _ask or _transform() is not None or _modes() or _tracing() is not None or torch.compiler.is_compiling():
         return False
     grad = torch.is_grad_enabled()
     for t in ts:

@@ -731,7 +731,8 @@ size_t paged_workspace(const PagedPlan& p, int64_t B, int K, int D) {
 }
 
 bool paged_sizes_ok(int64_t n_pages, int page, int64_t B, int H, int K, int D, int max_pages) {
-    return n_pages >= 0 && page >= 1 && B >= 0 && H >= 1 && K >= 1 && D >= 1 && max_pages >= 0 && H % K == 0;
+    return n_pages >= 0 && page >= 1 && B >= 0 && H >= 1 && K >= 1 && D >= 1 && max_pages >= 0 && H % K == 0 &&
+           B <= INT32_MAX / H;
 }
 
 template <typename F>
@@ -831,7 +832,8 @@ extern "C" int zg_append_pages(void* k_pages, void* v_pages, int64_t n_pages, in
 
 extern "C" size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int D, int max_pages, int page,
                                                     int window, int sinks, int dtype) {
-    if (!paged_sizes_ok(0, page, B, H, K, D, max_pages) || D > 256 || window < 0 || sinks < 0 || !zg::dtype_ok(dtype))
+    if (!paged_sizes_ok(0, page, B, H, K, D, max_pages) || B == 0 || D > 256 || window < 0 || sinks < 0 ||
+        !zg::dtype_ok(dtype))
         return 0;
     return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), B, K, D);
 }
@@ -856,7 +858,7 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
     if (need && (!workspace || workspace_bytes < need))
         return zg::fail(ZG_ERR_WORKSPACE, "zg_paged_attention: workspace of %zu bytes needed", need);
     const int64_t blocks = B * K * p.row_tiles * p.splits;
-    if (blocks > INT32_MAX || B * H > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: too many rows");
+    if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: too many rows");
     const int n = 16 / (int)zg::dtype_size(dtype);
     const int vec = D % n == 0 && aligned16(k_pages) && aligned16(v_pages);
     PagedArgs a{q, k_pages, v_pages, table, lengths, o, static_cast<float*>(workspace), ldq, n_pages, page, max_pages,

@@ -568,3 +568,62 @@ def test_wide_integers_do_not_wrap(cuda):
     table[1, 0] = 2 ** 32
     o = zg.paged_attention(q, kp, kp, table, torch.tensor([2 ** 32 + 3, 3], device=cuda))
     assert torch.isnan(o).all()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 72), (F32, 64)])
+def test_window_attention_not_finite_inputs(cuda, dtype, D):
+    """NaN and infinite keys and values reach exactly the rows that see them,
+    NaN queries their own row; all-NaN activations cost no more than others."""
+    Z, S, H, K = 2, 700, 4, 2
+    g = torch.Generator(device=cuda).manual_seed(D)
+    q, k, v = (torch.randn(Z, S, h, D, generator=g, device=cuda).to(dtype) for h in (H, K, K))
+    q[0, 5, 1] = math.nan
+    k[0, 300, 0, 3] = math.nan
+    v[0, 301, 1, 7] = math.inf
+    v[1, 650, 0, 2] = -math.inf
+    v[1, 651, 0, 2] = math.inf
+    k[1, 100, 1] = 0.0
+    k[1, 100, 1, 0] = math.inf
+    for window, sinks in ((None, 0), (60, 2), (100, 310)):
+        o = zg.window_attention(q, k, v, window, sinks)
+        want, mag = so.window_attention(q, k, v, window, sinks)
+        assert torch.isnan(want).any() and torch.isinf(want).any()
+        so.assert_within(o, want.cpu(), so.attention_tolerance(q, k, want, mag, dtype, S).cpu())
+    nan = torch.full_like(q, math.nan)
+    assert torch.isnan(zg.window_attention(nan, nan[:, :, :K], nan[:, :, :K], 100, 2)).all()
+    _ok()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_window_attention_padding_of_any_bits(cuda, D):
+    """Long padded sequences whose padding holds NaN: as fast and the same bits as with zeros there."""
+    Z, S, H = 3, 6000, 4
+    g = torch.Generator(device=cuda).manual_seed(D)
+    q, k, v = (torch.randn(Z, S, H, D, generator=g, device=cuda).to(BF) for _ in range(3))
+    lengths = torch.tensor([5873, 129, 4001], device=cuda)
+    for t in (q, k, v):
+        for z, n in enumerate(lengths.tolist()):
+            t[z, n:] = 0
+    want = zg.window_attention(q, k, v, lengths=lengths)
+    for t in (q, k, v):
+        for z, n in enumerate(lengths.tolist()):
+            t[z, n:] = math.nan
+    assert torch.equal(zg.window_attention(q, k, v, lengths=lengths), want)
+    _ok()
+
+
+def test_window_attention_rows_formed_again_in_a_long_sequence(cuda):
+    """An infinite value late in a long sequence: the rows of its block that do
+    not see it are formed again, for longer than the kernel's waits last."""
+    S, D = 60000, 64
+    g = torch.Generator(device=cuda).manual_seed(2)
+    q, k, v = (torch.randn(1, S, 1, D, generator=g, device=cuda).to(BF) for _ in range(3))
+    want = zg.window_attention(q, k, v)
+    at = 59990
+    v[0, at] = math.inf
+    o = zg.window_attention(q, k, v)
+    _ok()
+    assert torch.isinf(o[0, at:]).all() and torch.isfinite(o[0, :at]).all()
+    # each is off by 2^-8 sum w |v| + 2^-8 |o| at most (float32's part is far below)
+    err = (o[0, :at].double() - want[0, :at].double()).abs()
+    assert float(err.max()) <= 2 * 2.0 ** -7 * float(v[0, :at].abs().max())

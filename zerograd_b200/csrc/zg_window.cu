@@ -49,9 +49,12 @@ __device__ __forceinline__ int length_of(const WindowArgs& a, int z) {
 __device__ __forceinline__ bool sees(const WindowArgs& a, int i, int j) { return i - j < a.window || j < a.sinks; }
 
 // One output row by one warp, each visible key on its own in float32: what
-// the tiled kernels fall back to for a row that came out not finite.  A key
-// or value of a masked place that is infinite or NaN has a weight of zero,
-// and a tile's product would turn 0 * inf into NaN; here it is not read.
+// the tiled kernels fall back to for a row whose weights have a finite sum
+// and whose outputs are not all finite.  A value of a masked place that is
+// infinite or NaN has a weight of zero, and a tile's product turns 0 * inf
+// into NaN; here it is not read.  (A sum that is not finite, or zero, comes
+// of visible scores alone: all of the row is NaN, and stays as it is, so that
+// a candidate whose activations are all NaN costs nothing here.)
 template <typename T>
 __device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h) {
     const int lane = threadIdx.x % 32;
@@ -68,26 +71,44 @@ __device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h
         x[e] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j <= i; ++j) {
-        if (!sees(a, i, j)) {
-            j = i - a.window;  // the window's first position is next
+    // four positions at a time, their reads in flight together
+    for (int j0 = 0; j0 <= i; j0 += 4) {
+        if (!sees(a, i, j0) && !sees(a, i, j0 + 3 < i ? j0 + 3 : i)) {
+            j0 = i - a.window - 3;  // the window's first position is next
             continue;
         }
-        float s = 0.f;
+        float s[4], n = m;
+        bool on[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = lane + 32 * e;
-            if (d < a.D) s = fmaf(qv[e], zg_to_float(k[j * a.ldk + d]), s);
+        for (int g = 0; g < 4; ++g) {
+            on[g] = j0 + g <= i && sees(a, i, j0 + g);
+            s[g] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = lane + 32 * e;
+                if (on[g] && d < a.D) s[g] = fmaf(qv[e], zg_to_float(k[(j0 + g) * a.ldk + d]), s[g]);
+            }
         }
 #pragma unroll
-        for (int f = 16; f > 0; f >>= 1) s += __shfl_xor_sync(0xffffffffu, s, f);
-        const float n = fmaxf(m, s), base = n == -INFINITY ? 0.f : n;
-        const float c = exp2f(m - base), p = exp2f(s - base);
-        l = fmaf(l, c, p);
+        for (int g = 0; g < 4; ++g) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = lane + 32 * e;
-            if (d < a.D) x[e] = fmaf(p, zg_to_float(v[j * a.ldv + d]), x[e] * c);
+            for (int f = 16; f > 0; f >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], f);
+            s[g] = on[g] ? s[g] : -INFINITY;
+            n = fmaxf(n, s[g]);
+        }
+        const float base = n == -INFINITY ? 0.f : n, c = exp2f(m - base);
+        l *= c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= c;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float p = exp2f(s[g] - base);
+            l += p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int d = lane + 32 * e;
+                if (on[g] && d < a.D) x[e] = fmaf(p, zg_to_float(v[(j0 + g) * a.ldv + d]), x[e]);
+            }
         }
         m = n;
     }
@@ -287,13 +308,14 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
         }
         __syncthreads();  // the values have been read
     }
-    unsigned redo = 0;  // bit i: row i of this half warp is not finite
+    unsigned redo = 0;  // bit i: row i of this half warp is formed again
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int f = 8; f > 0; f >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], f);
         const int qi = i0 + ty + 8 * i;
         bool fine = true;
+        const bool known = l[i] > 0.f && l[i] < INFINITY;  // else all NaN, by its visible scores
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -306,7 +328,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
                 }
             }
         const unsigned half = 0xffffu << (threadIdx.x % 32 / 16 * 16);
-        if (__ballot_sync(0xffffffffu, !fine) & half) redo |= 1u << i;
+        if (__ballot_sync(0xffffffffu, known && !fine) & half) redo |= 1u << i;
     }
     // the rows of this warp's two halves, one at a time by the whole warp
     for (int t = 0; t < 2; ++t) {
@@ -349,22 +371,29 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 //
 // A persistent CTA per SM, 384 threads: warp 0 issues the TMA loads, warps
 // 1 and 2 the MMAs of a tile each, warps 4-7 and 8-11 are the softmax groups
-// of two tiles of 128 query rows (one thread a row).  A work unit is a pair of
-// neighbouring tiles of one (z, head), so that each block of 64 keys and
-// values is fetched once for both; the units with the most visible keys come
-// first.  Per block and tile: S = Q K^T into TMEM (M = 128, N = 64), a row's
-// maximum, the weights p = 2^(s - m) as bf16 back into TMEM over the scores,
-// O += P V with P read from TMEM.  Only blocks that a tile sees any key of are
-// visited, only those at the edge of a warp's mask test each key, and a warp
-// whose rows see none of a block's keys writes its zero weights at once.
+// of two tiles of 128 query rows (one thread a row); warp 3 fills the group of
+// four that setmaxnreg speaks to.  A work unit is a pair of neighbouring tiles
+// of one (z, head), so that each block of keys and values is fetched once for
+// both; the units with the most visible keys come first.  Per block and tile:
+// S = Q K^T into TMEM (M = 128, N = KEYS), a row's maximum, the weights
+// p = 2^(s - m) as bf16 back into TMEM, O += P V with P read from TMEM.  Only
+// blocks that a tile sees any key of are visited, and only those at the edge
+// of a warp's mask test each key.
 //
-// TMEM (512 columns): O of the two tiles; scores, one buffer of 64 columns a
-// tile with DP = 128 and two with DP = 64; weights, two buffers of 32 columns a
-// tile.  A group reads a block's scores into registers and says so, and the
-// next block's Q K^T runs under its softmax; the weights have columns of their
-// own, so that they do not hold it up.  (Weights over the scores they came
+// TMEM (512 columns): O of the two tiles, and of each tile one buffer of
+// scores and weights of their own columns: with DP = 64 blocks of 128 keys
+// (128 + 64 columns), with DP = 128, where O takes twice as much, blocks of 64
+// keys and two buffers of weights (64 + 2 * 32).  A group reads a block's
+// scores into registers and says so, and the next block's Q K^T runs under its
+// softmax; the weights do not hold it up.  (Weights over the scores they came
 // from, the next Q K^T behind P V: 2100 clocks a block of 64 at D = 128, 600 of
-// them waiting for scores.)
+// them waiting for scores.  Blocks of 64 keys at D = 64: each block's signals
+// between the roles cost what its exponentials do.)
+//
+// What bounds it is a group's exponentials, 16 a clock and SM, and the waits
+// around them; the MMAs take about half as long.  2 x 4096 tokens of 12 heads
+// (4 key heads) of 64, causal: 95 us, 0.54 PFLOP/s of the visible pairs; 8192
+// tokens of 16 heads (4) of 128 under a window of 1024: 99 us, 0.65 PFLOP/s.
 //
 // The maximum m that weights are taken against is moved, and O rescaled by
 // its group, only when a row's true maximum is more than 2^8 above it: the
@@ -402,8 +431,13 @@ struct WtShape {
 struct WtCtrl {
     uint64_t q_full[2], q_empty[2], kv_full[5], kv_empty[5], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2], done;
     uint32_t tmem_base;
+    uint32_t redo[8];  // of each softmax warp: rows are marked to be formed again
 };
 static_assert(sizeof(WtCtrl) <= 512, "control block");
+
+// What stands in column 0 of a row that is to be formed again: a NaN that no
+// rounding gives.
+constexpr uint16_t WT_REDO = 0x7fa5;
 
 // A unit as the role of tile t sees it: two tiles of 128 rows from i0, the
 // blocks of keys that either sees (first .. hi, next() from one to the next)
@@ -515,6 +549,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     WtCtrl& c = *reinterpret_cast<WtCtrl*>(smem + W::CTRL);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    if (threadIdx.x < 8) c.redo[threadIdx.x] = 0u;
     if (threadIdx.x == 0) {
         mbar_init(&c.done, 2);  // both issuers
         for (int i = 0; i < W::STAGES; ++i) {
@@ -606,11 +641,21 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             int vblock = -1;       // and the number of their block
             auto outputs = [&]() {
                 const uint32_t st = vstage;
+                const uint32_t va = ring + st * 2 * W::BLOCK + W::BLOCK;
+                if (x.n < a.S && (vblock + 1) * W::KEYS > x.n) {
+                    // rows of a padded batch behind this sequence: their weights are
+                    // zeros, and so are their values then, whatever they hold
+                    const uint32_t r0 = (uint32_t)(x.n - vblock * W::KEYS) * 128u;
+                    for (int d = 0; d < DP / 64; ++d)
+                        for (uint32_t at = r0 + lane * 16; at < W::BOX; at += 512)
+                            *reinterpret_cast<uint4*>(smem + (va - smem_u32(smem)) + d * W::BOX + at) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
                 if (!warp_wait(&c.p_full[t][npv & 1], (npv >> 1) & 1, 104)) return false;
                 // the last unit's outputs have been read
                 if (!started && !warp_wait(&c.o_empty[t], (nu & 1) ^ 1, 105)) return false;
                 tc_fence_after();
-                const uint32_t va = ring + st * 2 * W::BLOCK + W::BLOCK;
 #pragma unroll
                 for (int k = 0; k < W::KEYS / 16; ++k)
                     umma_ts_elect(tmem + W::o_col(t), tmem + W::p_col(t, npv) + k * 8, smem_desc(va + k * 2048, W::BOX, 1024),
@@ -698,7 +743,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (!all_seen && !warp_wait(&c.pv_done[t], (nb - 1) & 1, 112)) return false;
                         tc_fence_after();
                     }
-                    if (!__any_sync(0xffffffffu, !(mx <= m + 8.f))) return true;
+                    if (!__any_sync(0xffffffffu, i < x.n && !(mx <= m + 8.f))) return true;  // rows behind the sequence do not count
                     const float n = fmaxf(m, mx);
                     float f = exp2_fast(m - (n == -INFINITY ? 0.f : n));
                     // a score that is NaN or infinite: the row is formed again at the end
@@ -839,7 +884,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (!(ok = warp_wait(&c.o_full[t], nu & 1, 113))) break;
             ++nu;
             tc_fence_after();
-            const float inv = 1.f / ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+            const float l = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), inv = 1.f / l;
             const bool in = i < x.n;
             bool fine = true;
 #pragma unroll 1
@@ -861,11 +906,24 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             tc_fence_before();
             mbar_arrive(&c.o_empty[t]);
-            for (uint32_t rows = __ballot_sync(0xffffffffu, !fine); rows; rows &= rows - 1) {
-                __syncwarp();  // the row's first values are written before these
-                window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
+            if (!fine && l > 0.f && l < INFINITY) {
+                *reinterpret_cast<uint16_t*>(o) = WT_REDO;
+                c.redo[warp - 4] = 1u;
             }
         }
+        // The marked rows, when no role waits for this one any more: a row of
+        // 10^5 keys takes longer than the waits' limit.
+        __syncwarp();
+        if (ok && c.redo[warp - 4])
+            for (int64_t it = 0; it * gridDim.x < units; ++it) {
+                const int64_t u = wt_order(it);
+                if (u >= units) continue;
+                const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
+                const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;
+                const uint16_t* o = static_cast<const uint16_t*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
+                for (uint32_t rows = __ballot_sync(0xffffffffu, i < x.n && *o == WT_REDO); rows; rows &= rows - 1)
+                    window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
+            }
     }
     tc_fence_before();
     __syncthreads();
@@ -904,7 +962,7 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
 
 namespace zg {
 
-// Timed-out waits of the tensor-core kernel (codes 101-109, 111-113) or its
+// Timed-out waits of the tensor-core kernel (codes 101-108, 111-113) or its
 // shared memory not 1024-aligned (110); 0 = none.
 int window_error_word(int clear) { return ptx_error_word(clear); }
 

@@ -132,7 +132,11 @@ __device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h
 // neighbouring rows fall into different banks.  Float32 rows come by cp.async,
 // the next tile's keys under this one's second product and its values under
 // the next first one; others are converted on the way, a tile's words in
-// flight together.
+// flight together.  Of a tile at the edge of the mask only those sixteens of
+// keys are multiplied that any row sees: 3 x 777 tokens of 8 heads of 80 under
+// a window of 200, 65 -> 52 us.  What bounds it is the FMA pipe and the shared
+// memory reads that feed it, both over half busy: causal, 2048 tokens of 8
+// heads of 128, 274 us, 31 TFLOP/s of the visible pairs.
 // ---------------------------------------------------------------------------
 constexpr int WF_M = 32, WF_N = 64, WF_THREADS = 128, WF_PP = WF_N + 4;
 
@@ -230,66 +234,76 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
         load(k_rows, vs, v, a.ldv, j0);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
         __syncthreads();
-        float2 s2[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s2[i][j] = zero2;
-#pragma unroll 4
-        for (int d = 0; d < DP; d += 4) {
-            float4 qv[4], kv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * PITCH + d);
-                kv[i] = *reinterpret_cast<const float4*>(ks + (tx + 16 * i) * PITCH + d);
-            }
+        // the sixteens of this tile's keys that any row sees: [g0, g1)
+        int lo = i0 - a.window + 1 - j0, hi = last - j0;
+        if (lo <= 0 || j0 < a.sinks) lo = 0;
+        if (i0 - a.window + 1 - j0 >= WF_N) hi = a.sinks - j0;  // sinks alone
+        const int g0 = lo / 16, g1 = hi >= WF_N ? 4 : (hi + 15) / 16;
+        // the scores of NG sixteens, and their softmax into ps
+        auto scores = [&](auto groups) {
+            constexpr int NG = decltype(groups)::value;
+            const float* kr = ks + (16 * g0 + tx) * PITCH;
+            float2 s2[4][NG];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s2[i][j] = ffma2_tc(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
-                    s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+                for (int j = 0; j < NG; ++j) s2[i][j] = zero2;
+#pragma unroll 2
+            for (int d = 0; d < DP; d += 4) {
+                float4 qv[4], kv[NG];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * PITCH + d);
+#pragma unroll
+                for (int j = 0; j < NG; ++j) kv[j] = *reinterpret_cast<const float4*>(kr + 16 * j * PITCH + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) {
+                        s2[i][j] = ffma2_tc(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+                        s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+                    }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
+            __syncthreads();
+            if (next(kt) < kt_end)
+                load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
+            else
+                asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int qi = i0 + ty + 8 * i;
+                float s[NG], t = m[i];
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
+                    const int kj = j0 + 16 * (g0 + j) + tx;
+                    s[j] = kj <= qi && kj < n && sees(a, qi, kj) ? (s2[i][j].x + s2[i][j].y) * a.scale : -INFINITY;
+                    t = fmaxf(t, s[j]);
                 }
-        }
-        float s[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+                for (int f = 8; f > 0; f >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, f));
+                const float base = t == -INFINITY ? 0.f : t;
+                const float c = exp2f(m[i] - base);
+                m[i] = t;
+                l[i] *= c;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
-        asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
-        __syncthreads();
-        if (next(kt) < kt_end)
-            load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
-        else
-            asm volatile("cp.async.commit_group;" ::: "memory");
+                for (int j = 0; j < NG; ++j) {
+                    const float p = exp2f(s[j] - base);
+                    l[i] += p;
+                    ps[(ty + 8 * i) * WF_PP + 16 * (g0 + j) + tx] = p;
+                }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int qi = i0 + ty + 8 * i;
-            float t = m[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int kj = j0 + tx + 16 * j;
-                s[i][j] = kj <= qi && kj < n && sees(a, qi, kj) ? s[i][j] * a.scale : -INFINITY;
-                t = fmaxf(t, s[i][j]);
+                for (int e = 0; e < NC; ++e) x[i][e] = ffma2_tc(x[i][e], make_float2(c, c), zero2);
             }
-#pragma unroll
-            for (int f = 8; f > 0; f >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, f));
-            const float base = t == -INFINITY ? 0.f : t;
-            const float c = exp2f(m[i] - base);
-            m[i] = t;
-            l[i] *= c;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float p = exp2f(s[i][j] - base);
-                l[i] += p;
-                ps[(ty + 8 * i) * WF_PP + tx + 16 * j] = p;
-            }
-#pragma unroll
-            for (int e = 0; e < NC; ++e) x[i][e] = ffma2_tc(x[i][e], make_float2(c, c), zero2);
+        };
+        switch (g1 - g0) {
+            case 4: scores(std::integral_constant<int, 4>{}); break;
+            case 3: scores(std::integral_constant<int, 3>{}); break;
+            case 2: scores(std::integral_constant<int, 2>{}); break;
+            default: scores(std::integral_constant<int, 1>{});
         }
         __syncwarp();  // a row's weights are written and read by the same half warp
 #pragma unroll 2
-        for (int j = 0; j < WF_N; j += 4) {
+        for (int j = 16 * g0; j < 16 * g1; j += 4) {
             float4 pv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 8 * i) * WF_PP + j);
@@ -369,7 +383,7 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 // Tensor-core path: bf16, D <= DP (64 or 128, zeros behind D).
 //
-// A persistent CTA per SM, 384 threads: warp 0 issues the TMA loads, warps
+// A CTA per SM, which takes unit after unit, 384 threads: warp 0 issues the TMA loads, warps
 // 1 and 2 the MMAs of a tile each, warps 4-7 and 8-11 are the softmax groups
 // of two tiles of 128 query rows (one thread a row); warp 3 fills the group of
 // four that setmaxnreg speaks to.  A work unit is a pair of neighbouring tiles
@@ -392,8 +406,8 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 //
 // What bounds it is a group's exponentials, 16 a clock and SM, and the waits
 // around them; the MMAs take about half as long.  2 x 4096 tokens of 12 heads
-// (4 key heads) of 64, causal: 95 us, 0.54 PFLOP/s of the visible pairs; 8192
-// tokens of 16 heads (4) of 128 under a window of 1024: 99 us, 0.65 PFLOP/s.
+// (4 key heads) of 64, causal: 83 us, 0.62 PFLOP/s of the visible pairs; 8192
+// tokens of 16 heads (4) of 128 under a window of 1024: 87 us, 0.74 PFLOP/s.
 //
 // The maximum m that weights are taken against is moved, and O rescaled by
 // its group, only when a row's true maximum is more than 2^8 above it: the
@@ -428,15 +442,17 @@ struct WtShape {
 // ones), so each has a barrier; and that a block's scores are there says, by
 // the order of the issuer's commits, that P V of two blocks before is done.
 // With one buffer a group waits for P V of the block before.
-struct WtCtrl {
+struct alignas(16) WtCtrl {
+    uint4 unit[4];  // answers to the requests for the next unit
+    uint64_t unit_full[4], unit_empty[4];
     uint64_t q_full[2], q_empty[2], kv_full[5], kv_empty[5], s_full[2], s_read[2], p_full[2][2], pv_done[2], o_full[2], o_empty[2], done;
     uint32_t tmem_base;
-    uint32_t redo[8];  // of each softmax warp: rows are marked to be formed again
+    int redo[8];  // of each softmax warp: the last unit with rows to be formed again
 };
 static_assert(sizeof(WtCtrl) <= 512, "control block");
 
 // What stands in column 0 of a row that is to be formed again: a NaN that no
-// rounding gives.
+// rounding gives.  Columns 2 and 3 hold the warp's unit before with such rows.
 constexpr uint16_t WT_REDO = 0x7fa5;
 
 // A unit as the role of tile t sees it: two tiles of 128 rows from i0, the
@@ -452,13 +468,11 @@ struct WtUnit {
 };
 
 template <int KEYS>
-__device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int64_t u, int pairs, int t) {
+__device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int u, int pairs, int t) {
     WtUnit x;
-    const int64_t zh_count = (int64_t)a.Z * a.H;
-    const int pair = pairs - 1 - (int)(u / zh_count);
-    const int64_t zh = u % zh_count;
-    x.z = (int)(zh / a.H);
-    x.h = (int)(zh % a.H);
+    const int heads = a.Z * a.H, pair = pairs - 1 - u / heads, zh = u % heads;
+    x.z = zh / a.H;
+    x.h = zh % a.H;
     x.n = length_of(a, x.z);
     x.i0 = pair * 256;
     x.any = x.i0 < x.n;
@@ -473,10 +487,31 @@ __device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int64_t u, int pa
     return x;
 }
 
-// The i-th unit of a CTA: rows of gridDim.x units taken there and back, so
-// that the shorter units of a row go to the CTAs that had the longer ones.
-__device__ __forceinline__ int64_t wt_order(int64_t i) {
-    return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+// Units are the blocks of the grid, and a CTA that has taken one asks for the
+// next that no CTA has started, so that the CTAs end together whatever the
+// sequences' lengths are.  (Units dealt out beforehand, in rows there and back,
+// against this: 2 x 4096 causal 95 -> 83 us; 8192 under a window of 1024 102 ->
+// 87 us; 16 padded sequences of up to 1000 under a window of 100 52 -> 42 us.)
+// The loader asks, and every role reads the answer.
+__device__ __forceinline__ void unit_request(uint4* to, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(to)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The unit of an answer, -1 when there is none left.
+__device__ __forceinline__ int unit_answer(const uint4* from) {
+    int u;
+    asm volatile(
+        "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 h, [%1];\n\t"
+        "mov.b32 %0, -1;\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+        : "=r"(u)
+        : "r"(smem_u32(from))
+        : "memory");
+    return u;
 }
 
 // Bits 0 .. x of a word.
@@ -503,6 +538,16 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// The unit that follows a role's k-th: -1 for none, or when the wait ran out.
+__device__ __forceinline__ int unit_after(WtCtrl& c, uint32_t k, bool& ok) {
+    if (!ok || !(ok = warp_wait(&c.unit_full[k % 4], (k / 4) & 1, 109))) return -1;
+    const int u = unit_answer(&c.unit[k % 4]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) mbar_arrive(&c.unit_empty[k % 4]);
+    return __shfl_sync(0xffffffffu, u, 0);
 }
 
 // MMAs and commits issued by one elected lane of a converged warp, always the
@@ -538,7 +583,7 @@ __device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
 template <int DP>
 __global__ void __launch_bounds__(WT_THREADS, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                 const __grid_constant__ CUtensorMap tmV, const WindowArgs a, int pairs, int64_t units) {
+                 const __grid_constant__ CUtensorMap tmV, const WindowArgs a, int pairs) {
     using W = WtShape<DP>;
     // No static shared memory, so the dynamic block starts at the CTA's first
     // shared byte; the swizzled tiles need it 1024-aligned, which is checked.
@@ -549,9 +594,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     WtCtrl& c = *reinterpret_cast<WtCtrl*>(smem + W::CTRL);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-    if (threadIdx.x < 8) c.redo[threadIdx.x] = 0u;
+    if (threadIdx.x < 8) c.redo[threadIdx.x] = -1;
     if (threadIdx.x == 0) {
         mbar_init(&c.done, 2);  // both issuers
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&c.unit_full[i], 1);
+            mbar_init(&c.unit_empty[i], 10);  // the issuers and the softmax warps
+        }
         for (int i = 0; i < W::STAGES; ++i) {
             mbar_init(&c.kv_full[i], 1);
             mbar_init(&c.kv_empty[i], 2);
@@ -580,11 +629,18 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == 0) {
         if (lane == 0) {
             // blocks and query tiles loaded; a stage's parity follows from the count
-            uint32_t nk = 0, nq[2] = {0, 0};
+            uint32_t nk = 0, nq[2] = {0, 0}, nr = 0;
             bool ok = true;
-            for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
-                const int64_t u = wt_order(it);
-                if (u >= units) continue;
+            // the next unit, asked for when this one's blocks are on their way
+            auto request = [&]() {
+                uint64_t* full = &c.unit_full[nr % 4];
+                if (!ok || !(ok = mbar_wait(&c.unit_empty[nr % 4], ((nr / 4) & 1) ^ 1, 114))) return -1;
+                mbar_expect_tx(full, 16);
+                unit_request(&c.unit[nr % 4], full);
+                if (!(ok = mbar_wait(full, (nr / 4) & 1, 115))) return -1;
+                return unit_answer(&c.unit[nr++ % 4]);
+            };
+            for (int u = blockIdx.x; u >= 0; u = request()) {
                 const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, 0);
                 if (!x.any) continue;
                 const int kh = x.h / a.G;
@@ -627,11 +683,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int t = warp - 1;
         const uint32_t idesc_s = idesc_bf16(128, W::KEYS, 0), idesc_o = idesc_bf16(128, DP, 1);
         const uint32_t qa = smem_u32(smem + t * W::QTILE), ring = smem_u32(smem + W::RING);
-        uint32_t nk = 0, ns = 0, npv = 0, nu = 0;  // blocks, and of this tile scores, outputs, units
+        uint32_t nk = 0, ns = 0, npv = 0, nu = 0, taken = 0;  // blocks, and of this tile scores, outputs, units
         bool ok = true;
-        for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
-            const int64_t u = wt_order(it);
-            if (u >= units) continue;
+        for (int u = blockIdx.x; u >= 0; u = unit_after(c, taken++, ok)) {
             const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
             if (!x.any) continue;
             if (x.last >= 0 && !(ok = warp_wait(&c.q_full[t], nu & 1, 103))) break;
@@ -709,12 +763,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t oc = trow + W::o_col(t);
         const int64_t ldo = (int64_t)a.H * a.D;
         const float2 one2 = make_float2(1.f, 1.f), scale2 = make_float2(a.scale, a.scale);
-        uint32_t nb = 0, nu = 0;  // blocks and units of this tile so far
-        bool s_ready = false;     // the next scores have been seen to be there
+        uint32_t nb = 0, nu = 0, taken = 0;  // blocks and units of this tile so far, units of both
+        bool s_ready = false;                // the next scores have been seen to be there
         bool ok = true;
-        for (int64_t it = 0; ok && it * gridDim.x < units; ++it) {
-            const int64_t u = wt_order(it);
-            if (u >= units) continue;
+        for (int u = blockIdx.x; u >= 0; u = unit_after(c, taken++, ok)) {
             const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
             const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;  // the warp's first row, this thread's
             __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
@@ -906,24 +958,30 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             tc_fence_before();
             mbar_arrive(&c.o_empty[t]);
-            if (!fine && l > 0.f && l < INFINITY) {
-                *reinterpret_cast<uint16_t*>(o) = WT_REDO;
-                c.redo[warp - 4] = 1u;
+            const bool again = !fine && l > 0.f && l < INFINITY;
+            if (__any_sync(0xffffffffu, again)) {
+                int* before = &c.redo[warp - 4];
+                if (again) {
+                    *reinterpret_cast<uint16_t*>(o) = WT_REDO;
+                    *reinterpret_cast<int*>(o + 2) = *before;
+                }
+                __syncwarp();
+                if (lane == 0) *before = u;
+                __syncwarp();
             }
         }
-        // The marked rows, when no role waits for this one any more: a row of
-        // 10^5 keys takes longer than the waits' limit.
-        __syncwarp();
-        if (ok && c.redo[warp - 4])
-            for (int64_t it = 0; it * gridDim.x < units; ++it) {
-                const int64_t u = wt_order(it);
-                if (u >= units) continue;
-                const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
-                const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;
-                const uint16_t* o = static_cast<const uint16_t*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
-                for (uint32_t rows = __ballot_sync(0xffffffffu, i < x.n && *o == WT_REDO); rows; rows &= rows - 1)
-                    window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
-            }
+        // The marked rows, the last unit's first, when no role waits for this one
+        // any more: a row of 10^5 keys takes longer than the waits' limit.
+        for (int u = ok ? c.redo[warp - 4] : -1; u >= 0;) {
+            const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
+            const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;
+            const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
+            const bool again = i < x.n && *reinterpret_cast<const uint16_t*>(o) == WT_REDO;
+            const int before = again ? *reinterpret_cast<const int*>(o + 2) : -1;
+            uint32_t rows = __ballot_sync(0xffffffffu, again);
+            u = __shfl_sync(0xffffffffu, before, __ffs(rows) - 1);
+            for (; rows; rows &= rows - 1) window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -948,13 +1006,11 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
     if (cudaFuncSetAttribute(window_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM) !=
         cudaSuccess)
         return zg::fail(ZG_ERR_CUDA, "zg_window_attention: shared memory attribute");
-    int dev = 0, sms = 148;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int pairs = (a.S + 255) / 256;
     const int64_t units = (int64_t)a.Z * a.H * pairs;
+    if (units > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_window_attention: too many rows");
     zg::LaunchTimer zg_lt_("window_attention", st);
-    window_tc_kernel<DP><<<(unsigned)(units < sms ? units : sms), WT_THREADS, W::SMEM, st>>>(tq, tk, tv, a, pairs, units);
+    window_tc_kernel<DP><<<(unsigned)units, WT_THREADS, W::SMEM, st>>>(tq, tk, tv, a, pairs);
     return zg::check_launch("zg_window_attention");
 }
 
@@ -962,7 +1018,7 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
 
 namespace zg {
 
-// Timed-out waits of the tensor-core kernel (codes 101-108, 111-113) or its
+// Timed-out waits of the tensor-core kernel (codes 101-109, 111-115) or its
 // shared memory not 1024-aligned (110); 0 = none.
 int window_error_word(int clear) { return ptx_error_word(clear); }
 

@@ -45,8 +45,9 @@ __device__ __forceinline__ bool append_span(const AppendArgs& a, int b, int& sta
 
 // A warp per token, W the word that it is copied in (16 bytes, or one
 // element where a row's length or alignment does not allow that), key and
-// value words loaded before either is stored.  The warps behind the tokens'
-// own take a sequence each and write its new length.
+// value words loaded before either is stored, the first ones beside the page
+// table's entry.  The warps behind the tokens' own take a sequence each and
+// write its new length.
 template <typename W>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
     const int lane = threadIdx.x % 32;
@@ -68,28 +69,32 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
         if (lane == 0) a.new_lengths[b] = ok ? start + count : -1;
         return;
     }
-    const int b = (int)(w / a.S), s = (int)(w % a.S);
+    // (a 64-bit quotient costs some hundred instructions)
+    const int b = w <= INT32_MAX ? (int)((uint32_t)w / (uint32_t)a.S) : (int)(w / a.S), s = (int)(w - (int64_t)b * a.S);
     if (!append_span(a, b, start, count) || s >= count) return;
-    const int at = start + s;
-    const int32_t id = a.table[(int64_t)b * a.max_pages + at / a.page];
-    if (id < 0 || id >= a.n_pages) return;
-    const int64_t to = ((int64_t)id * a.page + at % a.page) * a.row;
+    const int at = start + s, p = at / a.page;
     const W* ks = static_cast<const W*>(a.k) + w * a.ldk;
     const W* vs = static_cast<const W*>(a.v) + w * a.ldv;
+    const int32_t id = a.table[(int64_t)b * a.max_pages + p];
+    W k0{}, k1{}, v0{}, v1{};
+    auto take = [&](int64_t i) {
+        if (i < a.row) k0 = ks[i], v0 = vs[i];
+        if (i + 32 < a.row) k1 = ks[i + 32], v1 = vs[i + 32];
+    };
+    take(lane);
+    if (id < 0 || id >= a.n_pages) return;
+    const int64_t to = ((int64_t)id * a.page + (at - p * a.page)) * a.row;
     W* kd = static_cast<W*>(a.kp) + to;
     W* vd = static_cast<W*>(a.vp) + to;
-    int64_t i = lane;
-    for (; i + 32 < a.row; i += 64) {
-        const W k0 = ks[i], k1 = ks[i + 32], v0 = vs[i], v1 = vs[i + 32];
-        kd[i] = k0;
-        kd[i + 32] = k1;
-        vd[i] = v0;
-        vd[i + 32] = v1;
-    }
-    if (i < a.row) {
-        const W k0 = ks[i], v0 = vs[i];
+    for (int64_t i = lane; i < a.row;) {
         kd[i] = k0;
         vd[i] = v0;
+        if (i + 32 < a.row) {
+            kd[i + 32] = k1;
+            vd[i + 32] = v1;
+        }
+        i += 64;
+        take(i);
     }
 }
 

@@ -25,12 +25,20 @@ constexpr int RO_THREADS = 128;
 
 enum { RO_POS_I32 = 0, RO_POS_I64 = 1, RO_POS_F32 = 2 };
 
+// Division of x by d as a product with ceil(2^32 / d): exact while x d < 2^32.
+struct Div {
+    uint32_t magic, one;  // one: all bits where d = 1
+    __device__ __forceinline__ int operator()(int x) const { return (int)(__umulhi((uint32_t)x, magic) + ((uint32_t)x & one)); }
+};
+Div divide_by(int64_t d) { return d == 1 ? Div{0u, ~0u} : Div{(uint32_t)(((1ull << 32) + d - 1) / d), 0u}; }
+
 struct RotaryArgs {
     const void *q, *k, *pos;
     void *q_out, *k_out;
     int64_t ldq, ldk, T, pos_rows;
     int H, K, D, A, pairs, pos_type, interleaved, tokens;  // tokens: per block
     float sign;
+    Div by_pairs, by_token, by_head;  // items of a token (0 for a token a block), and of a head
     double turns[RO_MAX_PAIRS];  // f_p / (2 pi)
     uint8_t axis[RO_MAX_PAIRS];
 };
@@ -42,7 +50,7 @@ template <typename F>
 __device__ __forceinline__ void rotary_angles(const RotaryArgs& a, int64_t t0, int nt, F put) {
     const int64_t row0 = t0 % a.pos_rows;
     for (int i = threadIdx.x; i < nt * a.pairs; i += RO_THREADS) {
-        const int tt = i / a.pairs, p = i - tt * a.pairs;
+        const int tt = a.by_pairs(i), p = i - tt * a.pairs;
         int64_t row = row0 + tt;
         while (row >= a.pos_rows) row -= a.pos_rows;
         const int64_t at = row * a.A + a.axis[p];
@@ -86,7 +94,8 @@ struct Vec16 {
 // behind the pairs are items of one word, copied.  A thread has RO_ITEMS
 // items' words on the way at a time, the first ones while the block forms its
 // angles.  336 MB of bf16 (two videos of 16384 tokens, 16 + 4 heads of 128):
-// 66 us, 5.1 TB/s; with the angles read one by one, lanes 64 bytes apart in
+// 64 us, 5.3 TB/s (66 with an item's token and head by the compiler's integer
+// divisions); with the angles read one by one, lanes 64 bytes apart in
 // shared memory, 74 us (the reads of four lanes met in a bank); persistent
 // blocks that fetch a group of tokens ahead by cp.async, 84 us (an SM's
 // instructions, not its reads in flight, are what is left).
@@ -114,8 +123,8 @@ __global__ void __launch_bounds__(RO_THREADS) rotary_vec_kernel(const __grid_con
             const int i = i0 + e * RO_THREADS + threadIdx.x;
             col[e] = -1;
             if (i >= nt * per_token) continue;
-            tt[e] = i / per_token;
-            const int r = i - tt[e] * per_token, hh = r / per_head, c = r - hh * per_head;
+            tt[e] = a.by_token(i);
+            const int r = i - tt[e] * per_token, hh = a.by_head(r), c = r - hh * per_head;
             const int64_t token = t0 + tt[e];
             const bool is_q = hh < a.H;
             const int h = is_q ? hh : hh - a.H;
@@ -204,12 +213,16 @@ int launch_rotary(RotaryArgs& a, cudaStream_t st) {
     // as many tokens a block as its threads have items in flight, fewer while
     // the grid is short of two blocks per SM
     const int pairs_of = a.interleaved ? 2 * a.pairs / N : a.pairs / N;
-    const int64_t items = vec ? (int64_t)(pairs_of + (a.D - 2 * a.pairs) / N) * (a.H + a.K)
-                              : (int64_t)(a.D - a.pairs) * (a.H + a.K);
+    const int per_head = vec ? pairs_of + (a.D - 2 * a.pairs) / N : a.D - a.pairs;
+    const int64_t items = (int64_t)per_head * (a.H + a.K);
     a.tokens = (int)(RO_ITEMS * RO_THREADS / items);
     if (a.tokens > 16) a.tokens = 16;
     if (a.tokens < 1) a.tokens = 1;
     while (a.tokens > 1 && (a.T + a.tokens - 1) / a.tokens < 2 * 148) a.tokens /= 2;
+    // two tokens or more have 512 items at most, and items of a token 2^23
+    a.by_pairs = divide_by(a.pairs);
+    a.by_token = a.tokens > 1 ? divide_by(items) : Div{0u, 0u};
+    a.by_head = divide_by(per_head);
     const int64_t blocks = (a.T + a.tokens - 1) / a.tokens;
     if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_rotary: too many tokens");
     const size_t smem = (size_t)a.tokens * a.pairs * sizeof(float2);

@@ -587,7 +587,7 @@ ZG_API int zg_append_pages(void* k_pages, void* v_pages, int64_t n_pages, int pa
  * bf16 pages with D a multiple of 8 are 16-byte aligned (and q 4-byte, ldq
  * even).  At most 2^30 positions in a row of the table and in the pool.  The
  * workspace (16-byte aligned) holds the splits' partial sums; 0 bytes where
- * one split does. */
+ * one split, or a cluster of up to eight, does. */
 ZG_API size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int D, int max_pages, int page, int window,
                                                 int sinks, int dtype);
 ZG_API int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,

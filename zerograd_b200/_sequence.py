@@ -22,6 +22,7 @@ transpose).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -36,17 +37,20 @@ _transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_st
 _modes = getattr(torch._C, "_len_torch_dispatch_stack", None)
 _tracing = getattr(torch._C, "_get_tracing_state", None)
 _ask = _transform is not None and _modes is not None and _tracing is not None
+_compiling, _grad_enabled, _Tensor = torch.compiler.is_compiling, torch.is_grad_enabled, torch.Tensor
+# half the host time of new_empty, which reads a list of sizes
+_empty, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
 
 
 def _plain_call(*ts) -> bool:
     """True when a call needs none of what the dispatcher adds (vmap, an
     autograd error, a tracing mode): the op is then launched without it,
     which a single token's call notices (about 20 us of host time)."""
-    if not _ask or _transform() is not None or _modes() or _tracing() is not None or torch.compiler.is_compiling():
+    if not _ask or _transform() is not None or _modes() or _tracing() is not None or _compiling():
         return False
-    grad = torch.is_grad_enabled()
+    grad = _grad_enabled()
     for t in ts:
-        if type(t) is not torch.Tensor:
+        if type(t) is not _Tensor:
             if t is not None:
                 return False
         elif grad and t.requires_grad:
@@ -142,7 +146,7 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
         k = k.to(dt)
     (q, ldq), (k, ldk) = _pitched(q), _pitched(k)
     positions = positions.contiguous()
-    qo, ko = q.new_empty(qs), k.new_empty(ks)
+    qo, ko = _empty(q, memory_format=_CONTIGUOUS), _empty(k, memory_format=_CONTIGUOUS)
     widths = (ctypes.c_int32 * len(axes))(*axes)
     _call(dev, "zg_rotary", q.data_ptr(), ldq, k.data_ptr(), ldk, positions.data_ptr(), pos_code, math.prod(tokens),
           positions.numel() // len(axes), qs[-2], ks[-2], qs[-1], len(axes), widths, base, interleaved, joint,
@@ -224,7 +228,7 @@ def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     if v.dtype is not dt:
         v = v.to(dt)
     (q, ldq), (k, ldk), (v, ldv) = _pitched(q), _pitched(k), _pitched(v)
-    o = q.new_empty(qs)
+    o = _empty(q, memory_format=_CONTIGUOUS)
     _call(dev, "zg_window_attention", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
           None if lengths is None else lengths.data_ptr(), math.prod(lead), S, H, K, D, window, sinks, code, o.data_ptr())
     return o
@@ -305,7 +309,7 @@ def launch_append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.T
             raise ValueError(f"counts of shape {tuple(counts.shape)} do not match the sequences {tuple(lead)}")
         counts = _int32(counts, "counts")
     (k, ldk), (v, ldv) = _pitched(k), _pitched(v)
-    new = had.new_empty(lead)
+    new = _empty(had)
     _call(dev, "zg_append_pages", k_pages.data_ptr(), v_pages.data_ptr(), N, page, K, D, k.data_ptr(), ldk, v.data_ptr(),
           ldv, math.prod(lead), ks[-3], table.data_ptr(), table.shape[-1], had.data_ptr(),
           None if counts is None else counts.data_ptr(), code, new.data_ptr())
@@ -360,6 +364,11 @@ def append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(*sizes) -> int:
+    return L.query("zg_paged_attention_workspace_size", *sizes)
+
+
 def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                            lengths: torch.Tensor, window: int, sinks: int) -> torch.Tensor:
     """q [..., H, D] over the pages of the sequences [...]; window 0: none."""
@@ -374,13 +383,13 @@ def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     table, had = _table(page_table, lengths, lead)
     B, M = math.prod(lead), table.shape[-1]
     code = L.dtype_code(dt)
-    o = q.new_empty(qs)
+    o = _empty(q, memory_format=_CONTIGUOUS)
     if B == 0:
         return o
     rows, ldq = _pitched(q)
     if rows.data_ptr() % 4 or ldq % 2:
         rows, ldq = rows.clone(memory_format=torch.contiguous_format), H * D
-    nbytes = L.query("zg_paged_attention_workspace_size", B, H, K, D, M, page, window, sinks, code)
+    nbytes = _paged_workspace(B, H, K, D, M, page, window, sinks, code)
     ws = L.workspace(nbytes, dev) if nbytes else None
     _call(dev, "zg_paged_attention", rows.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), N, page,
           table.data_ptr(), M, had.data_ptr(), B, H, K, D, window, sinks, code, o.data_ptr(), L.ptr(ws), nbytes)

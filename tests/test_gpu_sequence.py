@@ -627,3 +627,60 @@ def test_window_attention_rows_formed_again_in_a_long_sequence(cuda):
     # each is off by 2^-8 sum w |v| + 2^-8 |o| at most (float32's part is far below)
     err = (o[0, :at].double() - want[0, :at].double()).abs()
     assert float(err.max()) <= 2 * 2.0 ** -7 * float(v[0, :at].abs().max())
+
+
+# ------------------------------------------------ offsets beyond 32 bits of elements
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Rows more than 2^31 elements into q, o, the pages and the cache's pool."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    g = torch.Generator(device=cuda).manual_seed(8)
+    S, H, D, tail = 140010, 120, 128, 300
+    assert S * H * D > 2 ** 31
+    q = torch.zeros(1, S, H, D, device=cuda, dtype=BF)
+    k, v = (torch.zeros(1, S, 2, D, device=cuda, dtype=BF) for _ in range(2))
+    for t in (q, k, v):
+        t[:, -tail:] = torch.randn(1, tail, t.shape[2], D, generator=g, device=cuda).to(BF)
+    o = zg.window_attention(q, k, v, 64)[:, -tail:]
+    part = [t[:, -tail:] for t in (q, k, v)]
+    want, mag = so.window_attention(*part, 64)
+    tol = so.attention_tolerance(part[0], part[1], want, mag, BF, tail)
+    so.assert_within(o[:, 64:], want[:, 64:].cpu(), tol[:, 64:].cpu())
+    pos = torch.arange(S, device=cuda)[:, None]
+    rq, _ = zg.rotary(q, k, pos, (D,))
+    few, _ = zg.rotary(part[0], part[1], pos[-tail:], (D,))
+    assert torch.equal(rq[:, -tail:], few)
+    del q, k, v, o, rq
+    N, page, K = 33000, 64, 8
+    assert N * page * K * D > 2 ** 31
+    kp, vp = (torch.empty(N, page, K, D, device=cuda, dtype=BF) for _ in range(2))
+    k, v = (torch.randn(2, 150, K, D, generator=g, device=cuda).to(BF) for _ in range(2))
+    table = torch.tensor([[N - 1, 0, N - 2], [5, N - 3, 6]], device=cuda)
+    n = zg.append_pages(kp, vp, k, v, table, torch.zeros(2, dtype=torch.int64, device=cuda))
+    assert n.tolist() == [150, 150] and torch.equal(kp[N - 2, 21], k[0, 149]) and torch.equal(vp[N - 3, 0], v[1, 64])
+    q = torch.randn(2, 16, D, generator=g, device=cuda).to(BF)
+    o = zg.paged_attention(q, kp, vp, table, n)
+    small = torch.tensor([[0, 1, 2], [3, 4, 5]], device=cuda)
+    at = table.flatten()
+    assert torch.equal(o, zg.paged_attention(q, kp[at].contiguous(), vp[at].contiguous(), small, n))
+    _ok()
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 256), (F32, 128)])
+def test_window_attention_fma_offsets_beyond_32_bits(cuda, dtype, D):
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    g = torch.Generator(device=cuda).manual_seed(D)
+    H, tail = 120, 200
+    S = 2 ** 31 // (H * D) + 10
+    q = torch.zeros(1, S, H, D, device=cuda, dtype=dtype)
+    k, v = (torch.zeros(1, S, 1, D, device=cuda, dtype=dtype) for _ in range(2))
+    for t in (q, k, v):
+        t[:, -tail:] = torch.randn(1, tail, t.shape[2], D, generator=g, device=cuda).to(dtype)
+    o = zg.window_attention(q, k, v, 20)[:, -tail:]
+    part = [t[:, -tail:] for t in (q, k, v)]
+    want, mag = so.window_attention(*part, 20)
+    tol = so.attention_tolerance(part[0], part[1], want, mag, dtype, tail)
+    so.assert_within(o[:, 20:], want[:, 20:].cpu(), tol[:, 20:].cpu())

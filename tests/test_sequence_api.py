@@ -110,3 +110,25 @@ def test_plain_calls_skip_the_dispatcher():
     seen = []
     torch.func.vmap(lambda t: seen.append(_sequence._plain_call(x)) or t)(torch.zeros(3))
     assert seen == [False]
+
+
+def test_a_call_is_made_with_its_tensors_device_current(monkeypatch):
+    current, made = [0], []
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            current.append(self.dev.index)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[-1], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(L, "stream_ptr", lambda dev: ("stream of", dev.index))
+    monkeypatch.setattr(L, "call", lambda name, *args: made.append((name, current[-1], args)))
+    _sequence._call(torch.device("cuda", 0), "f", 1)
+    _sequence._call(torch.device("cuda", 3), "g", 2, 3)
+    assert made == [("f", 0, (1, ("stream of", 0))), ("g", 3, (2, 3, ("stream of", 3)))] and current == [0]

@@ -136,7 +136,7 @@ __device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h
 // keys are multiplied that any row sees: 3 x 777 tokens of 8 heads of 80 under
 // a window of 200, 65 -> 52 us.  What bounds it is the FMA pipe and the shared
 // memory reads that feed it, both over half busy: causal, 2048 tokens of 8
-// heads of 128, 274 us, 31 TFLOP/s of the visible pairs.
+// heads of 128, 269 us, 32 TFLOP/s of the visible pairs.
 // ---------------------------------------------------------------------------
 constexpr int WF_M = 32, WF_N = 64, WF_THREADS = 128, WF_PP = WF_N + 4;
 
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
             default: scores(std::integral_constant<int, 1>{});
         }
         __syncwarp();  // a row's weights are written and read by the same half warp
-#pragma unroll 2
+#pragma unroll 4
         for (int j = 16 * g0; j < 16 * g1; j += 4) {
             float4 pv[4];
 #pragma unroll

@@ -629,7 +629,9 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
 }
 
 // Joins the splits of one query head: a block per (b, h), its warps over the
-// splits, summed in warp order.
+// splits, summed in warp order.  It is launched so that its blocks start as
+// the splits' last one ends.  (With its blocks waiting in their places while
+// the splits run, one sequence of 131000 takes 54.3 us instead of 51.6.)
 template <typename T>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     __shared__ float4 sums[8][64];

@@ -105,10 +105,12 @@ struct PagedArgs {
     const void *q, *kp, *vp;
     const int32_t *table, *lengths;
     void* o;
-    float* part;  // splits > 1 without a cluster: per unit and split, m [R], l [R], then R rows of sums
+    float* part;  // share > 0: of each block m [R], l [R], then R rows of sums
     int64_t ldq, n_pages;
-    int page, max_pages, H, K, D, G, row_tiles, R;  // R: query rows of a unit (heads that share a key head)
-    int window, sinks, chunk, splits, cluster;  // cluster: a unit's splits are a cluster, which joins them
+    int page, max_pages, B, H, K, D, G, row_tiles, R;  // R: query rows of a unit (heads that share a key head)
+    // splits > 1: a unit's splits are a cluster, which joins them; share > 0:
+    // so many blocks have equal shares of all units, joined by a kernel
+    int window, sinks, splits, share;
     float scale;  // log2(e) / sqrt(D)
 };
 
@@ -128,6 +130,114 @@ __device__ __forceinline__ Seen seen_by(const PagedArgs& a, int b) {
     const int w = a.window > 0 && a.window < n ? a.window : n;
     const int s = a.sinks < n - w ? a.sinks : n - w;
     return Seen{w + s, s, n - w - s};
+}
+
+constexpr int PG_MIN_CHUNK = 128;  // positions of a share: less would be the pipeline's filling and the join
+
+// The blocks' equal shares, from the sequences' lengths (at most 64 of them):
+// lane l has those of sequences 2 l and 2 l + 1.
+struct Shares {
+    int chunk, splits[2], before;  // positions of a share, shares of one unit, blocks of the sequences before 2 l
+};
+__device__ __forceinline__ Shares shares_of(const PagedArgs& a) {
+    const int lane = threadIdx.x % 32, heads = a.K * a.row_tiles;
+    if (a.B == 1) {
+        const int v = lane == 0 ? seen_by(a, 0).vis : 0, each = a.share / heads;
+        const int even = ((v < 0 ? 0 : v) + each - 1) / each;
+        const int chunk = __shfl_sync(0xffffffffu, ((even < PG_MIN_CHUNK ? PG_MIN_CHUNK : even) + 63) / 64 * 64, 0);
+        return Shares{chunk, {v > 0 ? (v + chunk - 1) / chunk : 0, 0}, 0};
+    }
+    int vis[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        vis[j] = 2 * lane + j < a.B ? seen_by(a, 2 * lane + j).vis : 0;
+        if (vis[j] < 0) vis[j] = 0;
+    }
+    long long total = (long long)vis[0] + vis[1];
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    // the shortest shares that there are blocks for: from those that would all
+    // be full, a quarter of the way at a time, to those that are enough even if
+    // each unit ends in a share of its own
+    auto part = [&](int blocks) {
+        const int even = (int)ceil((double)(total * heads) / blocks);  // exact below 2^53
+        return ((even < PG_MIN_CHUNK ? PG_MIN_CHUNK : even) + 63) / 64 * 64;
+    };
+    const int least = part(a.share), most = part(a.share - a.B * heads);
+    Shares h;
+    h.chunk = most;
+#pragma unroll 1
+    for (int k = 0; k < 4 && least < most; ++k) {
+        const int c = least + (most - least) / 64 * k / 4 * 64;
+        int used = heads * ((vis[0] + c - 1) / c + (vis[1] + c - 1) / c);
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) used += __shfl_xor_sync(0xffffffffu, used, x);
+        if (used <= a.share) {
+            h.chunk = c;
+            break;
+        }
+    }
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        h.splits[j] = (vis[j] + h.chunk - 1) / h.chunk;
+        n += heads * h.splits[j];
+    }
+    h.before = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, h.before, x);
+        if ((int)threadIdx.x % 32 >= x) h.before += below;
+    }
+    h.before -= n;
+    return h;
+}
+
+// What this block does: positions c0 .. c0 + chunk - 1 of what row tile rt of
+// key head kh of sequence b sees.  on: it has any share.
+struct Work {
+    int b, kh, rt, split, c0, chunk;
+    bool on;
+};
+__device__ __forceinline__ Work work_of(const PagedArgs& a) {
+    Work w;
+    int unit;
+    w.on = true;
+    if (a.share) {
+        const int lane = threadIdx.x % 32, x = (int)blockIdx.x, heads = a.K * a.row_tiles;
+        const Shares h = shares_of(a);
+        const int mine = heads * (h.splits[0] + h.splits[1]);
+        const unsigned at = __ballot_sync(0xffffffffu, x >= h.before && x < h.before + mine);
+        w.on = at != 0;
+        const int from = w.on ? __ffs(at) - 1 : 0;
+        int left = x - __shfl_sync(0xffffffffu, h.before, from);
+        int splits = __shfl_sync(0xffffffffu, h.splits[0], from);
+        const int second = __shfl_sync(0xffffffffu, h.splits[1], from);
+        w.b = 2 * from;
+        if (left >= heads * splits) {
+            left -= heads * splits;
+            splits = second;
+            ++w.b;
+        }
+        unit = w.on ? left / splits : 0;
+        w.split = w.on ? left - unit * splits : 0;
+        w.chunk = h.chunk;
+    } else {
+        unit = (int)blockIdx.x / a.splits;
+        w.split = (int)blockIdx.x - unit * a.splits;
+        const int heads = a.K * a.row_tiles;
+        w.b = unit / heads;
+        unit -= w.b * heads;
+        w.chunk = 1 << 30;
+        if (a.splits > 1) {
+            const int vis = seen_by(a, w.b).vis;
+            w.chunk = (((vis < 0 ? 0 : vis) + a.splits - 1) / a.splits + 63) / 64 * 64;
+        }
+    }
+    w.kh = unit / a.row_tiles;
+    w.rt = unit - w.kh * a.row_tiles;
+    w.c0 = w.split * w.chunk;
+    return w;
 }
 
 // A position's entry of the page table, read one tile before it is used: the
@@ -189,8 +299,8 @@ constexpr int PG_CLUSTER = 8;  // splits that are joined in a cluster, at most
 // ms, ls [PG_WARPS][R] (the joined ones in the first R); os [PG_WARPS][R][pitch].
 template <typename T>
 __device__ __forceinline__ void join_warps(const PagedArgs& a, float* ms, float* ls, float* os, int pitch, int rows,
-                                           int b, int h0, int64_t unit, int split, bool bad, bool none) {
-    float* part = a.splits > 1 && !a.cluster ? a.part + (unit * a.splits + split) * part_floats(a.R, a.D) : nullptr;
+                                           int b, int h0, int split, bool bad, bool none) {
+    float* part = a.share ? a.part + blockIdx.x * part_floats(a.R, a.D) : nullptr;
     T* out = static_cast<T*>(a.o) + ((int64_t)b * a.H + h0) * a.D;
     for (int i = threadIdx.x; i < rows * a.D; i += PG_WARPS * 32) {
         const int r = i / a.D, d = i - r * a.D;
@@ -206,7 +316,7 @@ __device__ __forceinline__ void join_warps(const PagedArgs& a, float* ms, float*
             x = fmaf(os[(w * a.R + r) * pitch + d], f, x);
         }
         if (bad) l = __int_as_float(0x7fffffff);
-        if (a.cluster) {
+        if (a.splits > 1) {
             os[r * pitch + d] = x;  // read by this thread alone
         } else if (part) {
             if (d == 0) {
@@ -218,7 +328,7 @@ __device__ __forceinline__ void join_warps(const PagedArgs& a, float* ms, float*
             out[i] = zg_from_float<T>(none ? 0.f : x / l);
         }
     }
-    if (!a.cluster) return;
+    if (a.splits == 1) return;
     // the row's maximum and sum over the warps, by one warp's lanes (R <= 16)
     __syncthreads();
     if (threadIdx.x < a.R) {
@@ -296,16 +406,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float ms[PG_WARPS * 16], ls[PG_WARPS * 16];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t unit = blockIdx.x / a.splits;
-    const int split = (int)(blockIdx.x % a.splits);
-    const int rt = (int)(unit % a.row_tiles), kh = (int)(unit / a.row_tiles % a.K);
-    const int b = (int)(unit / a.row_tiles / a.K);
+    const Work w = work_of(a);
+    if (!w.on) return;
+    const int b = w.b, kh = w.kh, rt = w.rt, c0 = w.c0;
     const int rows = a.G - rt * 16 < 16 ? a.G - rt * 16 : 16;
     const int h0 = kh * a.G + rt * 16;
     const Seen see = seen_by(a, b);
-    const int c0 = split * a.chunk;
-    const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;  // this split: [c0, end)
-    if (c0 >= see.vis && a.splits > 1 && !a.cluster) return;  // nothing here; the join knows by the length
+    const int end = see.vis - c0 < w.chunk ? see.vis : c0 + w.chunk;  // this block: [c0, end)
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + 15) / 16 : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -454,7 +561,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
         *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(o[d][2], o[d][3]);
     }
     __syncthreads();
-    join_warps<T>(a, ms, ls, os, DP, rows, b, h0, unit, split, bad, see.vis == 0);
+    join_warps<T>(a, ms, ls, os, DP, rows, b, h0, w.split, bad, see.vis == 0);
 }
 
 // Any type, width and alignment, in float32 on the FMA pipe.  A warp's tile
@@ -472,16 +579,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
     __shared__ float ms[PG_WARPS * GT], ls[PG_WARPS * GT];
     __shared__ __align__(16) float qs[GT][36 * PARTS];  // parts of 32 columns, 4 banks apart
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t unit = blockIdx.x / a.splits;
-    const int split = (int)(blockIdx.x % a.splits);
-    const int rt = (int)(unit % a.row_tiles), kh = (int)(unit / a.row_tiles % a.K);
-    const int b = (int)(unit / a.row_tiles / a.K);
+    const Work w = work_of(a);
+    if (!w.on) return;
+    const int b = w.b, kh = w.kh, rt = w.rt, c0 = w.c0;
     const int rows = a.G - rt * GT < GT ? a.G - rt * GT : GT;
     const int h0 = kh * a.G + rt * GT;
     const Seen see = seen_by(a, b);
-    const int c0 = split * a.chunk;
-    const int end = see.vis - c0 < a.chunk ? see.vis : c0 + a.chunk;
-    if (c0 >= see.vis && a.splits > 1 && !a.cluster) return;
+    const int end = see.vis - c0 < w.chunk ? see.vis : c0 + w.chunk;
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + TT - 1) / TT : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -625,7 +729,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
         for (int c = 0; c < NI; ++c) os[(warp * GT + g) * DMAX + lane + 32 * c] = o[g][c];
     }
     __syncthreads();
-    join_warps<T>(a, ms, ls, os, DMAX, rows, b, h0, unit, split, bad, see.vis == 0);
+    join_warps<T>(a, ms, ls, os, DMAX, rows, b, h0, w.split, bad, see.vis == 0);
 }
 
 // Joins the splits of one query head: a block per (b, h), its warps over the
@@ -639,12 +743,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
     const int kh = h / a.G, rt = h % a.G / a.R, r = h % a.G % a.R;
-    const int64_t unit = ((int64_t)b * a.K + kh) * a.row_tiles + rt;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched before the splits' kernel has ended
     const int vis = seen_by(a, b).vis;
-    const int n = vis > 0 ? (vis + a.chunk - 1) / a.chunk : 0;
+    const Shares shares = shares_of(a);
+    const int even = __shfl_sync(0xffffffffu, shares.splits[0], b / 2), odd = __shfl_sync(0xffffffffu, shares.splits[1], b / 2);
+    const int n = b % 2 ? odd : even;  // shares of this unit, from block `first`
+    const int first = __shfl_sync(0xffffffffu, shares.before, b / 2) + (b % 2 ? a.K * a.row_tiles * even : 0) +
+                      (kh * a.row_tiles + rt) * n;
     const int64_t pf = part_floats(a.R, a.D);
-    const float* part = a.part + unit * a.splits * pf;
+    const float* part = a.part + first * pf;
     const int words = pad4(a.D) / 4;
     float M = -INFINITY;
     for (int s = lane; s < n; s += 32) M = fmaxf(M, part[s * pf + r]);
@@ -688,12 +795,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     static_cast<T*>(a.o)[((int64_t)b * a.H + h) * a.D + d] = zg_from_float<T>(out);
 }
 
-constexpr int PG_MIN_CHUNK = 128;
-
-// How a call is cut: R query rows of a unit, and the units' splits.
+// How a call is cut: R query rows of a unit, the units' splits, or the blocks
+// that share them.
 struct PagedPlan {
-    int R, row_tiles, chunk, splits;
-    bool mma, cluster;
+    int R, row_tiles, splits, share;
+    bool mma;
 };
 
 PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window, int sinks, int dtype) {
@@ -704,38 +810,28 @@ PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window
     p.row_tiles = (G + p.R - 1) / p.R;
     int64_t vis = longest;
     if (window > 0 && (int64_t)window + sinks < vis) vis = (int64_t)window + sinks;
-    if (vis < 1) vis = 1;
-    const int64_t units = B * K * p.row_tiles;
+    const int64_t units = B * K * p.row_tiles, blocks = (p.mma ? 2 : 3) * 148;
     // Two blocks run on each of 148 SMs (three of the FMA path): as many splits
     // as fill them once.  (Four times as many, so that a batch of 64 sequences
     // of different lengths evens out, was 126 us instead of 81: a block costs
     // its pipeline's filling and its part in the join.)  Up to PG_CLUSTER
-    // splits are a cluster, which joins them by itself.  Of more than that,
-    // where a kernel of its own joins them, a batch takes half as many again:
-    // 8 sequences of up to 30000 tokens 29.5 -> 27.1 us; one sequence, whose
-    // pieces are all of one length, does not (53 -> 72 us).
-    const int per_sm = p.mma ? 2 : 3;
-    int64_t splits = (per_sm * 148 + units - 1) / units;
-    if (splits > PG_CLUSTER && B > 1) splits = ((per_sm + 1) * 148 + units - 1) / units;
-    if (splits > 128) splits = 128;
-    int64_t chunk = (vis + splits - 1) / splits;
-    if (chunk < PG_MIN_CHUNK) chunk = PG_MIN_CHUNK;  // less would be the pipeline's filling and the join
-    chunk = (chunk + 63) / 64 * 64;
-    p.chunk = (int)(chunk > INT32_MAX ? INT32_MAX / 64 * 64 : chunk);
-    p.splits = (int)((vis + p.chunk - 1) / p.chunk);
-    p.cluster = p.splits > 1 && p.splits <= PG_CLUSTER;
-    if (p.cluster) {
-        // two, four or eight blocks, of equal shares
-        const int size = p.splits <= 2 ? 2 : p.splits <= 4 ? 4 : 8;
-        p.chunk = (int)(((vis + size - 1) / size + 63) / 64 * 64);
-        p.splits = size;
-    }
+    // splits are a cluster of two, four or eight blocks, which joins them by
+    // itself and whose blocks have equal parts of what its unit sees.  Units
+    // that would be cut further are shared out to all blocks by the lengths
+    // that the device knows, and a kernel of its own joins them.  (Split by the
+    // table's width instead, a sequence of 8000 in a table of 131072 took 42
+    // us, now 12.2; 8 of 1000 in a table of 16384 26 us, now 11.2.)
+    int64_t splits = (blocks + units - 1) / units;
+    if (splits > (vis + PG_MIN_CHUNK - 1) / PG_MIN_CHUNK) splits = (vis + PG_MIN_CHUNK - 1) / PG_MIN_CHUNK;
+    p.splits = 1;
+    if (splits > PG_CLUSTER)
+        p.share = (int)blocks;  // more than twice the units, of which there are less than 64
+    else if (splits > 1)
+        p.splits = splits <= 2 ? 2 : splits <= 4 ? 4 : 8;
     return p;
 }
 
-size_t paged_workspace(const PagedPlan& p, int64_t B, int K, int D) {
-    return p.splits > 1 && !p.cluster ? (size_t)(B * K * p.row_tiles * p.splits * part_floats(p.R, D)) * sizeof(float) : 0;
-}
+size_t paged_workspace(const PagedPlan& p, int D) { return (size_t)(p.share * part_floats(p.R, D)) * sizeof(float); }
 
 bool paged_sizes_ok(int64_t n_pages, int page, int64_t B, int H, int K, int D, int max_pages) {
     return n_pages >= 0 && page >= 1 && B >= 0 && H >= 1 && K >= 1 && D >= 1 && max_pages >= 0 && H % K == 0 &&
@@ -761,7 +857,7 @@ int launch_split(void (*f)(P...), const PagedArgs& a, int64_t blocks, size_t sme
     at.val.clusterDim.x = (unsigned)a.splits;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     c.attrs = &at;
-    c.numAttrs = a.cluster ? 1 : 0;
+    c.numAttrs = a.splits > 1 ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&c, f, args...);
     if (e != cudaSuccess) return zg::fail(ZG_ERR_CUDA, "zg_paged_attention: %s", cudaGetErrorString(e));
     return zg::check_launch("zg_paged_attention");
@@ -842,7 +938,7 @@ extern "C" size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int
     if (!paged_sizes_ok(0, page, B, H, K, D, max_pages) || B == 0 || D > 256 || window < 0 || sinks < 0 ||
         !zg::dtype_ok(dtype))
         return 0;
-    return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), B, K, D);
+    return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), D);
 }
 
 extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
@@ -861,15 +957,15 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
     if (!q || !lengths || !o || (max_pages && !table) || (n_pages && (!k_pages || !v_pages)))
         return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: null pointer");
     PagedPlan p = paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype);
-    const size_t need = paged_workspace(p, B, K, D);
+    const size_t need = paged_workspace(p, D);
     if (need && (!workspace || workspace_bytes < need))
         return zg::fail(ZG_ERR_WORKSPACE, "zg_paged_attention: workspace of %zu bytes needed", need);
-    const int64_t blocks = B * K * p.row_tiles * p.splits;
+    const int64_t blocks = p.share ? p.share : B * K * p.row_tiles * p.splits;
     if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: too many rows");
     const int n = 16 / (int)zg::dtype_size(dtype);
     const int vec = D % n == 0 && aligned16(k_pages) && aligned16(v_pages);
     PagedArgs a{q, k_pages, v_pages, table, lengths, o, static_cast<float*>(workspace), ldq, n_pages, page, max_pages,
-                H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.chunk, p.splits, p.cluster,
+                (int)B, H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.splits, p.share,
                 (float)(1.4426950408889634 / sqrt((double)D))};
     cudaStream_t st = zg::as_stream(stream);
     int rc;
@@ -883,7 +979,7 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
         rc = dtype == ZG_BF16 ? launch_fma_any<__nv_bfloat16>(a, vec, blocks, st)
                               : launch_fma_any<float>(a, vec, blocks, st);
     }
-    if (rc != ZG_OK || p.splits == 1 || p.cluster) return rc;
+    if (rc != ZG_OK || !p.share) return rc;
     zg::LaunchTimer zg_lt_("paged_join", st);
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((unsigned)(B * H));

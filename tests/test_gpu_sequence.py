@@ -684,3 +684,25 @@ def test_window_attention_fma_offsets_beyond_32_bits(cuda, dtype, D):
     want, mag = so.window_attention(*part, 20)
     tol = so.attention_tolerance(part[0], part[1], want, mag, dtype, tail)
     so.assert_within(o[:, 20:], want[:, 20:].cpu(), tol[:, 20:].cpu())
+
+
+@pytest.mark.parametrize("dtype,lengths", [
+    (BF, [5000, 0, -1, 130]), (F32, [1, 3000, 60001, 60000]), (BF, [7000]), (BF, [0, 0]), (F32, [-3]),
+    (BF, [12000, 11, 4097, 1, 128, 129, 8191]),
+])
+def test_paged_attention_in_wide_tables(cuda, dtype, lengths):
+    """Tables wider than the sequences: the work is shared out by the lengths."""
+    H, K, D, page, M = 4, 2, 64, 16, 3750
+    g = torch.Generator().manual_seed(len(lengths))
+    fits = [n if 0 <= n <= M * page else 0 for n in lengths]
+    kp, vp, table = _pool(fits, page, K, D, dtype, g)
+    wide = torch.full((len(lengths), M), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    q = _rand((len(lengths), H, D), dtype, g)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    want, mag = so.paged_attention(q, kp, vp, table, torch.tensor(fits, dtype=torch.int32))
+    o = zg.paged_attention(*(t.to(cuda) for t in (q, kp, vp, wide, n)))
+    good = torch.tensor([a == b for a, b in zip(lengths, fits)])
+    assert torch.isnan(o[~good.to(cuda)]).all()
+    tol = so.attention_tolerance(q, kp, want, mag, dtype, max(max(fits), 1))
+    so.assert_within(o[good.to(cuda)], want[good], tol[good])

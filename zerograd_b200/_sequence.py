@@ -143,7 +143,10 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
     dt = q.dtype
     code = L.dtype_code(dt)
     if k.dtype is not dt:
-        k = k.to(dt)
+        # a launch has one type: each by itself, the other without heads
+        L.dtype_code(k.dtype)
+        rest = (positions, axes, base, interleaved, joint, inverse)
+        return launch_rotary(q, q[..., :0, :], *rest)[0], launch_rotary(k[..., :0, :], k, *rest)[1]
     (q, ldq), (k, ldk) = _pitched(q), _pitched(k)
     positions = positions.contiguous()
     qo, ko = _empty(q, memory_format=_CONTIGUOUS), _empty(k, memory_format=_CONTIGUOUS)
@@ -179,7 +182,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes, base
            interleaved: bool = False, joint: bool = False,
            inverse: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """Queries [..., S, H, D] and keys [..., S, K, D] with rotary positions,
-    in one launch; both are returned, in their own type.
+    in one launch (two where their types differ); both are returned, each in
+    its own type.
 
     ``axes`` gives the rotated columns of each axis, all even: ``(64,)`` for
     text, ``(16, 24, 24)`` for time, height and width.  Their sum may be less

@@ -32,3 +32,23 @@ def test_rotary_of_two_types_keeps_both(calls):
         assert [(c[8], c[9], c[-3]) for _, c in calls] == [(4, 0, L.dtype_code(a)), (0, 2, L.dtype_code(b))]
     with pytest.raises(TypeError):
         _sequence.rotary(torch.zeros(2, 5, 4, 64, dtype=a), torch.zeros(2, 5, 2, 64, dtype=torch.half), pos, (64,))
+
+
+def test_sizes_beyond_32_bits_are_refused(calls):
+    """An axis, a page size, a table or heads of 2^32 and a few are not taken for the few."""
+    wide = 2 ** 32
+    q, k, pos = _meta(2, 5, 4, 64), _meta(2, 5, 2, 64), torch.zeros(5, 1, dtype=torch.int32)
+    table, n = _meta(2, 3, dtype=torch.int32), _meta(2, dtype=torch.int32)
+    pool = _meta(4, 8, 2, 64)
+    for call in (lambda: _sequence.rotary(q, k, pos, (wide + 64,)),
+                 lambda: _sequence.rotary(q, k, pos, (64 - wide,)),
+                 lambda: _sequence.rotary(_meta(1, 1, wide + 4, 64), k[:1, :1], pos[:1], (64,)),
+                 lambda: _sequence.window_attention(_meta(1, 1, wide + 4, 64), k[:1, :1], k[:1, :1]),
+                 lambda: _sequence.window_attention(*[_meta(1, 1, 1, wide + 64)] * 3),
+                 lambda: _sequence.append_pages(*[_meta(1, wide + 8, 2, 64)] * 2, k, k, table, n),
+                 lambda: _sequence.append_pages(pool, pool, k, k, _meta(2, wide + 1, dtype=torch.int32), n),
+                 lambda: _sequence.paged_attention(q[:, 0], *[_meta(1, wide + 8, 2, 64)] * 2, table, n),
+                 lambda: _sequence.paged_attention(_meta(2, wide + 4, 64), pool, pool, table, n)):
+        with pytest.raises(ValueError):
+            call()
+    assert not calls

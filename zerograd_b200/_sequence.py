@@ -78,6 +78,13 @@ def _call(dev: torch.device, name: str, *args) -> None:
             L.call(name, *args, L.stream_ptr(dev))
 
 
+def _narrow(*sizes: int) -> None:
+    """Refuses sizes that the entry points would get without their upper bits
+    (ctypes cuts an int to its 32 bits)."""
+    if max(sizes) > _INT_MAX:
+        raise ValueError(f"a size of {max(sizes)}: heads, head width, page size and table width are at most 2^31 - 1")
+
+
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
     """Whole numbers as contiguous int32; wider ones that int32 cannot hold
     become -1 or the largest, which the kernels refuse as they would the
@@ -147,6 +154,7 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
         L.dtype_code(k.dtype)
         rest = (positions, axes, base, interleaved, joint, inverse)
         return launch_rotary(q, q[..., :0, :], *rest)[0], launch_rotary(k[..., :0, :], k, *rest)[1]
+    _narrow(qs[-2], ks[-2], qs[-1])
     (q, ldq), (k, ldk) = _pitched(q), _pitched(k)
     positions = positions.contiguous()
     qo, ko = _empty(q, memory_format=_CONTIGUOUS), _empty(k, memory_format=_CONTIGUOUS)
@@ -201,6 +209,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes, base
     axes = [int(a) for a in axes]
     if not axes:
         raise ValueError("axes must name the columns of one axis at least")
+    if min(axes) < 1 or max(axes) > _INT_MAX:
+        raise ValueError(f"axes must be even, positive and at most D in all, got {axes}")
     args = (q, k, positions, axes, float(base), bool(interleaved), bool(joint), bool(inverse))
     return launch_rotary(*args) if _plain_call(q, k, positions) else _rotary_op(*args)
 
@@ -223,6 +233,7 @@ def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     K = ks[-2]
     if K < 1 or H % K:
         raise ValueError(f"{H} query heads are not a multiple of {K} key heads")
+    _narrow(H, D)
     if lengths is not None:
         if lengths.shape != lead:
             raise ValueError(f"lengths of shape {tuple(lengths.shape)} do not match the sequences {tuple(lead)}")
@@ -283,6 +294,7 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> torch.Size:
         raise ValueError("key and value pages must be contiguous")
     if shape[1] < 1 or shape[2] < 1 or shape[3] < 1:
         raise ValueError(f"pages of shape {tuple(shape)} hold nothing")
+    _narrow(*shape[1:])
     return shape
 
 
@@ -290,6 +302,7 @@ def _table(page_table: torch.Tensor, lengths: torch.Tensor, lead: torch.Size) ->
     if page_table.ndim < 1 or page_table.shape[:-1] != lead or lengths.shape != lead:
         raise ValueError(f"a page table of shape {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} do not "
                          f"match the sequences {tuple(lead)}")
+    _narrow(page_table.shape[-1])
     return _int32(page_table, "the page table"), _int32(lengths, "lengths")
 
 
@@ -345,7 +358,7 @@ def append_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, k: torch.Tensor, 
 
     ``k_pages`` and ``v_pages`` [pages, page size, K, D] are contiguous, of
     any page size.  ``page_table`` [..., M] (int32 or int64) names the pages
-    of each sequence in order; entries behind a sequence's last page are not
+    of each sequence in order, M times the page size at most 2^30 positions; entries behind a sequence's last page are not
     read and may hold anything.  ``k`` and ``v`` [..., S, K, D] are the new
     tokens, in the pages' type (views of a fused projection are fine); token
     s goes to position ``lengths`` + s.  ``counts`` [...]: how many of the S
@@ -384,6 +397,7 @@ def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if q.dtype is not dt:
         raise TypeError(f"q must have the pages' type {dt}, got {q.dtype}")
     lead, H = qs[:-2], qs[-2]
+    _narrow(H)
     table, had = _table(page_table, lengths, lead)
     B, M = math.prod(lead), table.shape[-1]
     code = L.dtype_code(dt)

@@ -30,3 +30,36 @@ def test_rotary_of_two_types(cuda, types):
     assert torch.equal(b, zg.rotary(q.to(types[1]), k, pos, (64,))[1])
     va, vb = torch.func.vmap(lambda x, y: zg.rotary(x, y, pos, (64,)))(q, k)
     assert torch.equal(va, a) and torch.equal(vb, b)
+
+
+def test_negated_views(cuda):
+    """Views with the negative bit, called one by one and under vmap, count with their sign."""
+    g = [_rand((2, 9, 2, 64), F32, s, cuda) for s in range(3)]
+    pos = torch.arange(9, device=cuda)[:, None]
+    table, n = torch.tensor([[2, 0], [1, 3]], device=cuda), torch.tensor([9, 4], device=cuda)
+    pool = [_rand((4, 8, 2, 64), F32, s, cuda) for s in (4, 5)]
+
+    def fresh():
+        return [t.clone() for t in pool]
+
+    def run(q, k, v, kp, vp, wk, wv):
+        return (*zg.rotary(q, k, pos, (64,)), zg.window_attention(q, k, v), zg.paged_attention(q[:, 0], kp, vp, table, n),
+                zg.append_pages(wk, wv, k, v, table, torch.zeros_like(n)))
+
+    neg = torch._neg_view
+    w1, w2 = fresh(), fresh()
+    want = run(*(-t for t in g), *(-t for t in pool), *w1)
+    for a, b in zip(run(*map(neg, g), *map(neg, pool), *w2), want):
+        assert torch.equal(a, b)
+    assert all(torch.equal(a, b) for a, b in zip(w1, w2))
+    both = torch.func.vmap(lambda q, k, v: (*zg.rotary(q, k, pos, (64,)), zg.window_attention(q, k, v)))
+    for a, b in zip(both(*map(neg, g)), want):
+        assert torch.equal(a, b)
+    one = torch.func.vmap(lambda q, t, m: zg.paged_attention(q, neg(pool[0]), neg(pool[1]), t, m))
+    assert torch.equal(one(neg(g[0][:, 0]), table, n), want[3])
+    w3 = fresh()
+    put = torch.func.vmap(lambda k, v, t, m: zg.append_pages(*w3, k, v, t, m))
+    put(neg(g[1]), neg(g[2]), table, torch.zeros_like(n))
+    assert all(torch.equal(a, b) for a, b in zip(w1, w3))
+    with pytest.raises(ValueError):
+        torch.func.vmap(lambda k, t, m: zg.append_pages(neg(pool[0]), neg(pool[1]), k, k, t, m))(g[1], table, n)

@@ -44,8 +44,9 @@ _empty, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
 
 def _plain_call(*ts) -> bool:
     """True when a call needs none of what the dispatcher adds (vmap, an
-    autograd error, a tracing mode): the op is then launched without it,
-    which a single token's call notices (about 20 us of host time)."""
+    autograd error, a tracing mode, the values of a negated view or of a zero
+    tensor without memory): the op is then launched without it, which a single
+    token's call notices (about 20 us of host time)."""
     if not _ask or _transform() is not None or _modes() or _tracing() is not None or _compiling():
         return False
     grad = _grad_enabled()
@@ -53,9 +54,19 @@ def _plain_call(*ts) -> bool:
         if type(t) is not _Tensor:
             if t is not None:
                 return False
-        elif grad and t.requires_grad:
+        elif (grad and t.requires_grad) or t.is_neg() or t._is_zerotensor():
             return False
     return True
+
+
+def _mapped(t: torch.Tensor | None, dim: int | None, P: int | None = None) -> torch.Tensor | None:
+    """An argument of a vmap rule with its candidate axis first (with P:
+    expanded to P where it has none), its values in its memory: the rules are
+    reached before the dispatcher resolves a negated view or a zero tensor."""
+    if t is None:
+        return None
+    t = _movedim0(t.clone() if t._is_zerotensor() else t.resolve_neg(), dim)
+    return t if dim is not None or P is None else t.expand(P, *t.shape)
 
 
 def _device(*ts) -> torch.device:
@@ -174,10 +185,8 @@ def _rotary_op(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axes: 
 @torch.library.register_vmap(f"{_NS}::rotary")
 def _rotary_vmap(info, in_dims, q, k, positions, axes, base, interleaved, joint, inverse):
     qd, kd, pd = in_dims[:3]
-    q, k, positions = _movedim0(q, qd), _movedim0(k, kd), _movedim0(positions, pd)
     P = info.batch_size
-    q = q if qd is not None else q.expand(P, *q.shape)
-    k = k if kd is not None else k.expand(P, *k.shape)
+    q, k, positions = _mapped(q, qd, P), _mapped(k, kd, P), _mapped(positions, pd)
     if pd is not None and positions.ndim < q.ndim - 1:
         # per candidate, shared by the axes between the candidates and the sequence
         lead = q.shape[1:q.ndim - positions.ndim]
@@ -257,8 +266,7 @@ def _window_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch
 
 @torch.library.register_vmap(f"{_NS}::window_attention")
 def _window_vmap(info, in_dims, q, k, v, lengths, window, sinks):
-    ts = [_movedim0(t, d) if t is not None else None for t, d in zip((q, k, v, lengths), in_dims)]
-    ts = [t if t is None or d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, in_dims)]
+    ts = [_mapped(t, d, info.batch_size) for t, d in zip((q, k, v, lengths), in_dims)]
     return launch_window_attention(*ts, window, sinks), 0
 
 
@@ -345,8 +353,9 @@ def _append_vmap(info, in_dims, k_pages, v_pages, k, v, page_table, lengths, cou
         raise NotImplementedError("pages batched over candidates are not supported: one pool holds every candidate's")
     if in_dims[4] is None:
         raise NotImplementedError("a page table shared by the candidates would let them write the same pages")
-    ts = [_movedim0(t, d) if t is not None else None for t, d in zip((k, v, page_table, lengths, counts), in_dims[2:])]
-    ts = [t if t is None or d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, in_dims[2:])]
+    if k_pages.is_neg() or v_pages.is_neg() or k_pages._is_zerotensor() or v_pages._is_zerotensor():
+        raise ValueError("pages to be written must be tensors in memory, not negated views or zero tensors")
+    ts = [_mapped(t, d, info.batch_size) for t, d in zip((k, v, page_table, lengths, counts), in_dims[2:])]
     return launch_append_pages(k_pages, v_pages, *ts), 0
 
 
@@ -424,10 +433,10 @@ def _paged_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 def _paged_vmap(info, in_dims, q, k_pages, v_pages, page_table, lengths, window, sinks):
     if in_dims[1] is not None or in_dims[2] is not None:
         raise NotImplementedError("pages batched over candidates are not supported: one pool holds every candidate's")
-    dims = (in_dims[0], in_dims[3], in_dims[4])
-    ts = [_movedim0(t, d) for t, d in zip((q, page_table, lengths), dims)]
-    ts = [t if d is not None else t.expand(info.batch_size, *t.shape) for t, d in zip(ts, dims)]
-    return launch_paged_attention(ts[0], k_pages, v_pages, ts[1], ts[2], window, sinks), 0
+    q, page_table, lengths = (_mapped(t, d, info.batch_size) for t, d in
+                              zip((q, page_table, lengths), (in_dims[0], in_dims[3], in_dims[4])))
+    return launch_paged_attention(q, _mapped(k_pages, None), _mapped(v_pages, None), page_table, lengths, window,
+                                  sinks), 0
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,

@@ -63,3 +63,16 @@ def test_negated_views_and_zero_tensors_take_the_dispatcher():
     m = _sequence._mapped(torch._efficientzerotensor((2,)), None, 4)
     assert m.shape == (4, 2) and not m._is_zerotensor() and m.sum() == 0
     assert _sequence._mapped(None, None, 4) is None
+
+
+def test_paged_attention_copies_queries_for_the_tensor_cores_alone(calls, monkeypatch):
+    """A float32 q of odd pitch, or bf16 with D not a multiple of 8, reaches the entry point as it is."""
+    monkeypatch.setattr(_sequence, "_paged_workspace", lambda *sizes: 0)
+    table, n = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for dtype, D, copied in ((F32, 7, False), (F32, 8, False), (BF, 7, False), (BF, 8, True)):
+        pool = torch.zeros(1, 4, 1, D, dtype=dtype)
+        q = torch.zeros(2, D + 1, dtype=dtype)[:, :D].unflatten(-1, (1, D)) if D % 2 == 0 else torch.zeros(2, 1, D, dtype=dtype)
+        calls.clear()
+        _sequence.paged_attention(q, pool, pool, table, n)
+        (_, args), = calls
+        assert (args[0] != q.data_ptr()) == copied and args[1] == (D if copied else q.stride(0)), (dtype, D)

@@ -414,7 +414,7 @@ def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if B == 0:
         return o
     rows, ldq = _pitched(q)
-    if rows.data_ptr() % 4 or ldq % 2:
+    if code == L.ZG_BF16 and D % 8 == 0 and (rows.data_ptr() % 4 or ldq % 2):  # the tensor cores' path reads pairs
         rows, ldq = rows.clone(memory_format=torch.contiguous_format), H * D
     nbytes = _paged_workspace(B, H, K, D, M, page, window, sinks, code)
     ws = L.workspace(nbytes, dev) if nbytes else None

@@ -12,6 +12,7 @@
 
 #include "zg_ptx.cuh"
 #include "zg_tc.cuh"
+#include "zg_warp.cuh"
 
 namespace {
 
@@ -24,12 +25,6 @@ struct WindowArgs {
     int window, sinks;  // window >= 1 (S where there is none)
     float scale;        // log2(e) / sqrt(D)
 };
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // The larger of two values, NaN if one is.
 __device__ __forceinline__ float max_nan(float x, float y) {
@@ -180,9 +175,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
             for (int e = 0; e < EACH; ++e) {
                 const int x = threadIdx.x + e * WF_THREADS, r = x / WORDS, d = x % WORDS * 4;
                 const bool on = r0 + r < n && d < a.D;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * PITCH + d)),
-                             "l"(on ? src + (r0 + r) * ld + d : src), "r"(on ? 16 : 0)
-                             : "memory");
+                copy16(smem_u32(dst + r * PITCH + d), on ? src + (r0 + r) * ld + d : src, on ? 16 : 0);
             }
         } else if (vec) {
             uint2 u[EACH];
@@ -205,7 +198,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
                 dst[r * PITCH + d] = r0 + r < n && d < a.D ? zg_to_float(src[(r0 + r) * ld + d]) : 0.f;
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copy_commit();
     };
     const std::integral_constant<int, WF_M> q_rows{};
     const std::integral_constant<int, WF_N> k_rows{};
@@ -232,7 +225,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
     for (; kt < kt_end; kt = next(kt)) {
         const int j0 = kt * WF_N;
         load(k_rows, vs, v, a.ldv, j0);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the keys
+        copy_wait<1>();  // the keys
         __syncthreads();
         // the sixteens of this tile's keys that any row sees: [g0, g1)
         int lo = i0 - a.window + 1 - j0, hi = last - j0;
@@ -263,12 +256,12 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
                         s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
                     }
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");  // the values
+            copy_wait<0>();  // the values
             __syncthreads();
             if (next(kt) < kt_end)
                 load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
             else
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                copy_commit();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int qi = i0 + ty + 8 * i;
@@ -420,7 +413,6 @@ constexpr int WT_THREADS = 384;
 template <int DP>
 struct WtShape {
     static constexpr int KEYS = DP == 64 ? 128 : 64;         // keys of a block
-    static constexpr int HALVES = KEYS / 64;
     static constexpr uint32_t QTILE = 128 * DP * 2;          // a query tile: DP / 64 boxes of 128 rows x 64 columns
     static constexpr uint32_t BOX = KEYS * 128;              // KEYS rows x 64 columns
     static constexpr uint32_t BLOCK = KEYS * DP * 2;         // a key or value block: DP / 64 boxes

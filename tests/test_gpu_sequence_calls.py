@@ -63,3 +63,103 @@ def test_negated_views(cuda):
     assert all(torch.equal(a, b) for a, b in zip(w1, w3))
     with pytest.raises(ValueError):
         torch.func.vmap(lambda k, t, m: zg.append_pages(neg(pool[0]), neg(pool[1]), k, k, t, m))(g[1], table, n)
+
+
+# ------------------------------------------ values that are infinite or NaN, or nearly
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 72), (BF, 20), (F32, 64), (F32, 136)])
+@pytest.mark.parametrize("window,sinks,ragged", [(None, 0, False), (40, 3, True), (130, 70, False), (1, 1, True)])
+def test_window_attention_values_not_finite_in_many_places(cuda, dtype, D, window, sinks, ragged):
+    """NaN and infinities in single places, in a whole position and in a whole
+    column reach the rows that see them, and what is masked no row at all."""
+    Z, S, H, K = 3, 420, 4, 2
+    q, k, v = (_rand((Z, S, h, D), dtype, D + h + i, cuda) for i, h in enumerate((H, K, K)))
+    g = torch.Generator().manual_seed(D)
+    for z in range(Z):  # up to 12 places a sequence, more blocks than are listed in the last
+        for _ in range((1, 4, 12)[z]):
+            j, h, d = (int(torch.randint(0, n, (1,), generator=g)) for n in (S, K, D))
+            v[z, j, h, d] = (math.nan, math.inf, -math.inf)[int(torch.randint(0, 3, (1,), generator=g))]
+    v[0, 100, 0] = math.nan
+    v[1, :, 1, 5] = math.inf
+    v[2, 200:, 0, 7] = -math.inf
+    v[2, 20, 1, 9], v[2, 300, 1, 9] = math.inf, -math.inf
+    lengths = torch.tensor([S, 150, 333], device=cuda) if ragged else None
+    o = zg.window_attention(q, k, v, window, sinks, lengths)
+    want, mag = so.window_attention(q, k, v, window, sinks, lengths)
+    assert L.load().zg_device_error(1) == 0
+    assert torch.isnan(want).any() and torch.isinf(want).any()
+    so.assert_within(o, want.cpu(), so.attention_tolerance(q, k, want, mag, dtype, S).cpu())
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (F32, 64)])
+def test_window_attention_weights_of_zero_on_infinite_values(cuda, dtype, D):
+    """A visible score of -inf is a weight of zero, and 0 * inf is NaN."""
+    S = 200
+    q, k, v = (_rand((1, S, 1, D), dtype, s, cuda) for s in range(3))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[0, 30, 0], v[0, 30, 0, :4] = 0, math.inf
+    k[0, 30, 0, 0] = -math.inf
+    v[0, 90, 0, 2:6] = math.inf
+    o = zg.window_attention(q, k, v, 100)
+    want, mag = so.window_attention(q, k, v, 100)
+    assert int(torch.isnan(want).sum()) == 4 * 100 and int(torch.isinf(want).sum()) == 4 * 100 - 2 * 40
+    so.assert_within(o, want.cpu(), so.attention_tolerance(q, torch.nan_to_num(k, 0, 0, 0), want, mag, dtype, S).cpu())
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 20), (F32, 64), (F32, 256)])
+def test_window_attention_of_values_near_the_largest(cuda, dtype, D):
+    """Sums of finite values do not overflow on the way to an average of them."""
+    S = 700
+    q, k = (_rand((1, S, 2, D), dtype, s, cuda) for s in range(2))
+    v = 2.5e38 * (1 + 0.1 * torch.rand(1, S, 2, D, generator=torch.Generator(device=cuda).manual_seed(3), device=cuda))
+    v = v.to(dtype)
+    v[:, :, 1] *= -1
+    for window, sinks in ((None, 0), (90, 5)):
+        o = zg.window_attention(q, k, v, window, sinks)
+        want, mag = so.window_attention(q, k, v, window, sinks)
+        so.assert_within(o, want.cpu(), so.attention_tolerance(q, k, want, mag, dtype, S).cpu())
+
+
+def _time(run, n=5):
+    """Device time of a call in ms: the least of n, after one untimed."""
+    run()
+    times = []
+    for _ in range(n):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        run()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("dtype,H,K,D,window,sinks", [
+    (BF, 12, 4, 64, None, 0), (BF, 8, 4, 128, 1024, 4), (F32, 4, 2, 64, None, 0), (F32, 4, 2, 128, 700, 4)])
+def test_window_attention_time_with_values_not_finite(cuda, dtype, H, K, D, window, sinks):
+    """One infinite value that most rows see, one beside the sinks, a NaN late,
+    a column of one sign, all-NaN values, all-NaN activations, padding of NaN:
+    without a cost where no row that does not see it is touched, and bounded
+    where many are.  (Rows gone over key by key took hundreds of times.)"""
+    S = 4096
+    q, k, v = (_rand((2, S, h, D), dtype, h, cuda) for h in (H, K, K))
+    lengths = torch.tensor([S, S // 2 + 1], device=cuda)
+    plain = _time(lambda: zg.window_attention(q, k, v, window, sinks))
+    padded = _time(lambda: zg.window_attention(q, k, v, window, sinks, lengths))
+    slow = {}
+    for name, at, value in (("first", (0, 0, slice(None), 3), math.inf), ("beside the sinks", (0, 50), math.inf),
+                            ("late", (1, S - 60), math.nan), ("column", (slice(None), slice(None), slice(None), 1), math.inf),
+                            ("all", (), math.nan)):
+        bad = v.clone()
+        bad[at] = value
+        slow[name] = _time(lambda: zg.window_attention(q, k, bad, window, sinks)) / plain
+    nan = [torch.full_like(t, math.nan) for t in (q, k, v)]
+    slow["activations"] = _time(lambda: zg.window_attention(*nan, window, sinks)) / plain
+    for t in (q, k, v):
+        t[1, S // 2 + 1:] = math.nan
+    slow["padding"] = _time(lambda: zg.window_attention(q, k, v, window, sinks, lengths)) / padded
+    print({n: round(x, 2) for n, x in slow.items()}, round(plain * 1e3, 1), "us")
+    assert L.load().zg_device_error(1) == 0
+    assert slow["first"] < 3 and slow["activations"] < 2 and slow["padding"] < 2, slow
+    assert slow["late"] < 12 and slow["beside the sinks"] < 12 and slow["column"] < 50 and slow["all"] < 50, slow

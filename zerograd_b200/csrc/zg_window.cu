@@ -24,6 +24,9 @@ struct WindowArgs {
     int Z, S, H, K, D, G;
     int window, sinks;  // window >= 1 (S where there is none)
     float scale;        // log2(e) / sqrt(D)
+    // 2^lift is above twice the sequence's length: weights are taken so much
+    // smaller, so that no sum of finite values overflows (O / l is the same)
+    int lift;
 };
 
 // The larger of two values, NaN if one is.
@@ -43,74 +46,136 @@ __device__ __forceinline__ int length_of(const WindowArgs& a, int z) {
 // Whether position i sees position j <= i.
 __device__ __forceinline__ bool sees(const WindowArgs& a, int i, int j) { return i - j < a.window || j < a.sinks; }
 
-// One output row by one warp, each visible key on its own in float32: what
-// the tiled kernels fall back to for a row whose weights have a finite sum
-// and whose outputs are not all finite.  A value of a masked place that is
-// infinite or NaN has a weight of zero, and a tile's product turns 0 * inf
-// into NaN; here it is not read.  (A sum that is not finite, or zero, comes
-// of visible scores alone: all of the row is NaN, and stays as it is, so that
-// a candidate whose activations are all NaN costs nothing here.)
-template <typename T>
-__device__ __noinline__ void window_row(const WindowArgs& a, int z, int i, int h) {
-    const int lane = threadIdx.x % 32;
-    const int kh = h / a.G;
-    const T* q = static_cast<const T*>(a.q) + ((int64_t)z * a.S + i) * a.ldq + (int64_t)h * a.D;
+// The blocks of keys that a group of rows visits: those that hold sinks, and
+// the window's, lo .. last.
+struct Blocks {
+    int keys, sinks, lo, last;  // keys of a block, blocks that hold sinks
+    __device__ __forceinline__ bool has(int b) const { return b <= last && (b >= lo || b < sinks); }
+    __device__ __forceinline__ int next(int b) const { return b + 1 < sinks || b + 1 >= lo ? b + 1 : lo; }
+};
+
+constexpr int WIN_BAD = 8;  // blocks that are listed by number
+
+// A value that is infinite or NaN reaches the rows that see it and no others,
+// but a product of tiles multiplies it with the zero weights of the others
+// too.  So where that happened the rows are formed once more with zeros in
+// such places, and the outputs that see them are written behind that: NaN
+// where a column's visible values hold a NaN or infinities of both signs,
+// otherwise the infinity.  On the FMA path that is done here, by one warp, a
+// row a lane (`on`: row i takes part: it lies in the sequence, and its weights'
+// sum is positive and finite; else all of it is NaN already).  Values are read
+// once for the warp's rows; of positions with an infinity also the keys, as a
+// weight of exactly zero (a score of -inf) makes it NaN.  blocks[0 .. found -
+// 1]: the blocks with such values; more than WIN_BAD: all that the rows visit
+// are looked over.  2 x 4096 tokens of 4 heads (2) of 64 in float32, causal,
+// 0.51 ms: with one infinite v[0] 0.87, all values NaN 1.2, one column of them
+// infinite 5 ms.
+template <typename T, int WORDS>
+__device__ __noinline__ void window_not_finite(const WindowArgs& a, int z, int h, int i, bool on,
+                                               const int* blocks, int found, const Blocks visited) {
+    if (!__any_sync(0xffffffffu, on)) return;
+    const int lane = threadIdx.x % 32, kh = h / a.G;
+    const T* q = static_cast<const T*>(a.q) + ((int64_t)z * a.S + (on ? i : 0)) * a.ldq + (int64_t)h * a.D;
     const T* k = static_cast<const T*>(a.k) + (int64_t)z * a.S * a.ldk + (int64_t)kh * a.D;
     const T* v = static_cast<const T*>(a.v) + (int64_t)z * a.S * a.ldv + (int64_t)kh * a.D;
-    T* o = static_cast<T*>(a.o) + (((int64_t)z * a.S + i) * a.H + h) * a.D;
-    float qv[8], x[8];
+    const int rows_end = __reduce_max_sync(0xffffffffu, on ? i + 1 : 0);
+    uint32_t nan[WORDS], up[WORDS], down[WORDS];  // columns lane' + 32 w of this lane's row as bits
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = lane + 32 * e;
-        qv[e] = d < a.D ? zg_to_float(q[d]) * a.scale : 0.f;
-        x[e] = 0.f;
-    }
-    float m = -INFINITY, l = 0.f;
-    // four positions at a time, their reads in flight together
-    for (int j0 = 0; j0 <= i; j0 += 4) {
-        if (!sees(a, i, j0) && !sees(a, i, j0 + 3 < i ? j0 + 3 : i)) {
-            j0 = i - a.window - 3;  // the window's first position is next
-            continue;
-        }
-        float s[4], n = m;
-        bool on[4];
+    for (int w = 0; w < WORDS; ++w) nan[w] = up[w] = down[w] = 0u;
+    constexpr int N = WORDS <= 4 ? 32 / WORDS : 4;  // positions read at a time
+    float q_size = -1.f;  // sum of |q|, when it is first needed
+    const bool listed = found <= WIN_BAD;
+    int at = 0, b = listed ? blocks[0] : visited.sinks > 0 ? 0 : visited.lo;
+    while (listed ? at < found : b <= visited.last) {
+        const int end = (b + 1) * visited.keys < rows_end ? (b + 1) * visited.keys : rows_end;
+        for (int j0 = visited.has(b) ? b * visited.keys : end; j0 < end; j0 += N) {
+            T raw[N][WORDS];
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            on[g] = j0 + g <= i && sees(a, i, j0 + g);
-            s[g] = 0.f;
+            for (int g = 0; g < N; ++g)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = lane + 32 * e;
-                if (on[g] && d < a.D) s[g] = fmaf(qv[e], zg_to_float(k[(j0 + g) * a.ldk + d]), s[g]);
+                for (int w = 0; w < WORDS; ++w)
+                    raw[g][w] = j0 + g < end && lane + 32 * w < a.D ? v[(j0 + g) * a.ldv + lane + 32 * w] : zg_from_float<T>(0.f);
+            float sum = 0.f;  // 0 x is NaN where x is not finite
+#pragma unroll
+            for (int g = 0; g < N; ++g)
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) sum = fmaf(zg_to_float(raw[g][w]), 0.f, sum);
+            if (!__any_sync(0xffffffffu, sum != 0.f)) continue;
+            uint32_t infinite = 0u;
+#pragma unroll
+            for (int g = 0; g < N; ++g)
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) infinite |= isinf(zg_to_float(raw[g][w])) ? 1u : 0u;
+            // whether a weight of these positions may be exactly zero: |q . k| is at most sum |q| max |k|
+            bool zeros = false;
+            if (__any_sync(0xffffffffu, infinite)) {
+                float size = 0.f;
+#pragma unroll
+                for (int g = 0; g < N; ++g)
+#pragma unroll
+                    for (int w = 0; w < WORDS; ++w)
+                        size = fmaxf(size, fabsf(j0 + g < end && lane + 32 * w < a.D
+                                                     ? zg_to_float(k[(j0 + g) * a.ldk + lane + 32 * w]) : 0.f));
+#pragma unroll
+                for (int f = 16; f > 0; f >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, f));
+                if (q_size < 0.f) {
+                    q_size = 0.f;
+#pragma unroll 16
+                    for (int d = 0; d < a.D; ++d) q_size += fabsf(zg_to_float(q[d]));
+                }
+                zeros = __any_sync(0xffffffffu, on && !(size * q_size < 1e38f));
+            }
+#pragma unroll
+            for (int g = 0; g < N; ++g) {
+                const int j = j0 + g;
+                const bool see = on && j <= i && j < end && sees(a, i, j);
+                bool zero = false;
+                if (zeros && j < end) {
+                    float score = 0.f;
+                    for (int d = 0; d < a.D; ++d) score = fmaf(zg_to_float(q[d]), zg_to_float(k[j * a.ldk + d]), score);
+                    zero = score == -INFINITY;
+                }
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {
+                    const float x = zg_to_float(raw[g][w]);
+                    const uint32_t bn = __ballot_sync(0xffffffffu, isnan(x)), bu = __ballot_sync(0xffffffffu, x == INFINITY);
+                    const uint32_t bd = __ballot_sync(0xffffffffu, x == -INFINITY);
+                    if (!see) continue;
+                    nan[w] |= zero ? bn | bu | bd : bn;
+                    up[w] |= zero ? 0u : bu;
+                    down[w] |= zero ? 0u : bd;
+                }
             }
         }
+        ++at;
+        b = !listed ? visited.next(b) : at < found ? blocks[at] : 0;
+        bool rest = false;  // a column that may still change
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-#pragma unroll
-            for (int f = 16; f > 0; f >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], f);
-            s[g] = on[g] ? s[g] : -INFINITY;
-            n = fmaxf(n, s[g]);
+        for (int w = 0; w < WORDS; ++w) {
+            const int left = a.D - 32 * w;
+            rest = rest || (nan[w] != (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u));
         }
-        const float base = n == -INFINITY ? 0.f : n, c = exp2f(m - base);
-        l *= c;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= c;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float p = exp2f(s[g] - base);
-            l += p;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int d = lane + 32 * e;
-                if (on[g] && d < a.D) x[e] = fmaf(p, zg_to_float(v[(j0 + g) * a.ldv + d]), x[e]);
-            }
-        }
-        m = n;
+        if (!__any_sync(0xffffffffu, on && rest)) break;
     }
+    uint32_t any = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = lane + 32 * e;
-        if (d < a.D) o[d] = zg_from_float<T>(x[e] / l);
+    for (int w = 0; w < WORDS; ++w) {
+        nan[w] |= up[w] & down[w];
+        any |= nan[w] | up[w] | down[w];
+    }
+    T* o = static_cast<T*>(a.o) + ((int64_t)z * a.S * a.H + h) * a.D;
+    __syncwarp();  // the rows' other columns are written before these
+    for (uint32_t rows = __ballot_sync(0xffffffffu, any != 0u); rows; rows &= rows - 1) {
+        const int r = __ffs(rows) - 1;
+        T* to = o + (int64_t)__shfl_sync(0xffffffffu, i, r) * a.H * a.D;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+            const uint32_t rn = __shfl_sync(0xffffffffu, nan[w], r), ru = __shfl_sync(0xffffffffu, up[w], r);
+            const uint32_t rd = __shfl_sync(0xffffffffu, down[w], r);
+            if ((rn | ru | rd) >> lane & 1)
+                to[lane + 32 * w] = zg_from_float<T>(rn >> lane & 1 ? __int_as_float(0x7fffffff)
+                                                     : ru >> lane & 1 ? INFINITY : -INFINITY);
+        }
     }
 }
 
@@ -205,147 +270,170 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
     load(q_rows, qs, q, a.ldq, i0);
 
     const float2 zero2 = make_float2(0.f, 0.f);
+    const float low = ldexpf(1.f, -a.lift);
     float2 x[4][NC];
     float m[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) x[i][c] = zero2;
-    }
     const int last = i0 + WF_M < n ? i0 + WF_M : n;  // rows [i0, last)
     const int kt_end = (last + WF_N - 1) / WF_N;
     const int w0 = i0 - a.window + 1 > 0 ? (i0 - a.window + 1) / WF_N : 0;  // the window's first tile
     int sink_end = (a.sinks + WF_N - 1) / WF_N;                              // tiles that hold sinks
     if (sink_end > w0) sink_end = w0;
     auto next = [&](int kt) { return kt + 1 < sink_end || kt >= w0 ? kt + 1 : w0; };
-    int kt = sink_end > 0 ? 0 : w0;
-    load(k_rows, ks, k, a.ldk, kt * WF_N);
-    for (; kt < kt_end; kt = next(kt)) {
-        const int j0 = kt * WF_N;
-        load(k_rows, vs, v, a.ldv, j0);
-        copy_wait<1>();  // the keys
-        __syncthreads();
-        // the sixteens of this tile's keys that any row sees: [g0, g1)
-        int lo = i0 - a.window + 1 - j0, hi = last - j0;
-        if (lo <= 0 || j0 < a.sinks) lo = 0;
-        if (i0 - a.window + 1 - j0 >= WF_N) hi = a.sinks - j0;  // sinks alone
-        const int g0 = lo / 16, g1 = hi >= WF_N ? 4 : (hi + 15) / 16;
-        // the scores of NG sixteens, and their softmax into ps
-        auto scores = [&](auto groups) {
-            constexpr int NG = decltype(groups)::value;
-            const float* kr = ks + (16 * g0 + tx) * PITCH;
-            float2 s2[4][NG];
+    // Where an output is not finite although the weights' sum is, a value of
+    // a visited tile is not: the block goes over its tiles once more, with
+    // zeros in such places, and notes the tiles.
+    __shared__ int tiles[WIN_BAD];
+    int found = 0;
+    // (Two instances: with the test in one, 3 x 777 tokens of 8 heads of 80 took 55.0 us instead of 51.7.)
+    auto pass = [&](auto second) {
+        constexpr bool CLEAN = decltype(second)::value;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < NG; ++j) s2[i][j] = zero2;
-#pragma unroll 2
-            for (int d = 0; d < DP; d += 4) {
-                float4 qv[4], kv[NG];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * PITCH + d);
-#pragma unroll
-                for (int j = 0; j < NG; ++j) kv[j] = *reinterpret_cast<const float4*>(kr + 16 * j * PITCH + d);
+            for (int c = 0; c < NC; ++c) x[i][c] = zero2;
+        }
+        int kt = sink_end > 0 ? 0 : w0;
+        load(k_rows, ks, k, a.ldk, kt * WF_N);
+        for (; kt < kt_end; kt = next(kt)) {
+            const int j0 = kt * WF_N;
+            load(k_rows, vs, v, a.ldv, j0);
+            copy_wait<1>();  // the keys
+            __syncthreads();
+            // the sixteens of this tile's keys that any row sees: [g0, g1)
+            int lo = i0 - a.window + 1 - j0, hi = last - j0;
+            if (lo <= 0 || j0 < a.sinks) lo = 0;
+            if (i0 - a.window + 1 - j0 >= WF_N) hi = a.sinks - j0;  // sinks alone
+            const int g0 = lo / 16, g1 = hi >= WF_N ? 4 : (hi + 15) / 16;
+            // the scores of NG sixteens, and their softmax into ps
+            auto scores = [&](auto groups) {
+                constexpr int NG = decltype(groups)::value;
+                const float* kr = ks + (16 * g0 + tx) * PITCH;
+                float2 s2[4][NG];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
+                    for (int j = 0; j < NG; ++j) s2[i][j] = zero2;
+#pragma unroll 2
+                for (int d = 0; d < DP; d += 4) {
+                    float4 qv[4], kv[NG];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(qs + (ty + 8 * i) * PITCH + d);
+#pragma unroll
+                    for (int j = 0; j < NG; ++j) kv[j] = *reinterpret_cast<const float4*>(kr + 16 * j * PITCH + d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < NG; ++j) {
+                            s2[i][j] = ffma2_tc(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+                            s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+                        }
+                }
+                copy_wait<0>();  // the values
+                __syncthreads();
+                if (next(kt) < kt_end)
+                    load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
+                else
+                    copy_commit();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int qi = i0 + ty + 8 * i;
+                    float s[NG], t = m[i];
+#pragma unroll
                     for (int j = 0; j < NG; ++j) {
-                        s2[i][j] = ffma2_tc(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
-                        s2[i][j] = ffma2_tc(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+                        const int kj = j0 + 16 * (g0 + j) + tx;
+                        s[j] = kj <= qi && kj < n && sees(a, qi, kj) ? (s2[i][j].x + s2[i][j].y) * a.scale : -INFINITY;
+                        t = fmaxf(t, s[j]);
                     }
-            }
-            copy_wait<0>();  // the values
-            __syncthreads();
-            if (next(kt) < kt_end)
-                load(k_rows, ks, k, a.ldk, next(kt) * WF_N);
-            else
-                copy_commit();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int qi = i0 + ty + 8 * i;
-                float s[NG], t = m[i];
+                    for (int f = 8; f > 0; f >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, f));
+                    const float base = t == -INFINITY ? 0.f : t;
+                    const float c = exp2f(m[i] - base);
+                    m[i] = t;
+                    l[i] *= c;
 #pragma unroll
-                for (int j = 0; j < NG; ++j) {
-                    const int kj = j0 + 16 * (g0 + j) + tx;
-                    s[j] = kj <= qi && kj < n && sees(a, qi, kj) ? (s2[i][j].x + s2[i][j].y) * a.scale : -INFINITY;
-                    t = fmaxf(t, s[j]);
+                    for (int j = 0; j < NG; ++j) {
+                        const float p = exp2f(s[j] - base) * low;
+                        l[i] += p;
+                        ps[(ty + 8 * i) * WF_PP + 16 * (g0 + j) + tx] = p;
+                    }
+#pragma unroll
+                    for (int e = 0; e < NC; ++e) x[i][e] = ffma2_tc(x[i][e], make_float2(c, c), zero2);
                 }
-#pragma unroll
-                for (int f = 8; f > 0; f >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, f));
-                const float base = t == -INFINITY ? 0.f : t;
-                const float c = exp2f(m[i] - base);
-                m[i] = t;
-                l[i] *= c;
-#pragma unroll
-                for (int j = 0; j < NG; ++j) {
-                    const float p = exp2f(s[j] - base);
-                    l[i] += p;
-                    ps[(ty + 8 * i) * WF_PP + 16 * (g0 + j) + tx] = p;
-                }
-#pragma unroll
-                for (int e = 0; e < NC; ++e) x[i][e] = ffma2_tc(x[i][e], make_float2(c, c), zero2);
+            };
+            switch (g1 - g0) {
+                case 4: scores(std::integral_constant<int, 4>{}); break;
+                case 3: scores(std::integral_constant<int, 3>{}); break;
+                case 2: scores(std::integral_constant<int, 2>{}); break;
+                default: scores(std::integral_constant<int, 1>{});
             }
-        };
-        switch (g1 - g0) {
-            case 4: scores(std::integral_constant<int, 4>{}); break;
-            case 3: scores(std::integral_constant<int, 3>{}); break;
-            case 2: scores(std::integral_constant<int, 2>{}); break;
-            default: scores(std::integral_constant<int, 1>{});
-        }
-        __syncwarp();  // a row's weights are written and read by the same half warp
+            __syncwarp();  // a row's weights are written and read by the same half warp
+            if constexpr (CLEAN) {
+                bool bad = false;
+                for (int e = threadIdx.x; e < WF_N * DP; e += WF_THREADS) {
+                    float& value = vs[e / DP * PITCH + e % DP];
+                    if (!isfinite(value)) {
+                        value = 0.f;
+                        bad = true;
+                    }
+                }
+                if (__syncthreads_or(bad)) {
+                    if (threadIdx.x == 0 && found < WIN_BAD) tiles[found] = kt;
+                    ++found;
+                }
+            }
 #pragma unroll 4
-        for (int j = 16 * g0; j < 16 * g1; j += 4) {
-            float4 pv[4];
+            for (int j = 16 * g0; j < 16 * g1; j += 4) {
+                float4 pv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 8 * i) * WF_PP + j);
+                for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(ps + (ty + 8 * i) * WF_PP + j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 4; ++e) {
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const float2 vv = *reinterpret_cast<const float2*>(vs + (j + e) * PITCH + 32 * c + 2 * tx);
+                    for (int c = 0; c < NC; ++c) {
+                        const float2 vv = *reinterpret_cast<const float2*>(vs + (j + e) * PITCH + 32 * c + 2 * tx);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
-                        x[i][c] = ffma2_tc(make_float2(p, p), vv, x[i][c]);
+                        for (int i = 0; i < 4; ++i) {
+                            const float p = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
+                            x[i][c] = ffma2_tc(make_float2(p, p), vv, x[i][c]);
+                        }
                     }
                 }
             }
+            __syncthreads();  // the values have been read
         }
-        __syncthreads();  // the values have been read
-    }
-    unsigned redo = 0;  // bit i: row i of this half warp is formed again
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int f = 8; f > 0; f >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], f);
-        const int qi = i0 + ty + 8 * i;
+        unsigned known = 0;  // bit i: row i's weights have a finite sum (else all of it is NaN, by its visible scores)
         bool fine = true;
-        const bool known = l[i] > 0.f && l[i] < INFINITY;  // else all NaN, by its visible scores
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = 32 * c + 2 * tx + e;
-                const float y = qi < n ? (e ? x[i][c].y : x[i][c].x) / l[i] : 0.f;
-                if (d < a.D) {
-                    fine = fine && isfinite(y);
-                    if (qi < a.S) o[qi * ldo + d] = zg_from_float<T>(y);
+            for (int f = 8; f > 0; f >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], f);
+            const int qi = i0 + ty + 8 * i;
+            if (l[i] > 0.f && l[i] < INFINITY) known |= 1u << i;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = 32 * c + 2 * tx + e;
+                    const float y = qi < n ? (e ? x[i][c].y : x[i][c].x) / l[i] : 0.f;
+                    if (d < a.D) {
+                        fine = fine && (isfinite(y) || !(known >> i & 1));
+                        if (qi < a.S) o[qi * ldo + d] = zg_from_float<T>(y);
+                    }
                 }
-            }
-        const unsigned half = 0xffffu << (threadIdx.x % 32 / 16 * 16);
-        if (__ballot_sync(0xffffffffu, known && !fine) & half) redo |= 1u << i;
-    }
-    // the rows of this warp's two halves, one at a time by the whole warp
-    for (int t = 0; t < 2; ++t) {
-        const unsigned rows = __shfl_sync(0xffffffffu, redo, 16 * t);
-        for (int i = 0; i < 4; ++i)
-            if (rows >> i & 1) {
-                __syncwarp();  // the row's first values are written before these
-                window_row<T>(a, z, i0 + (int)(threadIdx.x / 32) * 2 + t + 8 * i, h);
-            }
-    }
+        }
+        if constexpr (CLEAN) {
+            // lane r: row (r % 2) + 8 (r / 2) of this warp's eight
+            const int lane = threadIdx.x % 32, i = i0 + (int)(threadIdx.x / 32) * 2 + lane % 2 + 8 * (lane / 2);
+            const unsigned bits = __shfl_sync(0xffffffffu, known, 16 * (lane % 2));
+            if (found)
+                window_not_finite<T, NC>(a, z, h, i, lane < 8 && i < n && (bits >> (lane / 2 & 3) & 1), tiles, found,
+                                         Blocks{WF_N, sink_end, w0, kt_end - 1});
+        }
+        return fine;
+    };
+    if (__syncthreads_or(!pass(std::false_type{}))) pass(std::true_type{});
 }
 
 template <typename T, int DP>
@@ -452,10 +540,12 @@ constexpr uint16_t WT_REDO = 0x7fa5;
 // and those that this tile does.
 struct WtUnit {
     int z, h, n, i0, sink_blocks, lo0, hi;
-    int lo, last;  // the first block of this tile's window, and its last (-1: a tile behind the sequence)
+    int w0, lo, last;  // the first position of the unit's window; the first block of this tile's, and its last (-1: a tile behind the sequence)
     bool any, both;  // whether the sequence reaches the first tile, and the second
     __device__ __forceinline__ bool takes(int b) const { return b <= last && (b >= lo || b < sink_blocks); }
     __device__ __forceinline__ int first() const { return sink_blocks > 0 ? 0 : lo0; }
+    // whether the blocks that hold sinks hold no other keys that a row sees
+    __device__ __forceinline__ bool sinks_apart(int keys) const { return sink_blocks * keys <= w0; }
     __device__ __forceinline__ int next(int b) const { return b + 1 < sink_blocks || b + 1 >= lo0 ? b + 1 : lo0; }
 };
 
@@ -470,8 +560,9 @@ __device__ __forceinline__ WtUnit wt_unit(const WindowArgs& a, int u, int pairs,
     x.any = x.i0 < x.n;
     x.both = x.i0 + 128 < x.n;
     x.sink_blocks = (a.sinks + KEYS - 1) / KEYS;
-    const int w0 = x.i0 - a.window + 1, w = w0 + 128 * t;
-    x.lo0 = w0 > 0 ? w0 / KEYS : 0;
+    x.w0 = x.i0 - a.window + 1;
+    const int w = x.w0 + 128 * t;
+    x.lo0 = x.w0 > 0 ? x.w0 / KEYS : 0;
     x.lo = w > 0 ? w / KEYS : 0;
     const int end = x.i0 + 256 < x.n ? x.i0 + 256 : x.n, mine = x.i0 + 128 * (t + 1);
     x.hi = (end - 1) / KEYS;
@@ -504,6 +595,264 @@ __device__ __forceinline__ int unit_answer(const uint4* from) {
         : "r"(smem_u32(from))
         : "memory");
     return u;
+}
+
+// Whether a value that the blocks of a warp's 32 rows (from row0) hold and
+// that not all of them see is not finite: behind the first row, before the
+// last one's window, or beside the sinks.
+template <int KEYS>
+__device__ __forceinline__ bool masked_not_finite(const WindowArgs& a, const WtUnit& x, int row0) {
+    const int words = a.D / 8, last = row0 + 31 < x.n - 1 ? row0 + 31 : x.n - 1;
+    const int end = (x.last + 1) * KEYS < x.n ? (x.last + 1) * KEYS : x.n;
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+    __nv_bfloat162 sum = zero;  // 0 x is NaN where x is not finite
+#pragma unroll 1
+    for (int part = 0; part < 3; ++part) {
+        if (part == 2 && x.sinks_apart(KEYS)) break;
+        const int from = part == 0 ? row0 + 1 : part == 1 && x.lo * KEYS > a.sinks ? x.lo * KEYS : a.sinks;
+        const int to = part == 0 ? end : part == 1 ? last - a.window + 1 : x.sink_blocks * KEYS < end ? x.sink_blocks * KEYS : end;
+        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v) + ((int64_t)x.z * a.S + from) * a.ldv + (int64_t)(x.h / a.G) * a.D;
+#pragma unroll 4
+        for (int at = threadIdx.x % 32; at < (to - from) * words; at += 32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(v + at / words * a.ldv + at % words * 8);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.x), zero, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.y), zero, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.z), zero, sum);
+            sum = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w.w), zero, sum);
+        }
+    }
+    return __any_sync(0xffffffffu, __low2float(sum) != 0.f || __high2float(sum) != 0.f);
+}
+
+// Rows r0 .. of the set bits of `rows` once more, by one warp: 16 keys at a
+// time as in the paged kernel (a ring of tiles by cp.async, m16n8k16
+// products, a running maximum), over what any of the rows sees, with zeros
+// for values that are infinite or NaN.  Then those values are written into
+// the outputs that see them: of the blocks that held any, products of the mask
+// with ones in their places count in each output the visible NaN and
+// infinities of either sign.  (A visible score of -inf is a weight of zero,
+// and 0 x inf is NaN.)  ring: 24 KB of this warp's.  2 x 4096 tokens of 12
+// heads (4) of 64, causal, 0.10 ms a call: with one infinite v[0], which only
+// rows that see it meet, the same; with a NaN 60 positions before the end 0.43;
+// all values NaN, or one column infinite, 1.9 ms (0.6 us for 16 keys and 16
+// rows; rows of their own, key by key, would take over a second).
+template <int DP>
+__device__ __forceinline__ void window_rows(const WindowArgs& a, uint8_t* ring, int z, int h, int n, int r0, uint32_t rows) {
+    using T = __nv_bfloat16;
+    constexpr int TILE = 16 * DP * 2, STAGES = 24576 / (2 * TILE), CPR = DP / 8, ONE = 0x3f80;
+    const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4, kh = h / a.G;
+    const T* q = static_cast<const T*>(a.q) + (int64_t)z * a.S * a.ldq + (int64_t)h * a.D;
+    const T* k = static_cast<const T*>(a.k) + (int64_t)z * a.S * a.ldk + (int64_t)kh * a.D;
+    const T* v = static_cast<const T*>(a.v) + (int64_t)z * a.S * a.ldv + (int64_t)kh * a.D;
+    T* o = static_cast<T*>(a.o) + ((int64_t)z * a.S * a.H + h) * a.D;
+    const int w0 = r0 - a.window + 1, end = r0 + 15 < n - 1 ? r0 + 15 : n - 1;
+    const Blocks blocks{16, (a.sinks + 15) / 16, w0 > 0 ? w0 / 16 : 0, end / 16};
+    int bad[WIN_BAD], found = 0;  // blocks with such values
+
+    // body(block, its keys and values in shared memory), for all blocks or for the bad ones alone
+    auto walk = [&](bool all, auto body) {
+        int at = 0;
+        auto first = [&]() { return all ? (blocks.sinks > 0 ? 0 : blocks.lo) : bad[0]; };
+        auto fetch = [&](int stage, int b) {
+#pragma unroll
+            for (int it = 0; it < CPR / 2; ++it) {
+                const int x = it * 32 + lane, r = x / CPR, w = x % CPR;
+                const bool on = 16 * b + r < n && w * 8 < a.D;
+                const uint32_t to = shared_u32(ring + stage * 2 * TILE) + r * (DP * 2) + ((w ^ (r & 7)) * 16);
+                copy16(to, on ? k + (int64_t)(16 * b + r) * a.ldk + w * 8 : k, on ? 16 : 0);
+                copy16(to + TILE, on ? v + (int64_t)(16 * b + r) * a.ldv + w * 8 : v, on ? 16 : 0);
+            }
+        };
+        auto after = [&](int b, int& i) { return all ? blocks.next(b) : ++i < found ? bad[i] : INT32_MAX; };
+        int ahead = first(), ahead_at = 0;
+        for (int s = 0; s < STAGES - 1; ++s) {
+            if (ahead <= blocks.last) {
+                fetch(s, ahead);
+                ahead = after(ahead, ahead_at);
+            }
+            copy_commit();
+        }
+        int stage = 0;
+        for (int b = first(); b <= blocks.last; b = after(b, at)) {
+            copy_wait<STAGES - 2>();
+            __syncwarp();
+            if (ahead <= blocks.last) {
+                fetch((stage + STAGES - 1) % STAGES, ahead);
+                ahead = after(ahead, ahead_at);
+            }
+            copy_commit();
+            const uint32_t kt = shared_u32(ring + stage * 2 * TILE);
+            body(b, kt, kt + TILE);
+            stage = (stage + 1) % STAGES;
+        }
+        copy_wait<0>();
+        __syncwarp();
+    };
+
+    uint32_t qf[DP / 16][4];
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = r0 + g + 8 * (e & 1) < n ? r0 + g + 8 * (e & 1) : n - 1, d = 16 * t + 2 * c + 8 * (e >> 1);
+            qf[t][e] = d < a.D ? *reinterpret_cast<const uint32_t*>(q + i * a.ldq + d) : 0u;
+        }
+    const int k_row = (lane % 8) + 8 * (lane / 16), k_word = (lane / 8) % 2;
+    const int v_row = (lane % 8) + 8 * ((lane / 8) % 2), v_word = lane / 16;
+    auto scores = [&](float (&s)[2][4], uint32_t kt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[0][e] = s[1][e] = 0.f;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            uint32_t f[4];
+            ldmatrix4(f, kt + k_row * (DP * 2) + (((2 * t + k_word) ^ (k_row & 7)) * 16));
+            mma_bf16(s[0], qf[t], f[0], f[1]);
+            mma_bf16(s[1], qf[t], f[2], f[3]);
+        }
+    };
+    auto values = [&](uint32_t (&f)[4], uint32_t vt, int t) {
+        ldmatrix4_t(f, vt + v_row * (DP * 2) + (((2 * t + v_word) ^ (v_row & 7)) * 16));
+    };
+    // rows r0 + g and r0 + g + 8; a score's or an output's element e is of the row e / 2, and of the
+    // key or column 8 j + 2 c + e % 2
+    auto sees_key = [&](int b, int j, int e) {
+        const int i = r0 + g + 8 * (e >> 1), key = 16 * b + 8 * j + 2 * c + (e & 1);
+        return key <= i && sees(a, i, key);
+    };
+    float l[2] = {0.f, 0.f};
+    {
+        float x[DP / 8][4], m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) x[d][0] = x[d][1] = x[d][2] = x[d][3] = 0.f;
+        const float low = ldexpf(1.f, -a.lift);
+        walk(true, [&](int b, uint32_t kt, uint32_t vt) {
+            float s[2][4];
+            scores(s, kt);
+            float top[2] = {m[0], m[1]}, f[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[j][e] = sees_key(b, j, e) ? s[j][e] * a.scale : -INFINITY;
+                    top[e >> 1] = fmaxf(top[e >> 1], s[j][e]);
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                const float base = top[r] == -INFINITY ? 0.f : top[r];
+                f[r] = exp2_fast(m[r] - base);
+                m[r] = top[r];
+                l[r] *= f[r];
+                top[r] = base;
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[d][e] *= f[e >> 1];
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float y0 = exp2_fast(s[j][2 * r] - top[r]) * low, y1 = exp2_fast(s[j][2 * r + 1] - top[r]) * low;
+                    l[r] += y0 + y1;
+                    p[2 * j + r] = pack_bf16(y0, y1);
+                }
+            bool spoilt = false;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) {
+                uint32_t w[4];
+                values(w, vt, t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool lo = (w[e] & 0x7f80u) == 0x7f80u, hi = (w[e] & 0x7f800000u) == 0x7f800000u;
+                    spoilt = spoilt || lo || hi;
+                    w[e] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0x0000ffffu : ~0u);
+                }
+                mma_bf16(x[2 * t], p, w[0], w[1]);
+                mma_bf16(x[2 * t + 1], p, w[2], w[3]);
+            }
+            if (__any_sync(0xffffffffu, spoilt)) {
+                if (found < WIN_BAD) bad[found] = b;
+                ++found;
+            }
+        });
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            if (!(rows >> (g + 8 * r) & 1)) continue;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+                if (8 * d < a.D)
+                    *reinterpret_cast<uint32_t*>(o + (int64_t)(r0 + g + 8 * r) * a.H * a.D + 8 * d + 2 * c) =
+                        pack_bf16(x[d][2 * r] / l[r], x[d][2 * r + 1] / l[r]);
+        }
+    }
+    if (!found) return;
+    float up[DP / 8][4], down[DP / 8][4];  // visible +inf or NaN, and -inf or NaN
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) up[d][e] = down[d][e] = 0.f;
+    walk(found > WIN_BAD, [&](int b, uint32_t kt, uint32_t vt) {
+        float s[2][4];
+        scores(s, kt);
+        uint32_t some[4], none[4];  // ones where the weight is above zero, and where it is zero
+        bool zeros = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                some[2 * j + r] = none[2 * j + r] = 0u;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (!sees_key(b, j, 2 * r + e)) continue;
+                    const bool zero = s[j][2 * r + e] == -INFINITY;
+                    (zero ? none : some)[2 * j + r] |= ONE << 16 * e;
+                    zeros = zeros || zero;
+                }
+            }
+        zeros = __any_sync(0xffffffffu, zeros);
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) {
+            uint32_t w[4], wu[4], wd[4];
+            values(w, vt, t);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                wu[e] = wd[e] = 0u;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t y = w[e] >> 16 * x & 0xffffu;
+                    if ((y & 0x7fffu) > 0x7f80u || y == 0x7f80u) wu[e] |= ONE << 16 * x;
+                    if ((y & 0x7fffu) > 0x7f80u || y == 0xff80u) wd[e] |= ONE << 16 * x;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mma_bf16(up[2 * t + e], some, wu[2 * e], wu[2 * e + 1]);
+                mma_bf16(down[2 * t + e], some, wd[2 * e], wd[2 * e + 1]);
+            }
+            if (!zeros) continue;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mma_bf16(up[2 * t + e], none, wu[2 * e] | wd[2 * e], wu[2 * e + 1] | wd[2 * e + 1]);
+                mma_bf16(down[2 * t + e], none, wu[2 * e] | wd[2 * e], wu[2 * e + 1] | wd[2 * e + 1]);
+            }
+        }
+    });
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = e >> 1;
+            const bool known = l[r] > 0.f && l[r] < INFINITY;  // else all of the row is NaN
+            if (8 * d < a.D && known && (rows >> (g + 8 * r) & 1) && (up[d][e] > 0.f || down[d][e] > 0.f))
+                o[(int64_t)(r0 + g + 8 * r) * a.H * a.D + 8 * d + 2 * c + (e & 1)] =
+                    __float2bfloat16(up[d][e] > 0.f && down[d][e] > 0.f ? __int_as_float(0x7fffffff)
+                                     : up[d][e] > 0.f ? INFINITY : -INFINITY);
+        }
 }
 
 // Bits 0 .. x of a word.
@@ -575,7 +924,8 @@ __device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
 template <int DP>
 __global__ void __launch_bounds__(WT_THREADS, 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                 const __grid_constant__ CUtensorMap tmV, const WindowArgs a, int pairs) {
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmSinks, const WindowArgs a,
+                 int pairs) {
     using W = WtShape<DP>;
     // No static shared memory, so the dynamic block starts at the CTA's first
     // shared byte; the swizzled tiles need it 1024-aligned, which is checked.
@@ -656,7 +1006,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     for (int d = 0; d < DP / 64; ++d) {
                         uint8_t* to = smem + W::RING + st * 2 * W::BLOCK + d * W::BOX;
                         tma_load_4d(to, &tmK, &c.kv_full[st], 64 * d, kh, b * W::KEYS, x.z);
-                        tma_load_4d(to + W::BLOCK, &tmV, &c.kv_full[st], 64 * d, kh, b * W::KEYS, x.z);
+                        // the values beside the sinks, that nobody sees, as zeros (they may be infinite or NaN)
+                        tma_load_4d(to + W::BLOCK, b < x.sink_blocks && x.sinks_apart(W::KEYS) ? &tmSinks : &tmV,
+                                    &c.kv_full[st], 64 * d, kh, b * W::KEYS, x.z);
                     }
                 }
                 if (ok && ahead >= 0) ok = queries(1);  // a unit of two blocks or fewer
@@ -754,6 +1106,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint32_t trow = tmem + ((uint32_t)(quad * 32) << 16);
         const uint32_t oc = trow + W::o_col(t);
         const int64_t ldo = (int64_t)a.H * a.D;
+        const float lift = (float)a.lift + 8.f, slack = 8.f - lift;  // weights up to 2^8 times those of the maximum
         const float2 one2 = make_float2(1.f, 1.f), scale2 = make_float2(a.scale, a.scale);
         uint32_t nb = 0, nu = 0, taken = 0;  // blocks and units of this tile so far, units of both
         bool s_ready = false;                // the next scores have been seen to be there
@@ -769,7 +1122,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 }
                 continue;
             }
-            float m = -INFINITY;  // what the weights are taken against, in units of log2
+            float m = -INFINITY;  // what the weights are taken against, in units of log2: a maximum so far, and lift
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             bool first = true;
             for (int b = x.first(); b <= x.hi; b = x.next(b)) {
@@ -778,8 +1131,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 if (!s_ready && !(ok = warp_wait(&c.s_full[t], nb & 1, 111))) break;
                 tc_fence_after();
                 const int j0 = b * W::KEYS;
-                // The maximum m is moved to the row's (mx, scaled) where that is more
-                // than 2^8 above; false when a wait ran out.
+                // m is moved to the row's maximum (mx, scaled) and lift where that is
+                // more than 2^8 above the one it was taken from; false when a wait ran out.
                 auto settle = [&](float mx, bool pv_seen) {
                     // P V of the block before has read the weights' buffer and added to O
                     const bool all_seen = __all_sync(0xffffffffu, pv_seen);
@@ -787,10 +1140,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                         if (!all_seen && !warp_wait(&c.pv_done[t], (nb - 1) & 1, 112)) return false;
                         tc_fence_after();
                     }
-                    if (!__any_sync(0xffffffffu, i < x.n && !(mx <= m + 8.f))) return true;  // rows behind the sequence do not count
-                    const float n = fmaxf(m, mx);
+                    if (!__any_sync(0xffffffffu, i < x.n && !(mx <= m + slack))) return true;  // rows behind the sequence do not count
+                    const float n = fmaxf(m, mx + lift);
                     float f = exp2_fast(m - (n == -INFINITY ? 0.f : n));
-                    // a score that is NaN or infinite: the row is formed again at the end
+                    // a score that is NaN or +inf makes the weights' sum NaN, and with it all of the row
                     if (!(mx < INFINITY)) f = __int_as_float(0x7fffffff);
                     m = n;
 #pragma unroll
@@ -961,8 +1314,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             tc_fence_before();
             mbar_arrive(&c.o_empty[t]);
-            const bool again = !fine && l > 0.f && l < INFINITY;
-            if (__any_sync(0xffffffffu, again)) {
+            const bool again = in && !fine && l > 0.f && l < INFINITY;
+            if (__any_sync(0xffffffffu, again) && masked_not_finite<W::KEYS>(a, x, row0)) {
                 int* before = &c.redo[warp - 4];
                 if (again) {
                     *reinterpret_cast<uint16_t*>(o) = WT_REDO;
@@ -973,18 +1326,25 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 __syncwarp();
             }
         }
-        // The marked rows, the last unit's first, when no role waits for this one
-        // any more: a row of 10^5 keys takes longer than the waits' limit.
-        for (int u = ok ? c.redo[warp - 4] : -1; u >= 0;) {
+        const int last = ok ? c.redo[warp - 4] : -1;
+        tc_fence_before();
+        __syncthreads();
+        // The marked rows, the last unit's first, when nobody waits for this warp
+        // and the ring of blocks is free.
+        for (int u = last; u >= 0;) {
             const WtUnit x = wt_unit<W::KEYS>(a, u, pairs, t);
             const int row0 = x.i0 + 128 * t + 32 * quad, i = row0 + lane;
             const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(a.o) + ((int64_t)x.z * a.S + i) * ldo + (int64_t)x.h * a.D;
-            const bool again = i < x.n && *reinterpret_cast<const uint16_t*>(o) == WT_REDO;
-            const int before = again ? *reinterpret_cast<const int*>(o + 2) : -1;
-            uint32_t rows = __ballot_sync(0xffffffffu, again);
+            const bool again = i < x.n && *reinterpret_cast<const volatile uint16_t*>(o) == WT_REDO;
+            const int before = again ? *reinterpret_cast<const volatile int*>(o + 2) : -1;
+            const uint32_t rows = __ballot_sync(0xffffffffu, again);
             u = __shfl_sync(0xffffffffu, before, __ffs(rows) - 1);
-            for (; rows; rows &= rows - 1) window_row<__nv_bfloat16>(a, x.z, row0 + __ffs(rows) - 1, x.h);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half)
+                if (rows >> 16 * half & 0xffffu)
+                    window_rows<DP>(a, smem + (warp - 4) * 24576, x.z, x.h, x.n, row0 + 16 * half, rows >> 16 * half & 0xffffu);
         }
+        return;
     }
     tc_fence_before();
     __syncthreads();
@@ -997,14 +1357,15 @@ window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 template <int DP>
 int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
     using W = WtShape<DP>;
-    CUtensorMap tq, tk, tv;
-    auto map = [&](CUtensorMap* m, const void* p, int heads, int64_t ld, uint32_t rows) {
+    CUtensorMap tq, tk, tv, ts;
+    auto map = [&](CUtensorMap* m, const void* p, int heads, int64_t ld, uint32_t rows, int positions) {
         const uint32_t box[4] = {64, 1, rows, 1};
-        const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)heads, (uint64_t)a.S, (uint64_t)a.Z};
+        const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)heads, (uint64_t)positions, (uint64_t)a.Z};
         const uint64_t strides[3] = {(uint64_t)a.D * 2, (uint64_t)ld * 2, (uint64_t)a.S * ld * 2};
         return zg::tensor_map_bf16(m, p, 4, dims, strides, box, true);
     };
-    if (!map(&tq, a.q, a.H, a.ldq, 128) || !map(&tk, a.k, a.K, a.ldk, W::KEYS) || !map(&tv, a.v, a.K, a.ldv, W::KEYS))
+    if (!map(&tq, a.q, a.H, a.ldq, 128, a.S) || !map(&tk, a.k, a.K, a.ldk, W::KEYS, a.S) ||
+        !map(&tv, a.v, a.K, a.ldv, W::KEYS, a.S) || !map(&ts, a.v, a.K, a.ldv, W::KEYS, a.sinks > 0 ? a.sinks : 1))
         return zg::fail(ZG_ERR_CUDA, "zg_window_attention: tensor maps");
     if (cudaFuncSetAttribute(window_tc_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::SMEM) !=
         cudaSuccess)
@@ -1013,7 +1374,7 @@ int launch_window_tc(const WindowArgs& a, cudaStream_t st) {
     const int64_t units = (int64_t)a.Z * a.H * pairs;
     if (units > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_window_attention: too many rows");
     zg::LaunchTimer zg_lt_("window_attention", st);
-    window_tc_kernel<DP><<<(unsigned)units, WT_THREADS, W::SMEM, st>>>(tq, tk, tv, a, pairs);
+    window_tc_kernel<DP><<<(unsigned)units, WT_THREADS, W::SMEM, st>>>(tq, tk, tv, ts, a, pairs);
     return zg::check_launch("zg_window_attention");
 }
 
@@ -1040,9 +1401,11 @@ extern "C" int zg_window_attention(const void* q, int64_t ldq, const void* k, in
     if (!zg::dtype_ok(dtype)) return zg::fail(ZG_ERR_INVALID, "zg_window_attention: bad dtype");
     if (Z == 0 || S == 0) return ZG_OK;
     if (!q || !k || !v || !o) return zg::fail(ZG_ERR_INVALID, "zg_window_attention: null pointer");
+    int lift = 1;
+    while (((int64_t)1 << (lift - 1)) <= S) ++lift;
     const WindowArgs a{q, k, v, o, lengths, ldq, ldk, ldv, (int)Z, (int)S, H, K, D, H / K,
                        window > 0 && window < S ? window : (int)S, sinks < S ? sinks : (int)S,
-                       (float)(1.4426950408889634 / sqrt((double)D))};
+                       (float)(1.4426950408889634 / sqrt((double)D)), lift};
     cudaStream_t st = zg::as_stream(stream);
     auto al = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     if (dtype == ZG_BF16 && D <= 128 && D % 8 == 0 && ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && al(q) && al(k) &&

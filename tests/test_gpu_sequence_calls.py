@@ -141,7 +141,7 @@ def test_window_attention_time_with_values_not_finite(cuda, dtype, H, K, D, wind
     """One infinite value that most rows see, one beside the sinks, a NaN late,
     a column of one sign, all-NaN values, all-NaN activations, padding of NaN:
     without a cost where no row that does not see it is touched, and bounded
-    where many are.  (Rows gone over key by key took hundreds of times.)"""
+    where many are."""
     S = 4096
     q, k, v = (_rand((2, S, h, D), dtype, h, cuda) for h in (H, K, K))
     lengths = torch.tensor([S, S // 2 + 1], device=cuda)

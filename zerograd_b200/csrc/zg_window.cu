@@ -635,7 +635,7 @@ __device__ __forceinline__ bool masked_not_finite(const WindowArgs& a, const WtU
 // heads (4) of 64, causal, 0.10 ms a call: with one infinite v[0], which only
 // rows that see it meet, the same; with a NaN 60 positions before the end 0.43;
 // all values NaN, or one column infinite, 1.9 ms (0.6 us for 16 keys and 16
-// rows; rows of their own, key by key, would take over a second).
+// rows).
 template <int DP>
 __device__ __forceinline__ void window_rows(const WindowArgs& a, uint8_t* ring, int z, int h, int n, int r0, uint32_t rows) {
     using T = __nv_bfloat16;

@@ -585,9 +585,13 @@ ZG_API int zg_append_pages(void* k_pages, void* v_pages, int64_t n_pages, int pa
  * contiguous, D <= 256.  A length of 0 gives zeros; a length that the table
  * cannot hold, or a visible page that is not one of the pool's, gives NaN.
  * bf16 pages with D a multiple of 8 are 16-byte aligned (and q 4-byte, ldq
- * even).  At most 2^30 positions in a row of the table and in the pool.  The
- * workspace (16-byte aligned) holds the splits' partial sums; 0 bytes where
- * one split, or a cluster of up to eight, does. */
+ * even).  At most 2^30 positions in a row of the table and in the pool.  A
+ * sequence's result has the same bits whatever else is in the launch: it is cut
+ * by its own visible length and the heads.  bf16 with D a multiple of 8
+ * multiplies on the tensor cores: weights are rounded to bf16 for the second
+ * product (2^-8 of each), scores, sums and outputs so far are float32.  The
+ * workspace (16-byte aligned) holds the pieces' sums where a unit's blocks do
+ * not join them by themselves; else 0 bytes. */
 ZG_API size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int D, int max_pages, int page, int window,
                                                 int sinks, int dtype);
 ZG_API int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages, int64_t n_pages,

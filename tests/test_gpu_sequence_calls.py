@@ -163,3 +163,60 @@ def test_window_attention_time_with_values_not_finite(cuda, dtype, H, K, D, wind
     assert L.load().zg_device_error(1) == 0
     assert slow["first"] < 3 and slow["activations"] < 2 and slow["padding"] < 2, slow
     assert slow["late"] < 12 and slow["beside the sinks"] < 12 and slow["column"] < 50 and slow["all"] < 50, slow
+
+
+# ------------------------------------------------ a sequence's result is its own
+
+
+def _cache(lengths, page, K, D, dtype, device, seed=1, spare=2):
+    """A pool that holds the sequences, and their table (-1 behind each one's pages)."""
+    need = [-(-n // page) for n in lengths]
+    g = torch.Generator(device=device).manual_seed(seed)
+    kp, vp = (torch.randn((sum(need) + spare, page, K, D), generator=g, device=device).to(dtype) for _ in range(2))
+    order = torch.randperm(sum(need) + spare, generator=g, device=device).to(torch.int32)
+    table = torch.full((len(lengths), max(need + [1])), -1, dtype=torch.int32, device=device)
+    at = 0
+    for b, m in enumerate(need):
+        table[b, :m] = order[at:at + m]
+        at += m
+    return kp, vp, table
+
+
+@pytest.mark.parametrize("dtype,H,K,D,window,sinks", [
+    (BF, 4, 2, 64, None, 0), (BF, 8, 1, 128, None, 0), (BF, 12, 12, 64, 3000, 4), (BF, 4, 4, 192, None, 0),
+    (BF, 20, 1, 128, None, 0), (BF, 3, 1, 20, None, 0), (F32, 4, 2, 64, None, 0), (F32, 16, 2, 136, 2500, 0),
+    (F32, 2, 2, 128, None, 0)])
+def test_paged_attention_of_a_sequence_whatever_else_is_in_the_launch(cuda, dtype, H, K, D, window, sinks):
+    """The bits of a sequence's output do not depend on the other sequences,
+    their number, or the table's width: a candidate's loss is its own."""
+    lengths = [9000, 0, 4096, 130, 1, 2000, 700, 1024, 5555, 300]
+    kp, vp, table = _cache(lengths, 16, K, D, dtype, cuda)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    q = _rand((len(lengths), H, D), dtype, 3, cuda)
+    want = zg.paged_attention(q, kp, vp, table, n, window, sinks)
+    full, mag = so.paged_attention(q.cpu(), kp.cpu(), vp.cpu(), table.cpu(), n.cpu(), window, sinks)
+    so.assert_within(want, full, so.attention_tolerance(q.cpu(), kp.cpu(), full, mag, dtype, max(lengths)))
+    wide = torch.nn.functional.pad(table, (0, 4000), value=-1)
+    assert torch.equal(zg.paged_attention(q, kp, vp, wide, n, window, sinks), want)
+    for b, m in enumerate(lengths):
+        own = table[b:b + 1, :max(1, -(-m // 16))].contiguous()
+        for t in (own, wide[b:b + 1]):
+            assert torch.equal(zg.paged_attention(q[b:b + 1], kp, vp, t, n[b:b + 1], window, sinks)[0], want[b]), m
+    for some in ([0, 3], [2, 5, 7, 8], [9, 6, 3] * 20, list(range(10)) * 7, [5, 7, 0, 4] * 110):
+        at = torch.tensor(some, device=cuda)
+        for t in (table, wide):
+            got = zg.paged_attention(q[at], kp, vp, t[at], n[at], window, sinks)
+            assert torch.equal(got, want[at]), len(some)
+
+
+@pytest.mark.parametrize("dtype,D,longest", [(BF, 64, 5000), (BF, 128, 900), (F32, 64, 5000)])
+def test_paged_attention_under_vmap_over_long_caches(cuda, dtype, D, longest):
+    """Three candidates of two sequences: the bits of the calls candidate by candidate."""
+    P, H, K = 3, 4, 2
+    lengths = [longest, longest // 3, 17, longest - 1, longest // 2, 640]
+    kp, vp, table = _cache(lengths, 16, K, D, dtype, cuda)
+    table, n = table.reshape(P, 2, -1), torch.tensor(lengths, device=cuda).reshape(P, 2)
+    q = _rand((P, 2, H, D), dtype, 5, cuda)
+    got = torch.func.vmap(lambda qq, tt, nn: zg.paged_attention(qq, kp, vp, tt, nn))(q, table, n)
+    for p in range(P):
+        assert torch.equal(zg.paged_attention(q[p], kp, vp, table[p], n[p]), got[p])

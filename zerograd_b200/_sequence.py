@@ -451,9 +451,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     row of :func:`window_attention` does.  Pages may be shared by sequences.
     A sequence of length 0 gives zeros; a length the table cannot hold, or a
     visible page that is not one of the pool's, gives NaN.  D is at most 256;
-    float32 or bf16 (bf16 with D a multiple of 8 multiplies on the tensor
-    cores, pages 16-byte aligned).  The cache is read once; the work is split
-    over its length and joined in a fixed order."""
+    float32 or bf16.  bf16 with D a multiple of 8 multiplies on the tensor
+    cores (pages 16-byte aligned; scores and sums in float32, weights rounded
+    to bf16).  The cache is read once.  A sequence is cut by its own visible
+    length and joined in a fixed order, so its result has the same bits
+    whatever else is in the launch: other sequences, other candidates under
+    vmap, a wider table."""
     w, s = _span(window, sinks)
     args = (q, k_pages, v_pages, page_table, lengths, w, s)
     return launch_paged_attention(*args) if _plain_call(*args[:5]) else _paged_op(*args)

@@ -16,6 +16,9 @@
 // ---------------------------------------------------------------------------
 namespace zg {
 
+// SMs of the current device (148 where there is none).
+int sm_count();
+
 void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);

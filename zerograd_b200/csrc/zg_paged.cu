@@ -102,21 +102,38 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // ---------------------------------------------------------------------------
 // attention of one token
 // ---------------------------------------------------------------------------
+// How a sequence is cut is a matter of what it sees and of the heads alone, so
+// that its result has the same bits whatever else is in the launch (another
+// candidate's sequences, a wider table): into n chunks of its visible
+// positions, whose tiles the four warps take by turns.  A warp has a maximum,
+// a sum and outputs of its own for each chunk; those of one warp are folded
+// chunk after chunk, and the four warps' joined behind that.  How many chunks
+// a block takes is a matter of the launch:
+//   whole:   a block takes a unit (a sequence, a key head and up to 16 of its
+//            query heads), its warps fold chunk after chunk as they go;
+//   cluster: a unit's chunks are one block each of a cluster, which folds them;
+//   share:   blocks take runs of chunks, a kernel of its own folds them: equal
+//            parts of a unit's, or where there are few units runs of about as
+//            many positions, by the lengths that the device knows.
+// (The four warps joined at each chunk's end, which is less to keep, makes them
+// wait for one another: 64 sequences of 1000 to 4000 took 95 us.)
 struct PagedArgs {
     const void *q, *kp, *vp;
     const int32_t *table, *lengths;
     void* o;
-    float* part;  // share > 0: of each block m [R], l [R], then R rows of sums
+    float* part;  // share > 0: of each unit, chunk and warp, P rows of sums, then m [P], l [P]
     int64_t ldq, n_pages;
-    int page, max_pages, B, H, K, D, G, row_tiles, R;  // R: query rows of a unit (heads that share a key head)
-    // splits > 1: a unit's splits are a cluster, which joins them; share > 0:
-    // so many blocks have equal shares of all units, joined by a kernel
+    // R: query rows of a unit (heads that share a key head), P: those that there are
+    int page, max_pages, B, H, K, D, G, row_tiles, R, P;
+    // splits: the blocks of a unit (a cluster unless part is set); share > 0: so many blocks of all units instead
     int window, sinks, splits, share;
-    float scale;  // log2(e) / sqrt(D)
+    int each, most;  // chunks of a sequence: at most, and at most in this launch
+    int least;       // positions of a chunk where there are more than 8 PG_CHUNK, at least
+    float scale;     // log2(e) / sqrt(D)
 };
 
 __host__ __device__ __forceinline__ int pad4(int d) { return (d + 3) / 4 * 4; }
-__host__ __device__ __forceinline__ int64_t part_floats(int R, int D) { return 2 * (int64_t)R + (int64_t)R * pad4(D); }
+__host__ __device__ __forceinline__ int64_t part_floats(int P, int D) { return ((int64_t)P * (pad4(D) + 2) + 3) / 4 * 4; }
 
 // What the newest of `length` tokens sees: positions 0 .. s-1 and, behind a
 // gap, the last of them; vis of them in all.  vis < 0: the length is not one
@@ -133,114 +150,141 @@ __device__ __forceinline__ Seen seen_by(const PagedArgs& a, int b) {
     return Seen{w + s, s, n - w - s};
 }
 
-constexpr int PG_MIN_CHUNK = 128;  // positions of a share: less would be the pipeline's filling and the join
+constexpr int PG_CHUNK = 128;  // positions of a chunk at least: less would be the pipeline's filling and the join
 
-// The blocks' equal shares, from the sequences' lengths (at most 64 of them):
-// lane l has those of sequences 2 l and 2 l + 1.
+// Positions of a chunk of `vis`, a multiple of 64.  Above the eight chunks of
+// a cluster those of the tensor-core kernel are twice as long at least, as
+// each costs a whole unit's warps their fold: 64 sequences of 1000 to 4000 take
+// 83.7 us with 256, 88 with 128 (and 79.5 cut not at all); one of 8000 over 12
+// heads 11.8, with 512 14.9.  (float32's products take longer for the same
+// bytes: 2 sequences of 9000, 10 heads of one key head, 22 us with 128, 28 with 256.)
+__device__ __forceinline__ int chunk_of(const PagedArgs& a, int vis) {
+    const int even = (vis + a.each - 1) / a.each, least = vis <= 8 * PG_CHUNK ? PG_CHUNK : a.least;
+    return ((even < least ? least : even) + 63) / 64 * 64;
+}
+__device__ __forceinline__ int chunks_of(const PagedArgs& a, int vis) {
+    if (vis <= 0) return 0;
+    const int chunk = chunk_of(a, vis);
+    return (vis + chunk - 1) / chunk;
+}
+
+// The blocks of each unit, from the lengths of at most 64 sequences, so that
+// each has about as many positions: lane l has those of sequences 2 l and
+// 2 l + 1.
 struct Shares {
-    int chunk, splits[2], before;  // positions of a share, shares of one unit, blocks of the sequences before 2 l
+    int n[2], blocks[2], before;  // chunks and blocks of a unit; blocks of the sequences before 2 l
 };
 __device__ __forceinline__ Shares shares_of(const PagedArgs& a) {
     const int lane = threadIdx.x % 32, heads = a.K * a.row_tiles;
-    if (a.B == 1) {
-        const int v = lane == 0 ? seen_by(a, 0).vis : 0, each = a.share / heads;
-        const int even = ((v < 0 ? 0 : v) + each - 1) / each;
-        const int chunk = __shfl_sync(0xffffffffu, ((even < PG_MIN_CHUNK ? PG_MIN_CHUNK : even) + 63) / 64 * 64, 0);
-        return Shares{chunk, {v > 0 ? (v + chunk - 1) / chunk : 0, 0}, 0};
-    }
+    Shares h;
     int vis[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        vis[j] = 2 * lane + j < a.B ? seen_by(a, 2 * lane + j).vis : 0;
-        if (vis[j] < 0) vis[j] = 0;
+        const int v = 2 * lane + j < a.B ? seen_by(a, 2 * lane + j).vis : 0;
+        vis[j] = v > 0 ? v : 0;
+        h.n[j] = chunks_of(a, v);
     }
     long long total = (long long)vis[0] + vis[1];
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    // the shortest shares that there are blocks for: from those that would all
-    // be full, a quarter of the way at a time, to those that are enough even if
-    // each unit ends in a share of its own
-    auto part = [&](int blocks) {
-        const int even = (int)ceil((double)(total * heads) / blocks);  // exact below 2^53
-        return ((even < PG_MIN_CHUNK ? PG_MIN_CHUNK : even) + 63) / 64 * 64;
-    };
-    const int least = part(a.share), most = part(a.share - a.B * heads);
-    Shares h;
-    h.chunk = most;
-#pragma unroll 1
-    for (int k = 0; k < 4 && least < most; ++k) {
-        const int c = least + (most - least) / 64 * k / 4 * 64;
-        int used = heads * ((vis[0] + c - 1) / c + (vis[1] + c - 1) / c);
+    for (int f = 1; f < 32; f <<= 1) total += __shfl_xor_sync(0xffffffffu, total, f);
+    total *= heads;
+    auto used = [&](int positions) {  // blocks, if each takes so many
+        int x = 0;
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) used += __shfl_xor_sync(0xffffffffu, used, x);
-        if (used <= a.share) {
-            h.chunk = c;
-            break;
+        for (int j = 0; j < 2; ++j) {
+            const int blocks = (int)((vis[j] + (unsigned)positions - 1) / (unsigned)positions);
+            h.blocks[j] = blocks < h.n[j] ? blocks : h.n[j];
+            x += h.blocks[j];
         }
-    }
-    int n = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        h.splits[j] = (vis[j] + h.chunk - 1) / h.chunk;
-        n += heads * h.splits[j];
-    }
-    h.before = n;
+        for (int f = 1; f < 32; f <<= 1) x += __shfl_xor_sync(0xffffffffu, x, f);
+        return heads * x;
+    };
+    // the fewest positions that there are blocks for: from those if all were
+    // full, a quarter of the way at a time, to those if each unit's last is not
+    const int lo = (int)(total / a.share) + 1, hi = (int)(total / (a.share - a.B * heads)) + 1;
+#pragma unroll 1
+    for (int k = 0; k <= 4; ++k)
+        if (used(lo + (int)((long long)(hi - lo) * k / 4)) <= a.share) break;
+    const int mine = heads * (h.blocks[0] + h.blocks[1]);
+    h.before = mine;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
         const int below = __shfl_up_sync(0xffffffffu, h.before, x);
-        if ((int)threadIdx.x % 32 >= x) h.before += below;
+        if (lane >= x) h.before += below;
     }
-    h.before -= n;
+    h.before -= mine;
     return h;
 }
 
-// What this block does: positions c0 .. c0 + chunk - 1 of what row tile rt of
-// key head kh of sequence b sees.  on: it has any share.
+// What this block does: chunks c0 .. c1 - 1 of row tile rt of key head kh of
+// sequence b, its visible positions first .. end - 1; n: the sequence's chunks.
+// on: it has any part.
 struct Work {
-    int b, kh, rt, split, c0, chunk;
+    int b, kh, rt, c0, c1, n, chunk, first, end;
     bool on;
+    // (of a whole unit known without the chunks, whose two quotients are formed
+    // while the first rows are on their way)
+    __device__ __forceinline__ void positions(const PagedArgs& a, int vis, bool whole) {
+        first = 0;
+        end = vis;
+        if (whole) return;
+        chunks(a, vis, false);
+        first = c0 * chunk;
+        if (c1 < n) end = c1 * chunk;
+    }
+    __device__ __forceinline__ void chunks(const PagedArgs& a, int vis, bool whole) {
+        chunk = chunk_of(a, vis > 0 ? vis : 0);
+        n = vis > 0 ? (vis + chunk - 1) / chunk : 0;
+        if (whole) c1 = n;
+        if (c1 > n) c1 = n;
+    }
 };
-// (SHARE, a.share > 0, is an instance of its own: with both in one, 64
-// sequences took 80.1 us instead of 77.9.)
+// (SHARE, with leaves in the workspace, is an instance of its own: with both
+// in one, 64 sequences took 80.1 us instead of 77.9.)
 template <bool SHARE>
 __device__ __forceinline__ Work work_of(const PagedArgs& a) {
     Work w;
-    int unit;
+    const int heads = a.K * a.row_tiles;
+    int unit;  // of its sequence
     w.on = true;
-    if constexpr (SHARE) {
-        const int lane = threadIdx.x % 32, x = (int)blockIdx.x, heads = a.K * a.row_tiles;
+    if (SHARE && a.share > 0) {
+        const int x = (int)blockIdx.x;
         const Shares h = shares_of(a);
-        const int mine = heads * (h.splits[0] + h.splits[1]);
-        const unsigned at = __ballot_sync(0xffffffffu, x >= h.before && x < h.before + mine);
-        w.on = at != 0;
-        const int from = w.on ? __ffs(at) - 1 : 0;
+        const int mine = heads * (h.blocks[0] + h.blocks[1]);
+        const unsigned found = __ballot_sync(0xffffffffu, x >= h.before && x < h.before + mine);
+        w.on = found != 0;
+        if (!w.on) return w;
+        const int from = __ffs(found) - 1;
         int left = x - __shfl_sync(0xffffffffu, h.before, from);
-        int splits = __shfl_sync(0xffffffffu, h.splits[0], from);
-        const int second = __shfl_sync(0xffffffffu, h.splits[1], from);
+        int blocks = __shfl_sync(0xffffffffu, h.blocks[0], from), n = __shfl_sync(0xffffffffu, h.n[0], from);
+        const int blocks1 = __shfl_sync(0xffffffffu, h.blocks[1], from), n1 = __shfl_sync(0xffffffffu, h.n[1], from);
         w.b = 2 * from;
-        if (left >= heads * splits) {
-            left -= heads * splits;
-            splits = second;
+        if (left >= heads * blocks) {
+            left -= heads * blocks;
+            blocks = blocks1;
+            n = n1;
             ++w.b;
         }
-        unit = w.on ? left / splits : 0;
-        w.split = w.on ? left - unit * splits : 0;
-        w.chunk = h.chunk;
+        unit = left / blocks;
+        left -= unit * blocks;
+        w.c0 = n * left / blocks;
+        w.c1 = n * (left + 1) / blocks;
     } else {
         unit = (int)blockIdx.x / a.splits;
-        w.split = (int)blockIdx.x - unit * a.splits;
-        const int heads = a.K * a.row_tiles;
+        const int at = (int)blockIdx.x - unit * a.splits;
         w.b = unit / heads;
         unit -= w.b * heads;
-        w.chunk = 1 << 30;
-        if (a.splits > 1) {
-            const int vis = seen_by(a, w.b).vis;
-            w.chunk = (((vis < 0 ? 0 : vis) + a.splits - 1) / a.splits + 63) / 64 * 64;
+        w.c0 = at;  // the blocks of a cluster have a chunk each
+        w.c1 = at + 1;
+        if (SHARE) {
+            const int n = chunks_of(a, seen_by(a, w.b).vis);
+            w.c0 = n * at / a.splits;
+            w.c1 = n * (at + 1) / a.splits;
         }
     }
     w.kh = unit / a.row_tiles;
     w.rt = unit - w.kh * a.row_tiles;
-    w.c0 = w.split * w.chunk;
     return w;
 }
 
@@ -277,79 +321,123 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-constexpr int PG_CLUSTER = 8;  // splits that are joined in a cluster, at most
+constexpr int PG_CLUSTER = 8;  // chunks that a cluster folds, at most
 
-// Joins the warps' (m, l, sums) of one unit in shared memory, in warp order;
-// then writes the output (one split), or this split's partial, or joins the
-// splits of a cluster, in split order, each block a part of the outputs.
-// ms, ls [PG_WARPS][R] (the joined ones in the first R); os [PG_WARPS][R][pitch].
-template <typename T>
-__device__ __forceinline__ void join_warps(const PagedArgs& a, float* ms, float* ls, float* os, int pitch, int rows,
-                                           int b, int h0, int split, bool bad, bool none) {
-    float* part = a.share ? a.part + blockIdx.x * part_floats(a.R, a.D) : nullptr;
-    T* out = static_cast<T*>(a.o) + ((int64_t)b * a.H + h0) * a.D;
-    for (int i = threadIdx.x; i < rows * a.D; i += PG_WARPS * 32) {
-        const int r = i / a.D, d = i - r * a.D;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[w * a.R + r]);
-        const float base = M == -INFINITY ? 0.f : M;
-        float l = 0.f, x = 0.f;
+// One more chunk (m, l, and of a column x) onto those before (M, L, X).  The
+// same operations wherever it is done.
+struct Fold {
+    float before, next;  // factors of those before, and of the chunk
+    __device__ __forceinline__ Fold(float& M, float& L, float m, float l) {
+        const float n = fmaxf(M, m), base = n == -INFINITY ? 0.f : n;
+        before = exp2f(M - base);
+        next = exp2f(m - base);
+        L = __fmaf_rn(l, next, __fmul_rn(L, before));
+        M = n;
+    }
+    __device__ __forceinline__ float operator()(float X, float x) const { return __fmaf_rn(x, next, __fmul_rn(X, before)); }
+};
+// The four warps' (M, L) of a row: their factors and the sum.
+struct Warps {
+    float f[PG_WARPS], L;
+    __device__ __forceinline__ Warps(const float (&M)[PG_WARPS], const float (&l)[PG_WARPS]) {
+        const float m = fmaxf(fmaxf(M[0], M[1]), fmaxf(M[2], M[3])), base = m == -INFINITY ? 0.f : m;
+        L = 0.f;
 #pragma unroll
         for (int w = 0; w < PG_WARPS; ++w) {
-            const float f = exp2_fast(ms[w * a.R + r] - base);
-            l = fmaf(ls[w * a.R + r], f, l);
-            x = fmaf(os[(w * a.R + r) * pitch + d], f, x);
-        }
-        if (bad) l = __int_as_float(0x7fffffff);
-        if (a.splits > 1) {
-            os[r * pitch + d] = x;  // read by this thread alone
-        } else if (part) {
-            if (d == 0) {
-                part[r] = M;
-                part[a.R + r] = l;
-            }
-            part[2 * a.R + r * pad4(a.D) + d] = x;
-        } else {
-            out[i] = zg_from_float<T>(none ? 0.f : x / l);
+            f[w] = exp2f(M[w] - base);
+            L = __fmaf_rn(l[w], f[w], L);
         }
     }
-    if (a.splits == 1) return;
-    // the row's maximum and sum over the warps, by one warp's lanes (R <= 16)
-    __syncthreads();
-    if (threadIdx.x < a.R) {
-        const int r = threadIdx.x;
-        float M = -INFINITY, l = 0.f;
+    __device__ __forceinline__ float operator()(const float (&X)[PG_WARPS]) const {
+        float x = 0.f;
 #pragma unroll
-        for (int w = 0; w < PG_WARPS; ++w) M = fmaxf(M, ms[w * a.R + r]);
-        const float base = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < PG_WARPS; ++w) x = __fmaf_rn(X[w], f[w], x);
+        return x / L;
+    }
+};
+
+// The leaf of this warp in chunk c: where its sums go in the workspace.
+__device__ __forceinline__ float* leaf_of(const PagedArgs& a, const Work& w, int c) {
+    return a.part + ((((int64_t)w.b * a.K + w.kh) * a.row_tiles + w.rt) * a.most * PG_WARPS + c * PG_WARPS + threadIdx.x / 32) *
+                        part_floats(a.P, a.D);
+}
+
+// The outputs of a unit from its warps' (m, l, sums), or in a cluster from all
+// blocks' of them, each block a part.  ms, ls [PG_WARPS][R]; os [PG_WARPS][R]
+// [pitch]; spare: shared memory that no other block reads.
+template <typename T>
+__device__ __forceinline__ void join_warps(const PagedArgs& a, const float* ms, const float* ls, const float* os, int pitch,
+                                           float* spare, const Work& w, int rows, int h0, int vis) {
+    T* out = static_cast<T*>(a.o) + ((int64_t)w.b * a.H + h0) * a.D;
+    const float nothing = vis < 0 ? __int_as_float(0x7fffffff) : 0.f;
+    if (a.splits == 1) {
+        for (int i = threadIdx.x; i < rows * a.D; i += PG_WARPS * 32) {
+            const int r = i / a.D, d = i - r * a.D;
+            float M[PG_WARPS], L[PG_WARPS], X[PG_WARPS];
 #pragma unroll
-        for (int w = 0; w < PG_WARPS; ++w) l = fmaf(ls[w * a.R + r], exp2_fast(ms[w * a.R + r] - base), l);
-        ms[r] = M;  // read by this thread alone
-        ls[r] = bad ? __int_as_float(0x7fffffff) : l;
+            for (int x = 0; x < PG_WARPS; ++x) {
+                M[x] = ms[x * a.R + r];
+                L[x] = ls[x * a.R + r];
+                X[x] = os[(x * a.R + r) * pitch + d];
+            }
+            out[i] = zg_from_float<T>(w.n == 0 ? nothing : Warps(M, L)(X));
+        }
+        return;
     }
     cluster_sync_all();
-    for (int i = split * PG_WARPS * 32 + threadIdx.x; i < rows * a.D; i += a.splits * PG_WARPS * 32) {
+    // this thread's first output's sums, on their way while the factors are formed
+    int i = (int)blockIdx.x % a.splits * PG_WARPS * 32 + threadIdx.x;
+    float x[PG_WARPS][PG_CLUSTER];
+    auto take = [&]() {
+        if (i >= rows * a.D) return;
         const int r = i / a.D, d = i - r * a.D;
-        float m[PG_CLUSTER], l[PG_CLUSTER], x[PG_CLUSTER], M = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < PG_CLUSTER; ++s)
-            if (s < a.splits) {
-                m[s] = cluster_float(ms + r, s);
-                l[s] = cluster_float(ls + r, s);
-                x[s] = cluster_float(os + r * pitch + d, s);
-                M = fmaxf(M, m[s]);
-            }
-        const float base = M == -INFINITY ? 0.f : M;
-        float num = 0.f, den = 0.f;
+        for (int y = 0; y < PG_WARPS; ++y)
 #pragma unroll
-        for (int s = 0; s < PG_CLUSTER; ++s)
-            if (s < a.splits) {
-                const float f = exp2_fast(m[s] - base);
-                num = fmaf(x[s], f, num);
-                den = fmaf(l[s], f, den);
+            for (int c = 0; c < PG_CLUSTER; ++c)
+                if (c < w.n) x[y][c] = cluster_float(os + (y * a.R + r) * pitch + d, c);
+    };
+    take();
+    // per row and warp: the factors of each block's chunk, and the end's maximum and sum
+    float2* factor = reinterpret_cast<float2*>(spare);          // [R][PG_WARPS][PG_CLUSTER]
+    float* end = spare + 2 * a.R * PG_WARPS * PG_CLUSTER;       // [R][PG_WARPS][2]
+    if ((int)threadIdx.x < rows * PG_WARPS) {  // at most 64
+        const int at = threadIdx.x, r = at / PG_WARPS, y = at % PG_WARPS;
+        float m[PG_CLUSTER], l[PG_CLUSTER], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int c = 0; c < PG_CLUSTER; ++c)
+            if (c < w.n) {
+                m[c] = cluster_float(ms + y * a.R + r, c);
+                l[c] = cluster_float(ls + y * a.R + r, c);
             }
-        out[i] = zg_from_float<T>(none ? 0.f : num / den);
+#pragma unroll
+        for (int c = 0; c < PG_CLUSTER; ++c)
+            if (c < w.n) {
+                const Fold fold(M, L, m[c], l[c]);
+                factor[at * PG_CLUSTER + c] = make_float2(fold.before, fold.next);
+            }
+        end[2 * at] = M;
+        end[2 * at + 1] = L;
+    }
+    __syncthreads();
+    while (i < rows * a.D) {
+        const int r = i / a.D;
+        float M[PG_WARPS], L[PG_WARPS], X[PG_WARPS];
+#pragma unroll
+        for (int y = 0; y < PG_WARPS; ++y) {
+            M[y] = end[2 * (r * PG_WARPS + y)];
+            L[y] = end[2 * (r * PG_WARPS + y) + 1];
+            X[y] = 0.f;
+#pragma unroll
+            for (int c = 0; c < PG_CLUSTER; ++c)
+                if (c < w.n) {
+                    const float2 f = factor[(r * PG_WARPS + y) * PG_CLUSTER + c];
+                    X[y] = __fmaf_rn(x[y][c], f.y, __fmul_rn(X[y], f.x));
+                }
+        }
+        out[i] = zg_from_float<T>(w.n == 0 ? nothing : Warps(M, L)(X));
+        i += a.splits * PG_WARPS * 32;
+        take();
     }
     cluster_sync_all();  // no block leaves while another reads its memory
 }
@@ -371,13 +459,15 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float ms[PG_WARPS * 16], ls[PG_WARPS * 16];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Work w = work_of<SHARE>(a);
+    Work w = work_of<SHARE>(a);
     if (!w.on) return;
-    const int b = w.b, kh = w.kh, rt = w.rt, c0 = w.c0;
+    const int b = w.b, kh = w.kh, rt = w.rt;
     const int rows = a.G - rt * 16 < 16 ? a.G - rt * 16 : 16;
     const int h0 = kh * a.G + rt * 16;
     const Seen see = seen_by(a, b);
-    const int end = see.vis - c0 < w.chunk ? see.vis : c0 + w.chunk;  // this block: [c0, end)
+    const bool whole = !SHARE && a.splits == 1;
+    w.positions(a, see.vis, whole);
+    const int c0 = w.first, end = w.end;  // this block: [c0, end)
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + 15) / 16 : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -434,99 +524,157 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 
     const int k_row = (lane % 8) + 8 * (lane / 16), k_chunk = (lane / 8) % 2;
     const int v_row = (lane % 8) + 8 * ((lane / 8) % 2), v_chunk = lane / 16;
-    for (int i = 0; i < tiles; ++i) {
-        copy_wait<STAGES - 2>();
-        __syncwarp();  // every lane's copies of tile i have landed, and tile i-1 has been read
-        {
-            const Entry next = entries(i + STAGES);
-            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
-            copy_commit();
-            entry = next;
-        }
-        const uint32_t kt = shared_u32(ring + (i % STAGES) * 2 * TILE), vt = kt + TILE;
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // The chunks before this one.  With DP = 256 in shared memory: behind the
+    // ring of three stages there is room for 8 rows, behind one of two for 16.
+    constexpr int ROWS = DP == 256 && STAGES == 3 ? 8 : 16;
+    float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
+    float kept[DP == 256 ? 1 : DP / 8][4];
+    float* kept_far = reinterpret_cast<float*>(smem + PG_WARPS * STAGES * 2 * TILE) + warp * ROWS * DP + lane;
+    auto so_far = [&](int d, int e) -> float& {
+        if constexpr (DP == 256) return kept_far[(d * (ROWS / 4) + e) * 32];
+        else return kept[d][e];
+    };
+    if constexpr (!SHARE) {
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            uint32_t f[4];
-            ldmatrix4(f, kt + k_row * (DP * 2) + (((2 * k + k_chunk) ^ (k_row & 7)) * 16));
-            mma_bf16(s[0], qf[k], f[0], f[1]);
-            mma_bf16(s[1], qf[k], f[2], f[3]);
-        }
-        const int t0 = c0 + (warp + PG_WARPS * i) * 16;
-        float n0 = -INFINITY, n1 = -INFINITY;
+        for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[j][e] = t0 + j * 8 + (lane % 4) * 2 + (e & 1) < end ? s[j][e] * a.scale : -INFINITY;
-                if (e < 2) n0 = fmaxf(n0, s[j][e]);
-                else n1 = fmaxf(n1, s[j][e]);
+            for (int e = 0; e < ROWS / 4; ++e) so_far(d, e) = 0.f;
+    }
+    if (whole) w.chunks(a, see.vis, true);
+    const int per_chunk = w.chunk / (16 * PG_WARPS);  // tiles of a chunk for each warp
+    int i = 0;
+    for (int c = w.c0; c < w.c1; ++c) {
+        const int upto = (c + 1 - w.c0) * per_chunk < tiles ? (c + 1 - w.c0) * per_chunk : tiles;
+#pragma unroll 1
+        for (; i < upto; ++i) {
+            copy_wait<STAGES - 2>();
+            __syncwarp();  // every lane's copies of tile i have landed, and tile i-1 has been read
+            {
+                const Entry next = entries(i + STAGES);
+                if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
+                copy_commit();
+                entry = next;
             }
+            const uint32_t kt = shared_u32(ring + (i % STAGES) * 2 * TILE), vt = kt + TILE;
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t f[4];
+                ldmatrix4(f, kt + k_row * (DP * 2) + (((2 * k + k_chunk) ^ (k_row & 7)) * 16));
+                mma_bf16(s[0], qf[k], f[0], f[1]);
+                mma_bf16(s[1], qf[k], f[2], f[3]);
+            }
+            const int t0 = c0 + (warp + PG_WARPS * i) * 16;
+            float n0 = -INFINITY, n1 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[j][e] = t0 + j * 8 + (lane % 4) * 2 + (e & 1) < end ? __fmul_rn(s[j][e], a.scale) : -INFINITY;
+                    if (e < 2) n0 = fmaxf(n0, s[j][e]);
+                    else n1 = fmaxf(n1, s[j][e]);
+                }
+#pragma unroll
+            for (int x = 1; x < 4; x <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+            }
+            n0 = fmaxf(n0, m0);
+            n1 = fmaxf(n1, m1);
+            const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+            if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
+                const float f0 = exp2_fast(m0 - b0), f1 = exp2_fast(m1 - b1);
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int d = 0; d < DP / 8; ++d) {
+                    o[d][0] *= f0;
+                    o[d][1] *= f0;
+                    o[d][2] *= f1;
+                    o[d][3] *= f1;
+                }
+                m0 = n0;
+                m1 = n1;
+            }
+            // weights, rounded to bf16 as the second product's operand (their sum
+            // is of the unrounded ones): half a step of each weight, 2^-8
+            uint32_t p[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float p0 = exp2_fast(s[j][0] - b0), p1 = exp2_fast(s[j][1] - b0);
+                const float p2 = exp2_fast(s[j][2] - b1), p3 = exp2_fast(s[j][3] - b1);
+                l0 += p0 + p1;
+                l1 += p2 + p3;
+                p[2 * j] = pack_bf16(p0, p1);
+                p[2 * j + 1] = pack_bf16(p2, p3);
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) {
+                uint32_t f[4];
+                ldmatrix4_t(f, vt + v_row * (DP * 2) + (((2 * d + v_chunk) ^ (v_row & 7)) * 16));
+                mma_bf16(o[2 * d], p, f[0], f[1]);
+                mma_bf16(o[2 * d + 1], p, f[2], f[3]);
+            }
+        }
+        // this warp's leaf
 #pragma unroll
         for (int x = 1; x < 4; x <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+            l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
         }
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-            const float f0 = exp2_fast(m0 - b0), f1 = exp2_fast(m1 - b1);
-            l0 *= f0;
-            l1 *= f1;
+        if constexpr (SHARE) {
+            if (__any_sync(0xffffffffu, bad)) l0 = l1 = __int_as_float(0x7fffffff);
+            float* leaf = leaf_of(a, w, c);
+            const int pitch = pad4(a.D);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = lane / 4 + 8 * e;
+                if (r >= rows) continue;
+#pragma unroll
+                for (int d = 0; d < DP / 8; ++d)
+                    if (d * 8 < a.D)
+                        *reinterpret_cast<float2*>(leaf + r * pitch + d * 8 + (lane % 4) * 2) = make_float2(o[d][2 * e], o[d][2 * e + 1]);
+                if (lane % 4 == 0) {
+                    leaf[a.P * pitch + r] = e ? m1 : m0;
+                    leaf[a.P * pitch + a.P + r] = e ? l1 : l0;
+                }
+            }
+        } else {
+            const Fold f0(M[0], L[0], m0, l0), f1(M[1], L[1], m1, l1);
 #pragma unroll
             for (int d = 0; d < DP / 8; ++d) {
-                o[d][0] *= f0;
-                o[d][1] *= f0;
-                o[d][2] *= f1;
-                o[d][3] *= f1;
+#pragma unroll
+                for (int e = 0; e < ROWS / 4; ++e) {
+                    float& x = so_far(d, e);
+                    x = (e < 2 ? f0 : f1)(x, o[d][e]);
+                }
             }
-            m0 = n0;
-            m1 = n1;
-        }
-        // weights, rounded to bf16 as the second product's operand (their sum
-        // is of the unrounded ones): half a step of each weight, 2^-9
-        uint32_t p[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float p0 = exp2_fast(s[j][0] - b0), p1 = exp2_fast(s[j][1] - b0);
-            const float p2 = exp2_fast(s[j][2] - b1), p3 = exp2_fast(s[j][3] - b1);
-            l0 += p0 + p1;
-            l1 += p2 + p3;
-            p[2 * j] = pack_bf16(p0, p1);
-            p[2 * j + 1] = pack_bf16(p2, p3);
         }
 #pragma unroll
-        for (int d = 0; d < DP / 16; ++d) {
-            uint32_t f[4];
-            ldmatrix4_t(f, vt + v_row * (DP * 2) + (((2 * d + v_chunk) ^ (v_row & 7)) * 16));
-            mma_bf16(o[2 * d], p, f[0], f[1]);
-            mma_bf16(o[2 * d + 1], p, f[2], f[3]);
-        }
+        for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.f;
     }
     copy_wait<0>();
+    if constexpr (!SHARE) {
+        bad = __syncthreads_or(bad);  // the rings are free from here on
+        float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][16][DP]
+        const int r = lane / 4;
+        if (lane % 4 == 0) {
+            ms[warp * 16 + r] = M[0];
+            ms[warp * 16 + r + 8] = M[1];
+            ls[warp * 16 + r] = bad ? __int_as_float(0x7fffffff) : L[0];
+            ls[warp * 16 + r + 8] = bad ? __int_as_float(0x7fffffff) : L[1];
+        }
 #pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+        for (int d = 0; d < DP / 8; ++d) {
+            float* to = os + (warp * 16 + r) * DP + d * 8 + (lane % 4) * 2;
+            *reinterpret_cast<float2*>(to) = make_float2(so_far(d, 0), so_far(d, 1));
+            if (ROWS > 8) *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(so_far(d, 2), so_far(d, 3));
+        }
+        __syncthreads();
+        join_warps<T>(a, ms, ls, os, DP, os + PG_WARPS * 16 * DP, w, rows, h0, see.vis);
     }
-    bad = __syncthreads_or(bad || see.vis < 0);  // the rings are free from here on
-    float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][16][DP]
-    const int r = lane / 4;
-    if (lane % 4 == 0) {
-        ms[warp * 16 + r] = m0;
-        ms[warp * 16 + r + 8] = m1;
-        ls[warp * 16 + r] = l0;
-        ls[warp * 16 + r + 8] = l1;
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 8; ++d) {
-        float* to = os + (warp * 16 + r) * DP + d * 8 + (lane % 4) * 2;
-        *reinterpret_cast<float2*>(to) = make_float2(o[d][0], o[d][1]);
-        *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(o[d][2], o[d][3]);
-    }
-    __syncthreads();
-    join_warps<T>(a, ms, ls, os, DP, rows, b, h0, w.split, bad, see.vis == 0);
 }
 
 // Any type, width and alignment, in float32 on the FMA pipe.  A warp's tile
@@ -544,13 +692,15 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
     __shared__ float ms[PG_WARPS * GT], ls[PG_WARPS * GT];
     __shared__ __align__(16) float qs[GT][36 * PARTS];  // parts of 32 columns, 4 banks apart
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Work w = work_of<SHARE>(a);
+    Work w = work_of<SHARE>(a);
     if (!w.on) return;
-    const int b = w.b, kh = w.kh, rt = w.rt, c0 = w.c0;
+    const int b = w.b, kh = w.kh, rt = w.rt;
     const int rows = a.G - rt * GT < GT ? a.G - rt * GT : GT;
     const int h0 = kh * a.G + rt * GT;
     const Seen see = seen_by(a, b);
-    const int end = see.vis - c0 < w.chunk ? see.vis : c0 + w.chunk;
+    const bool whole = !SHARE && a.splits == 1;
+    w.positions(a, see.vis, whole);
+    const int c0 = w.first, end = w.end;
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + TT - 1) / TT : 0;
     const int tiles = tiles_all > warp ? (tiles_all - warp + PG_WARPS - 1) / PG_WARPS : 0;
@@ -615,156 +765,219 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
         for (int i = 0; i < NI; ++i) o[g][i] = 0.f;
     }
     const int tok = lane % TT, part = lane / TT;
-    for (int i = 0; i < tiles; ++i) {
-        copy_wait<STAGES - 2>();
-        __syncwarp();
-        {
-            const Entry next = entries(i + STAGES);
-            if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
-            copy_commit();
-            entry = next;
-        }
-        const uint8_t* kt = ring + (i % STAGES) * 2 * TILE;
-        const uint8_t* vt = kt + TILE;
-        float s[GT];
+    float kept[GT][NI], M[GT], L[GT];  // the chunks before this one
 #pragma unroll
-        for (int g = 0; g < GT; ++g) s[g] = 0.f;
-        const T* kr = reinterpret_cast<const T*>(kt + tok * PITCH) + part * 32;
+    for (int g = 0; g < GT; ++g) {
+        M[g] = -INFINITY;
+        L[g] = 0.f;
 #pragma unroll
-        for (int d = 0; d < 32; d += 4) {
-            float kv[4];
-            if constexpr (sizeof(T) == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(kr + d);
-                kv[0] = x.x; kv[1] = x.y; kv[2] = x.z; kv[3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(kr + d);
-                kv[0] = __uint_as_float(x.x << 16); kv[1] = __uint_as_float(x.x & 0xffff0000u);
-                kv[2] = __uint_as_float(x.y << 16); kv[3] = __uint_as_float(x.y & 0xffff0000u);
+        for (int x = 0; x < NI; ++x) kept[g][x] = 0.f;
+    }
+    if (whole) w.chunks(a, see.vis, true);
+    const int per_chunk = w.chunk / (TT * PG_WARPS);
+    int i = 0;
+    for (int c = w.c0; c < w.c1; ++c) {
+        const int upto = (c + 1 - w.c0) * per_chunk < tiles ? (c + 1 - w.c0) * per_chunk : tiles;
+#pragma unroll 1
+        for (; i < upto; ++i) {
+            copy_wait<STAGES - 2>();
+            __syncwarp();
+            {
+                const Entry next = entries(i + STAGES);
+                if (i + STAGES - 1 < tiles) fetch((i + STAGES - 1) % STAGES, place_of(a, entry, bad));
+                copy_commit();
+                entry = next;
             }
+            const uint8_t* kt = ring + (i % STAGES) * 2 * TILE;
+            const uint8_t* vt = kt + TILE;
+            float s[GT];
+#pragma unroll
+            for (int g = 0; g < GT; ++g) s[g] = 0.f;
+            const T* kr = reinterpret_cast<const T*>(kt + tok * PITCH) + part * 32;
+#pragma unroll
+            for (int d = 0; d < 32; d += 4) {
+                float kv[4];
+                if constexpr (sizeof(T) == 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(kr + d);
+                    kv[0] = x.x; kv[1] = x.y; kv[2] = x.z; kv[3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(kr + d);
+                    kv[0] = __uint_as_float(x.x << 16); kv[1] = __uint_as_float(x.x & 0xffff0000u);
+                    kv[2] = __uint_as_float(x.y << 16); kv[3] = __uint_as_float(x.y & 0xffff0000u);
+                }
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const float4 x = *reinterpret_cast<const float4*>(&qs[g][part * 36 + d]);
+                    s[g] = fmaf(kv[0], x.x, fmaf(kv[1], x.y, fmaf(kv[2], x.z, fmaf(kv[3], x.w, s[g]))));
+                }
+            }
+            const bool on = c0 + (warp + PG_WARPS * i) * TT + tok < end;
 #pragma unroll
             for (int g = 0; g < GT; ++g) {
-                const float4 x = *reinterpret_cast<const float4*>(&qs[g][part * 36 + d]);
-                s[g] = fmaf(kv[0], x.x, fmaf(kv[1], x.y, fmaf(kv[2], x.z, fmaf(kv[3], x.w, s[g]))));
+#pragma unroll
+                for (int x = TT; x < 32; x <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], x);
+                s[g] = on ? s[g] : -INFINITY;
+                float n = s[g];
+#pragma unroll
+                for (int x = 1; x < TT; x <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
+                n = fmaxf(n, m[g]);
+                const float base = n == -INFINITY ? 0.f : n;
+                const float f = exp2f(m[g] - base);
+                m[g] = n;
+                s[g] = exp2f(s[g] - base);
+                l[g] = fmaf(l[g], f, part == 0 ? s[g] : 0.f);
+#pragma unroll
+                for (int c = 0; c < NI; ++c) o[g][c] *= f;
+            }
+#pragma unroll 4
+            for (int t = 0; t < TT; ++t) {
+                float v[NI];
+                const T* vr = reinterpret_cast<const T*>(vt + t * PITCH);
+#pragma unroll
+                for (int c = 0; c < NI; ++c) v[c] = zg_to_float(vr[lane + 32 * c]);
+#pragma unroll
+                for (int g = 0; g < GT; ++g) {
+                    const float p = __shfl_sync(0xffffffffu, s[g], t);
+#pragma unroll
+                    for (int c = 0; c < NI; ++c) o[g][c] = fmaf(p, v[c], o[g][c]);
+                }
             }
         }
-        const bool on = c0 + (warp + PG_WARPS * i) * TT + tok < end;
+        // this warp's leaf
+#pragma unroll
+        for (int g = 0; g < GT; ++g)
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], x);
+        if constexpr (SHARE) {
+            const bool spoilt = __any_sync(0xffffffffu, bad);
+            float* leaf = leaf_of(a, w, c);
+            const int pitch = pad4(a.D);
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                if (g >= rows) continue;
+#pragma unroll
+                for (int x = 0; x < NI; ++x)
+                    if (lane + 32 * x < pitch) leaf[g * pitch + lane + 32 * x] = o[g][x];
+                if (lane == 0) {
+                    leaf[a.P * pitch + g] = m[g];
+                    leaf[a.P * pitch + a.P + g] = spoilt ? __int_as_float(0x7fffffff) : l[g];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                const Fold fold(M[g], L[g], m[g], l[g]);
+#pragma unroll
+                for (int x = 0; x < NI; ++x) kept[g][x] = fold(kept[g][x], o[g][x]);
+            }
+        }
 #pragma unroll
         for (int g = 0; g < GT; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.f;
 #pragma unroll
-            for (int x = TT; x < 32; x <<= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], x);
-            s[g] = on ? s[g] : -INFINITY;
-            float n = s[g];
-#pragma unroll
-            for (int x = 1; x < TT; x <<= 1) n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
-            n = fmaxf(n, m[g]);
-            const float base = n == -INFINITY ? 0.f : n;
-            const float f = exp2f(m[g] - base);
-            m[g] = n;
-            s[g] = exp2f(s[g] - base);
-            l[g] = fmaf(l[g], f, part == 0 ? s[g] : 0.f);
-#pragma unroll
-            for (int c = 0; c < NI; ++c) o[g][c] *= f;
-        }
-#pragma unroll 4
-        for (int t = 0; t < TT; ++t) {
-            float v[NI];
-            const T* vr = reinterpret_cast<const T*>(vt + t * PITCH);
-#pragma unroll
-            for (int c = 0; c < NI; ++c) v[c] = zg_to_float(vr[lane + 32 * c]);
-#pragma unroll
-            for (int g = 0; g < GT; ++g) {
-                const float p = __shfl_sync(0xffffffffu, s[g], t);
-#pragma unroll
-                for (int c = 0; c < NI; ++c) o[g][c] = fmaf(p, v[c], o[g][c]);
-            }
+            for (int x = 0; x < NI; ++x) o[g][x] = 0.f;
         }
     }
     copy_wait<0>();
-    bad = __syncthreads_or(bad || see.vis < 0);
-    float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][GT][DMAX]
+    if constexpr (!SHARE) {
+        bad = __syncthreads_or(bad);
+        float* os = reinterpret_cast<float*>(smem);  // [PG_WARPS][GT][DMAX]
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
+        for (int g = 0; g < GT; ++g) {
+            if (lane == 0) {
+                ms[warp * GT + g] = M[g];
+                ls[warp * GT + g] = bad ? __int_as_float(0x7fffffff) : L[g];
+            }
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], x);
-        if (lane == 0) {
-            ms[warp * GT + g] = m[g];
-            ls[warp * GT + g] = l[g];
+            for (int x = 0; x < NI; ++x) os[(warp * GT + g) * DMAX + lane + 32 * x] = kept[g][x];
         }
-#pragma unroll
-        for (int c = 0; c < NI; ++c) os[(warp * GT + g) * DMAX + lane + 32 * c] = o[g][c];
+        __syncthreads();
+        join_warps<T>(a, ms, ls, os, DMAX, os + PG_WARPS * GT * DMAX, w, rows, h0, see.vis);
     }
-    __syncthreads();
-    join_warps<T>(a, ms, ls, os, DMAX, rows, b, h0, w.split, bad, see.vis == 0);
 }
 
-// Joins the splits of one query head: a block per (b, h), its warps over the
-// splits, summed in warp order.  It is launched so that its blocks start as
-// the splits' last one ends.  (With its blocks waiting in their places while
-// the splits run, one sequence of 131000 takes 54.3 us instead of 51.6.)
+// Folds the chunks of one query head in their order, each warp's apart, and
+// joins those: a block per (b, h) and 32 columns, a warp for each warp of the
+// chunks' blocks, a lane a column.  The factors come of the maxima alone; they
+// are formed first, while the first sums are on their way.  It is launched so
+// that its blocks start as the last chunk's block ends.  (With its blocks
+// waiting in their places meanwhile, one sequence of 131000 took 54.3 us
+// instead of 51.6.)
+constexpr int PJ_MOST = 448, PJ_AHEAD = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
-    __shared__ float4 sums[8][64];
-    __shared__ float sum_l[8];
+__global__ void __launch_bounds__(PG_WARPS * 32) paged_join_kernel(const PagedArgs a) {
+    __shared__ float2 factor[PG_WARPS][PJ_MOST];
+    __shared__ float ls[PG_WARPS][PJ_MOST], Xs[PG_WARPS][32], Ms[PG_WARPS], Ls[PG_WARPS];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H);
+    const int b = (int)(blockIdx.x / a.H), h = (int)(blockIdx.x % a.H), d = (int)blockIdx.y * 32 + lane;
     const int kh = h / a.G, rt = h % a.G / a.R, r = h % a.G % a.R;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched before the splits' kernel has ended
-    const int vis = seen_by(a, b).vis;
-    const Shares shares = shares_of(a);
-    const int even = __shfl_sync(0xffffffffu, shares.splits[0], b / 2), odd = __shfl_sync(0xffffffffu, shares.splits[1], b / 2);
-    const int n = b % 2 ? odd : even;  // shares of this unit, from block `first`
-    const int first = __shfl_sync(0xffffffffu, shares.before, b / 2) + (b % 2 ? a.K * a.row_tiles * even : 0) +
-                      (kh * a.row_tiles + rt) * n;
-    const int64_t pf = part_floats(a.R, a.D);
-    const float* part = a.part + first * pf;
-    const int words = pad4(a.D) / 4;
-    float M = -INFINITY;
-    for (int s = lane; s < n; s += 32) M = fmaxf(M, part[s * pf + r]);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched before the chunks' kernel has ended
+    const int vis = seen_by(a, b).vis, n = chunks_of(a, vis);
+    const int64_t pf = part_floats(a.P, a.D), step = PG_WARPS * pf;
+    const int pitch = pad4(a.D);
+    const float* part = a.part + ((((int64_t)b * a.K + kh) * a.row_tiles + rt) * a.most * PG_WARPS + warp) * pf;
+    const float* column = part + r * pitch + (d < pitch ? d : 0);
+    float x[PJ_AHEAD];
+    auto load = [&](int c0) {
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-    const float base = M == -INFINITY ? 0.f : M;
-    float l = 0.f;
-    float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 4
-    for (int s = warp; s < n; s += 8) {
-        const float* p = part + s * pf;
-        const float f = exp2f(p[r] - base);
-        l = fmaf(p[a.R + r], f, l);
-        const float* row = p + 2 * a.R + r * (words * 4);
+        for (int e = 0; e < PJ_AHEAD; ++e)
+            if (c0 + e < n) x[e] = column[(c0 + e) * step];
+    };
+    load(0);
+    float M = -INFINITY;  // of the chunks before these 32
+    for (int c0 = 0; c0 < n; c0 += 32) {
+        const float* ml = part + (c0 + lane) * step + a.P * pitch;
+        const bool on = c0 + lane < n;
+        const float m = on ? ml[r] : -INFINITY;
+        if (on) ls[warp][c0 + lane] = ml[a.P + r];
+        float top = m;  // of these up to this lane's
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            if (lane + 32 * j < words) {
-                // rows start on 8-byte boundaries at least (2 R floats, R even, or R = 1)
-                const float2 u = *reinterpret_cast<const float2*>(row + 4 * (lane + 32 * j));
-                const float2 w = *reinterpret_cast<const float2*>(row + 4 * (lane + 32 * j) + 2);
-                x[j].x = fmaf(u.x, f, x[j].x);
-                x[j].y = fmaf(u.y, f, x[j].y);
-                x[j].z = fmaf(w.x, f, x[j].z);
-                x[j].w = fmaf(w.y, f, x[j].w);
+        for (int f = 1; f < 32; f <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, top, f);
+            if (lane >= f) top = fmaxf(top, y);
+        }
+        const float above = __shfl_up_sync(0xffffffffu, top, 1);
+        float before = lane ? fmaxf(M, above) : M, sum = 0.f;
+        const Fold fold(before, sum, m, 0.f);
+        if (on) factor[warp][c0 + lane] = make_float2(fold.before, fold.next);
+        M = fmaxf(M, __shfl_sync(0xffffffffu, top, 31));
+    }
+    __syncwarp();
+    float X = 0.f, L = 0.f;
+    for (int c0 = 0; c0 < n; c0 += PJ_AHEAD) {
+#pragma unroll
+        for (int e = 0; e < PJ_AHEAD; ++e)
+            if (c0 + e < n) {
+                const float2 f = factor[warp][c0 + e];
+                X = __fmaf_rn(x[e], f.y, __fmul_rn(X, f.x));
+                L = __fmaf_rn(ls[warp][c0 + e], f.y, __fmul_rn(L, f.x));
             }
+        if (c0 + PJ_AHEAD < n) load(c0 + PJ_AHEAD);
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (lane + 32 * j < words) sums[warp][lane + 32 * j] = x[j];
-    if (lane == 0) sum_l[warp] = l;
+    Xs[warp][lane] = X;
+    if (lane == 0) {
+        Ms[warp] = M;
+        Ls[warp] = L;
+    }
     __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= a.D) return;
-    float num = 0.f, den = 0.f;
+    if (warp || d >= a.D) return;
+    float Mw[PG_WARPS], Lw[PG_WARPS], Xw[PG_WARPS];
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        num += reinterpret_cast<const float*>(sums[w])[d];
-        den += sum_l[w];
+    for (int w = 0; w < PG_WARPS; ++w) {
+        Mw[w] = Ms[w];
+        Lw[w] = Ls[w];
+        Xw[w] = Xs[w][lane];
     }
-    const float out = vis < 0 ? __int_as_float(0x7fffffff) : vis == 0 ? 0.f : num / den;
+    const float out = vis < 0 ? __int_as_float(0x7fffffff) : n == 0 ? 0.f : Warps(Mw, Lw)(Xw);
     static_cast<T*>(a.o)[((int64_t)b * a.H + h) * a.D + d] = zg_from_float<T>(out);
 }
 
-// How a call is cut: R query rows of a unit, the units' splits, or the blocks
-// that share them.
+// How a call is cut: R query rows of a unit, the chunks of a sequence, and
+// what the blocks are.
 struct PagedPlan {
-    int R, row_tiles, splits, share;
-    bool mma;
+    int R, row_tiles, P, each, most, splits, share;
+    bool mma, leaves;  // leaves: in the workspace
 };
 
 PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window, int sinks, int dtype) {
@@ -773,30 +986,49 @@ PagedPlan paged_plan(int64_t B, int H, int K, int D, int64_t longest, int window
     p.mma = dtype == ZG_BF16 && D % 8 == 0;
     p.R = p.mma ? 16 : G == 1 ? 1 : G <= 4 ? 4 : 8;
     p.row_tiles = (G + p.R - 1) / p.R;
+    p.P = G < p.R ? G : p.R;
     int64_t vis = longest;
     if (window > 0 && (int64_t)window + sinks < vis) vis = (int64_t)window + sinks;
-    const int64_t units = B * K * p.row_tiles, blocks = (p.mma ? 2 : 3) * 148;
-    // Two blocks run on each of 148 SMs (three of the FMA path): as many splits
-    // as fill them once.  (Four times as many, so that a batch of 64 sequences
-    // of different lengths evens out, was 126 us instead of 81: a block costs
-    // its pipeline's filling and its part in the join.)  Up to PG_CLUSTER
-    // splits are a cluster of two, four or eight blocks, which joins them by
-    // itself and whose blocks have equal parts of what its unit sees.  Units
-    // that would be cut further are shared out to all blocks by the lengths
-    // that the device knows, and a kernel of its own joins them.  (Split by the
-    // table's width instead, a sequence of 8000 in a table of 131072 took 42
-    // us, now 12.2; 8 of 1000 in a table of 16384 26 us, now 11.2.)
-    int64_t splits = (blocks + units - 1) / units;
-    if (splits > (vis + PG_MIN_CHUNK - 1) / PG_MIN_CHUNK) splits = (vis + PG_MIN_CHUNK - 1) / PG_MIN_CHUNK;
+    // Blocks that run on an SM at once, by the instances' shared memory and
+    // registers: of the tensor cores' two, above 128 columns (192 KB) one; of
+    // the FMA path three, above 128 columns (up to 255 registers) two.
+    const int per_sm = p.mma ? (D <= 128 ? 2 : 1) : D <= 128 ? 3 : 2;
+    // A sequence alone fills the places of a whole chip once (148 SMs: a
+    // constant, as the cut is part of the result).
+    const int heads = K * p.row_tiles;
+    p.each = per_sm * 148 / heads > 1 ? per_sm * 148 / heads : 1;
+    const int64_t fill = (vis + PG_CHUNK - 1) / PG_CHUNK;
+    p.most = (int)(fill < p.each ? (fill > 0 ? fill : 1) : p.each);
+    // Units that fill most places are not cut further, nor short ones that fill
+    // half of them (32 sequences of up to 1000, 32 heads of 8 key heads: 27.3
+    // us, 41.6 with leaves in the workspace).  A block of its own for each chunk
+    // costs its pipeline's filling: 64 sequences of different lengths cut four
+    // times as often were 126 us.  Below that a cluster of up to eight chunks
+    // joins them by itself.  Otherwise the leaves go through the workspace: with
+    // two, four or eight equal parts of a unit (16 sequences of up to 8000, 8 key
+    // heads: 71.6 us, by the lengths 76.7), or where that would not fill the
+    // places, shared out by the lengths that the device knows (by the table's
+    // width a sequence of 8000 in a table of 131072 took 42 us, now 11.9).
+    const int64_t units = B * heads, places = (int64_t)per_sm * zg::sm_count();
     p.splits = 1;
-    if (splits > PG_CLUSTER)
-        p.share = (int)blocks;  // more than twice the units, of which there are less than 64
-    else if (splits > 1)
-        p.splits = splits <= 2 ? 2 : splits <= 4 ? 4 : 8;
+    if (5 * units >= 4 * places || (2 * units >= places && p.most <= 8) || p.most == 1) return p;
+    const int blocks = p.most <= 2 ? 2 : p.most <= 4 ? 4 : 8;
+    const int64_t parts = (places + units - 1) / units;
+    if (p.most <= PG_CLUSTER && units * blocks <= 2 * places) {
+        p.splits = blocks;
+    } else {
+        p.leaves = true;
+        if (parts <= 8)
+            p.splits = parts <= 2 ? 2 : parts <= 4 ? 4 : 8;
+        else
+            p.share = (int)places;  // more than eight times the units, of which there are less than 64
+    }
     return p;
 }
 
-size_t paged_workspace(const PagedPlan& p, int D) { return (size_t)(p.share * part_floats(p.R, D)) * sizeof(float); }
+size_t paged_workspace(const PagedPlan& p, int64_t B, int K, int D) {
+    return p.leaves ? (size_t)(B * K * p.row_tiles * p.most * PG_WARPS * part_floats(p.P, D)) * sizeof(float) : 0;
+}
 
 bool paged_sizes_ok(int64_t n_pages, int page, int64_t B, int H, int K, int D, int max_pages) {
     return n_pages >= 0 && page >= 1 && B >= 0 && H >= 1 && K >= 1 && D >= 1 && max_pages >= 0 && H % K == 0 &&
@@ -822,7 +1054,7 @@ int launch_split(void (*f)(P...), const PagedArgs& a, int64_t blocks, size_t sme
     at.val.clusterDim.x = (unsigned)a.splits;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     c.attrs = &at;
-    c.numAttrs = a.splits > 1 ? 1 : 0;
+    c.numAttrs = a.splits > 1 && !a.part ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&c, f, args...);
     if (e != cudaSuccess) return zg::fail(ZG_ERR_CUDA, "zg_paged_attention: %s", cudaGetErrorString(e));
     return zg::check_launch("zg_paged_attention");
@@ -830,8 +1062,9 @@ int launch_split(void (*f)(P...), const PagedArgs& a, int64_t blocks, size_t sme
 
 template <int DP, int STAGES>
 int launch_mma(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
-    const size_t smem = (size_t)PG_WARPS * STAGES * 2 * 16 * DP * 2;
-    const auto f = a.share ? paged_mma_kernel<DP, STAGES, true> : paged_mma_kernel<DP, STAGES, false>;
+    const size_t smem = (size_t)PG_WARPS * STAGES * 2 * 16 * DP * 2  +
+                        (DP == 256 && !a.part ? PG_WARPS * (STAGES == 3 ? 8 : 16) * DP * sizeof(float) : 0);
+    const auto f = a.part ? paged_mma_kernel<DP, STAGES, true> : paged_mma_kernel<DP, STAGES, false>;
     if (int rc = set_smem(f, smem)) return rc;
     zg::LaunchTimer zg_lt_("paged_attention", st);
     return launch_split(f, a, blocks, smem, st, a);
@@ -840,9 +1073,10 @@ int launch_mma(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
 template <typename T, int PARTS, int GT>
 int launch_fma(const PagedArgs& a, int vec, int64_t blocks, cudaStream_t st) {
     const size_t ring = (size_t)PG_WARPS * PG_FMA_STAGES * 2 * (32 / PARTS) * (32 * PARTS * sizeof(T) + 16);
-    const size_t out = (size_t)PG_WARPS * GT * 32 * PARTS * sizeof(float);
+    // behind the end's sums there is room for a cluster's factors
+    const size_t out = (size_t)PG_WARPS * GT * (32 * PARTS + 2 * PG_CLUSTER + 2) * sizeof(float);
     const size_t smem = ring > out ? ring : out;
-    const auto f = a.share ? paged_fma_kernel<T, PARTS, GT, true> : paged_fma_kernel<T, PARTS, GT, false>;
+    const auto f = a.part ? paged_fma_kernel<T, PARTS, GT, true> : paged_fma_kernel<T, PARTS, GT, false>;
     if (int rc = set_smem(f, smem)) return rc;
     zg::LaunchTimer zg_lt_("paged_attention_fma", st);
     return launch_split(f, a, blocks, smem, st, a, vec);
@@ -905,7 +1139,7 @@ extern "C" size_t zg_paged_attention_workspace_size(int64_t B, int H, int K, int
     if (!paged_sizes_ok(0, page, B, H, K, D, max_pages) || B == 0 || D > 256 || window < 0 || sinks < 0 ||
         !zg::dtype_ok(dtype))
         return 0;
-    return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), D);
+    return paged_workspace(paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype), B, K, D);
 }
 
 extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_pages, const void* v_pages,
@@ -924,21 +1158,22 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
     if (!q || !lengths || !o || (max_pages && !table) || (n_pages && (!k_pages || !v_pages)))
         return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: null pointer");
     PagedPlan p = paged_plan(B, H, K, D, (int64_t)max_pages * page, window, sinks, dtype);
-    const size_t need = paged_workspace(p, D);
+    const size_t need = paged_workspace(p, B, K, D);
     if (need && (!workspace || workspace_bytes < need))
         return zg::fail(ZG_ERR_WORKSPACE, "zg_paged_attention: workspace of %zu bytes needed", need);
     const int64_t blocks = p.share ? p.share : B * K * p.row_tiles * p.splits;
     if (blocks > INT32_MAX) return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: too many rows");
     const int n = 16 / (int)zg::dtype_size(dtype);
     const int vec = D % n == 0 && aligned16(k_pages) && aligned16(v_pages);
-    PagedArgs a{q, k_pages, v_pages, table, lengths, o, static_cast<float*>(workspace), ldq, n_pages, page, max_pages,
-                (int)B, H, K, D, H / K, p.row_tiles, p.R, window, sinks, p.splits, p.share,
+    PagedArgs a{q, k_pages, v_pages, table, lengths, o, p.leaves ? static_cast<float*>(workspace) : nullptr, ldq, n_pages, page, max_pages,
+                (int)B, H, K, D, H / K, p.row_tiles, p.R, p.P, window, sinks, p.splits, p.share, p.each, p.most, p.mma ? 2 * PG_CHUNK : PG_CHUNK,
                 (float)(1.4426950408889634 / sqrt((double)D))};
     cudaStream_t st = zg::as_stream(stream);
     int rc;
     if (p.mma && vec && ldq % 2 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0) {
         rc = D <= 64 ? launch_mma<64, 4>(a, blocks, st)
-             : D <= 128 ? launch_mma<128, 3>(a, blocks, st) : launch_mma<256, 3>(a, blocks, st);
+             : D <= 128 ? launch_mma<128, 3>(a, blocks, st)
+             : p.P <= 8 || p.leaves ? launch_mma<256, 3>(a, blocks, st) : launch_mma<256, 2>(a, blocks, st);
     } else if (p.mma) {
         return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: bf16 pages with D a multiple of 8 must be 16-byte "
                                         "aligned, q 4-byte aligned with an even pitch");
@@ -946,11 +1181,11 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
         rc = dtype == ZG_BF16 ? launch_fma_any<__nv_bfloat16>(a, vec, blocks, st)
                               : launch_fma_any<float>(a, vec, blocks, st);
     }
-    if (rc != ZG_OK || !p.share) return rc;
+    if (rc != ZG_OK || !p.leaves) return rc;
     zg::LaunchTimer zg_lt_("paged_join", st);
     cudaLaunchConfig_t c{};
-    c.gridDim = dim3((unsigned)(B * H));
-    c.blockDim = dim3(256);
+    c.gridDim = dim3((unsigned)(B * H), (unsigned)((D + 31) / 32));
+    c.blockDim = dim3(PG_WARPS * 32);
     c.stream = st;
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;

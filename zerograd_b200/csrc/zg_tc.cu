@@ -973,6 +973,8 @@ int launch_tc_pair(const CUtensorMap& ta, const CUtensorMap& tb, const TcArgs& a
 
 namespace zg {
 
+int sm_count() { return num_sms(); }
+
 bool tc_available() {
     static int ok = -1;
     if (ok < 0) {

@@ -220,3 +220,16 @@ def test_paged_attention_under_vmap_over_long_caches(cuda, dtype, D, longest):
     got = torch.func.vmap(lambda qq, tt, nn: zg.paged_attention(qq, kp, vp, tt, nn))(q, table, n)
     for p in range(P):
         assert torch.equal(zg.paged_attention(q[p], kp, vp, table[p], n[p]), got[p])
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 256), (BF, 20), (F32, 64), (F32, 200)])
+def test_paged_attention_of_values_near_the_largest(cuda, dtype, D):
+    """Sums of finite values do not overflow on the way to an average of them."""
+    lengths = [700, 3, 4000]
+    kp, vp, table = _cache(lengths, 16, 2, D, dtype, cuda)
+    vp = (2.5e38 * (1 + 0.1 * vp.float().sigmoid())).to(dtype) * torch.tensor([1, -1], device=cuda, dtype=dtype)[:, None]
+    q, n = _rand((3, 4, D), dtype, 6, cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    for window in (None, 90):
+        o = zg.paged_attention(q, kp, vp, table, n, window, 2)
+        want, mag = so.paged_attention(q.cpu(), kp.cpu(), vp.cpu(), table.cpu(), n.cpu(), window, 2)
+        so.assert_within(o, want, so.attention_tolerance(q.cpu(), kp.cpu(), want, mag, dtype, 4000))

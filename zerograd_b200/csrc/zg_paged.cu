@@ -217,6 +217,10 @@ __device__ __forceinline__ Shares shares_of(const PagedArgs& a) {
     return h;
 }
 
+// Weights are taken 2^-lift times smaller, so that no sum of `vis` finite
+// values overflows on its way (the quotient is the same).
+__device__ __forceinline__ int lift_of(int vis) { return 33 - __clz(vis > 0 ? vis : 1); }
+
 // What this block does: chunks c0 .. c1 - 1 of row tile rt of key head kh of
 // sequence b, its visible positions first .. end - 1; n: the sequence's chunks.
 // on: it has any part.
@@ -467,6 +471,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     const Seen see = seen_by(a, b);
     const bool whole = !SHARE && a.splits == 1;
     w.positions(a, see.vis, whole);
+    const float lift = (float)lift_of(see.vis);
     const int c0 = w.first, end = w.end;  // this block: [c0, end)
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + 15) / 16 : 0;
@@ -582,6 +587,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
             n0 = fmaxf(n0, m0);
             n1 = fmaxf(n1, m1);
             const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
+            const float b0l = b0 + lift, b1l = b1 + lift;
             if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
                 const float f0 = exp2_fast(m0 - b0), f1 = exp2_fast(m1 - b1);
                 l0 *= f0;
@@ -601,8 +607,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
             uint32_t p[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float p0 = exp2_fast(s[j][0] - b0), p1 = exp2_fast(s[j][1] - b0);
-                const float p2 = exp2_fast(s[j][2] - b1), p3 = exp2_fast(s[j][3] - b1);
+                const float p0 = exp2_fast(s[j][0] - b0l), p1 = exp2_fast(s[j][1] - b0l);
+                const float p2 = exp2_fast(s[j][2] - b1l), p3 = exp2_fast(s[j][3] - b1l);
                 l0 += p0 + p1;
                 l1 += p2 + p3;
                 p[2 * j] = pack_bf16(p0, p1);
@@ -700,6 +706,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
     const Seen see = seen_by(a, b);
     const bool whole = !SHARE && a.splits == 1;
     w.positions(a, see.vis, whole);
+    const float low = ldexpf(1.f, -lift_of(see.vis));
     const int c0 = w.first, end = w.end;
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
     const int tiles_all = end > c0 ? (end - c0 + TT - 1) / TT : 0;
@@ -824,7 +831,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_fma_kernel(const PagedArg
                 const float base = n == -INFINITY ? 0.f : n;
                 const float f = exp2f(m[g] - base);
                 m[g] = n;
-                s[g] = exp2f(s[g] - base);
+                s[g] = exp2f(s[g] - base) * low;
                 l[g] = fmaf(l[g], f, part == 0 ? s[g] : 0.f);
 #pragma unroll
                 for (int c = 0; c < NI; ++c) o[g][c] *= f;

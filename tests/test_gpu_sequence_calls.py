@@ -233,3 +233,100 @@ def test_paged_attention_of_values_near_the_largest(cuda, dtype, D):
         o = zg.paged_attention(q, kp, vp, table, n, window, 2)
         want, mag = so.paged_attention(q.cpu(), kp.cpu(), vp.cpu(), table.cpu(), n.cpu(), window, 2)
         so.assert_within(o, want, so.attention_tolerance(q.cpu(), kp.cpu(), want, mag, dtype, 4000))
+
+
+# ------------------------------------------------ the form that shares work out, with its workspace and second kernel
+
+
+SHARED = [
+    # dtype, H, K, D, lengths: few units, tables above 1024 positions
+    (BF, 4, 2, 64, [3000, 40, 5000]), (BF, 8, 1, 128, [20000]), (F32, 4, 2, 64, [9000, 1, 2500]), (BF, 6, 2, 192, [0, 6000]),
+    (BF, 16, 2, 64, [1100] * 30),  # equal parts of a unit
+]
+
+
+def _sharing_step(cuda, dtype, H, K, D, lengths, seed=1):
+    """The newest tokens written and attended, in new tensors: the inputs and the call."""
+    kp, vp, table = _cache([n + 1 for n in lengths], 16, K, D, dtype, cuda, seed)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    x = _rand((len(lengths), 1, H + 2 * K, D), dtype, seed + 9, cuda)
+
+    def run():
+        m = zg.append_pages(kp, vp, x[:, :, H:H + K], x[:, :, H + K:], table, n)
+        return zg.paged_attention(x[:, 0, :H], kp, vp, table, m)
+
+    return x, run, (kp, vp, table, n + 1)
+
+
+def _workspace_of(x, K, table, D, dtype, H):
+    B, M = table.shape
+    return L.load().zg_paged_attention_workspace_size(B, H, K, D, M, 16, 0, 0, L.dtype_code(dtype))
+
+
+@pytest.mark.parametrize("dtype,H,K,D,lengths", SHARED)
+def test_sharing_form_captured_and_replayed(cuda, dtype, H, K, D, lengths):
+    """Two calls' graphs, replayed in turn and on two streams at once on new
+    values, give the bits of the eager calls, which hold against the oracle."""
+    steps = [_sharing_step(cuda, dtype, H, K, D, lengths, seed) for seed in (1, 5)]
+    graphs = []
+    for x, run, (_, _, table, _) in steps:
+        assert _workspace_of(x, K, table, D, dtype, H) > 0
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for seed in (2, 3):
+        want = []
+        for i, (x, run, (kp, vp, table, n)) in enumerate(steps):
+            x.copy_(_rand(x.shape, F32, 10 * i + seed, cuda))
+            want.append(run().clone())
+            full, mag = so.paged_attention(x[:, 0, :H].cpu(), kp.cpu(), vp.cpu(), table.cpu(), n.cpu())
+            so.assert_within(want[i], full, so.attention_tolerance(x.cpu(), kp.cpu(), full, mag, dtype, max(lengths)))
+        for at_once in (False, True):
+            for _, out in graphs:
+                out.zero_()
+            torch.cuda.synchronize()
+            for (graph, _), stream in zip(graphs, streams):
+                with torch.cuda.stream(stream if at_once else torch.cuda.current_stream()):
+                    graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(out, w) for (_, out), w in zip(graphs, want))
+
+
+@pytest.mark.parametrize("dtype,H,K,D,lengths", SHARED)
+def test_sharing_form_on_two_streams_at_once(cuda, dtype, H, K, D, lengths):
+    steps = [_sharing_step(cuda, dtype, H, K, D, lengths, seed) for seed in (1, 5)]
+    want = [run() for _, run, _ in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(10):
+        for i, (stream, (_, run, _)) in enumerate(zip(streams, steps)):
+            with torch.cuda.stream(stream):
+                outs.append((i, run()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in outs)
+
+
+@pytest.mark.parametrize("dtype,H,K,D,lengths", SHARED)
+def test_sharing_form_with_a_page_outside_the_pool(cuda, dtype, H, K, D, lengths):
+    """A bad page in the middle of a sequence makes that one NaN and no other."""
+    kp, vp, table = _cache(lengths, 16, K, D, dtype, cuda)
+    q, n = _rand((len(lengths), H, D), dtype, 8, cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    assert _workspace_of(q, K, table, D, dtype, H) > 0
+    want = zg.paged_attention(q, kp, vp, table, n)
+    at = max(range(len(lengths)), key=lambda b: lengths[b])
+    for page, bad in ((0, -1), (lengths[at] // 32, kp.shape[0]), ((lengths[at] - 1) // 16, 2 ** 31 - 1)):
+        broken = table.clone()
+        broken[at, page] = bad
+        o = zg.paged_attention(q, kp, vp, broken, n)
+        assert torch.isnan(o[at]).all()
+        rest = torch.arange(len(lengths), device=cuda) != at
+        assert torch.equal(o[rest], want[rest])
+    for length in (-1, table.shape[1] * 16 + 1):
+        m = n.clone()
+        m[at] = length
+        o = zg.paged_attention(q, kp, vp, table, m)
+        assert torch.isnan(o[at]).all() and torch.equal(o[rest], want[rest])

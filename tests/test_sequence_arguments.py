@@ -76,3 +76,11 @@ def test_paged_attention_copies_queries_for_the_tensor_cores_alone(calls, monkey
         _sequence.paged_attention(q, pool, pool, table, n)
         (_, args), = calls
         assert (args[0] != q.data_ptr()) == copied and args[1] == (D if copied else q.stride(0)), (dtype, D)
+
+
+def test_window_attention_of_more_heads_than_a_grid_counts():
+    """Sequences times heads beyond 31 bits are refused before their product with the tiles wraps."""
+    for Z, S, H, K, D in ((2 ** 31 - 1, 2 ** 30, 2 ** 30, 1, 4), (2 ** 30, 256, 8, 8, 64)):
+        assert L.load().zg_window_attention(None, H * D, None, K * D, None, K * D, None, Z, S, H, K, D, 0, 0, L.ZG_BF16, None,
+                                            None) == L.ZG_ERR_INVALID
+        assert b"bad sizes" in L.load().zg_last_error()

@@ -1391,7 +1391,7 @@ int window_error_word(int clear) { return ptx_error_word(clear); }
 extern "C" int zg_window_attention(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                                    const int32_t* lengths, int64_t Z, int64_t S, int H, int K, int D, int window,
                                    int sinks, int dtype, void* o, void* stream) {
-    if (Z < 0 || S < 0 || Z > INT32_MAX || S > (1 << 30) || H < 1 || K < 1 || H % K || D < 1)
+    if (Z < 0 || S < 0 || Z > INT32_MAX || S > (1 << 30) || H < 1 || K < 1 || H % K || D < 1 || Z > INT32_MAX / H)
         return zg::fail(ZG_ERR_INVALID, "zg_window_attention: bad sizes");
     if (D > 256) return zg::fail(ZG_ERR_UNSUPPORTED, "zg_window_attention: head dim above 256");
     if (window < 0 || sinks < 0)

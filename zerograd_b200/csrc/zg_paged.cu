@@ -121,7 +121,7 @@ struct PagedArgs {
     const void *q, *kp, *vp;
     const int32_t *table, *lengths;
     void* o;
-    float* part;  // share > 0: of each unit, chunk and warp, P rows of sums, then m [P], l [P]
+    float* part;  // of each unit, chunk and warp, P rows of sums, then m [P], l [P]; null where blocks join by themselves
     int64_t ldq, n_pages;
     // R: query rows of a unit (heads that share a key head), P: those that there are
     int page, max_pages, B, H, K, D, G, row_tiles, R, P;
@@ -155,7 +155,7 @@ constexpr int PG_CHUNK = 128;  // positions of a chunk at least: less would be t
 // Positions of a chunk of `vis`, a multiple of 64.  Above the eight chunks of
 // a cluster those of the tensor-core kernel are twice as long at least, as
 // each costs a whole unit's warps their fold: 64 sequences of 1000 to 4000 take
-// 83.7 us with 256, 88 with 128 (and 79.5 cut not at all); one of 8000 over 12
+// 84.7 us with 256, 89 with 128 (and 79.5 cut not at all); one of 8000 over 12
 // heads 11.8, with 512 14.9.  (float32's products take longer for the same
 // bytes: 2 sequences of 9000, 10 heads of one key head, 22 us with 128, 28 with 256.)
 __device__ __forceinline__ int chunk_of(const PagedArgs& a, int vis) {
@@ -245,7 +245,7 @@ struct Work {
     }
 };
 // (SHARE, with leaves in the workspace, is an instance of its own: with both
-// in one, 64 sequences took 80.1 us instead of 77.9.)
+// in one, 64 sequences took 80.1 us instead of 77.9 before there were leaves.)
 template <bool SHARE>
 __device__ __forceinline__ Work work_of(const PagedArgs& a) {
     Work w;
@@ -322,6 +322,7 @@ __device__ __forceinline__ float cluster_float(const float* p, int rank) {
     return v;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();  // the barrier below is a converged warp's
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -360,7 +361,7 @@ struct Warps {
     }
 };
 
-// The leaf of this warp in chunk c: where its sums go in the workspace.
+// The leaf of this warp in chunk c (its maximum, sum and outputs): where it goes in the workspace.
 __device__ __forceinline__ float* leaf_of(const PagedArgs& a, const Work& w, int c) {
     return a.part + ((((int64_t)w.b * a.K + w.kh) * a.row_tiles + w.rt) * a.most * PG_WARPS + c * PG_WARPS + threadIdx.x / 32) *
                         part_floats(a.P, a.D);

@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(WF_THREADS, DP <= 96 ? 3 : DP <= 128 ? 2 : 1) 
     // zeros in such places, and notes the tiles.
     __shared__ int tiles[WIN_BAD];
     int found = 0;
-    // (Two instances: with the test in one, 3 x 777 tokens of 8 heads of 80 took 55.0 us instead of 51.7.)
+    // (Two instances: with the test in one, 3 x 777 tokens of 8 heads of 80 took 55.0 us instead of 51.3.)
     auto pass = [&](auto second) {
         constexpr bool CLEAN = decltype(second)::value;
 #pragma unroll
@@ -488,7 +488,7 @@ int launch_window_any(const WindowArgs& a, cudaStream_t st) {
 // What bounds it is a group's exponentials, 16 a clock and SM, and the waits
 // around them; the MMAs take about half as long.  2 x 4096 tokens of 12 heads
 // (4 key heads) of 64, causal: 82 us, 0.62 PFLOP/s of the visible pairs; 8192
-// tokens of 16 heads (4) of 128 under a window of 1024: 87 us, 0.74 PFLOP/s.
+// tokens of 16 heads (4) of 128 under a window of 1024: 85 us, 0.76 PFLOP/s.
 //
 // The maximum m that weights are taken against is moved, and O rescaled by
 // its group, only when a row's true maximum is more than 2^8 above it: the

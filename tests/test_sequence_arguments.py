@@ -54,10 +54,11 @@ def test_sizes_beyond_32_bits_are_refused(calls):
     assert not calls
 
 
-def test_negated_views_and_zero_tensors_take_the_dispatcher():
-    """A tensor whose memory does not hold its values is not read as it lies there."""
+def test_negated_views_take_the_dispatcher():
+    """A tensor whose memory does not hold its values is not read as it lies
+    there, nor in a vmap rule one without memory."""
     x = torch.ones(2, 3)
-    assert not _sequence._plain_call(x, torch._neg_view(x)) and not _sequence._plain_call(torch._efficientzerotensor((2,)))
+    assert _sequence._plain_call(x) and not _sequence._plain_call(x, torch._neg_view(x))
     m = _sequence._mapped(torch._neg_view(x), 1)
     assert not m.is_neg() and m.tolist() == [[-1.0, -1.0]] * 3
     m = _sequence._mapped(torch._efficientzerotensor((2,)), None, 4)

@@ -44,9 +44,10 @@ _empty, _CONTIGUOUS = torch.empty_like, torch.contiguous_format
 
 def _plain_call(*ts) -> bool:
     """True when a call needs none of what the dispatcher adds (vmap, an
-    autograd error, a tracing mode, the values of a negated view or of a zero
-    tensor without memory): the op is then launched without it, which a single
-    token's call notices (about 20 us of host time)."""
+    autograd error, a tracing mode, the values of a negated view): the op is
+    then launched without it, which a single token's call notices (about 20 us
+    of host time).  (A zero tensor, which has no memory, is refused by the entry
+    points as a null pointer: asking costs a tenth of a microsecond a tensor.)"""
     if not _ask or _transform() is not None or _modes() or _tracing() is not None or _compiling():
         return False
     grad = _grad_enabled()
@@ -54,7 +55,7 @@ def _plain_call(*ts) -> bool:
         if type(t) is not _Tensor:
             if t is not None:
                 return False
-        elif (grad and t.requires_grad) or t.is_neg() or t._is_zerotensor():
+        elif (grad and t.requires_grad) or t.is_neg():
             return False
     return True
 
@@ -89,11 +90,10 @@ def _call(dev: torch.device, name: str, *args) -> None:
             L.call(name, *args, L.stream_ptr(dev))
 
 
-def _narrow(*sizes: int) -> None:
-    """Refuses sizes that the entry points would get without their upper bits
-    (ctypes cuts an int to its 32 bits)."""
-    if max(sizes) > _INT_MAX:
-        raise ValueError(f"a size of {max(sizes)}: heads, head width, page size and table width are at most 2^31 - 1")
+def _too_wide(*sizes: int) -> ValueError:
+    """Sizes above _INT_MAX, which the entry points would get without their
+    upper bits (ctypes cuts an int to its 32 bits)."""
+    return ValueError(f"a size of {max(sizes)}: heads, head width, page size and table width are at most 2^31 - 1")
 
 
 def _int32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -165,7 +165,8 @@ def launch_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, axe
         L.dtype_code(k.dtype)
         rest = (positions, axes, base, interleaved, joint, inverse)
         return launch_rotary(q, q[..., :0, :], *rest)[0], launch_rotary(k[..., :0, :], k, *rest)[1]
-    _narrow(qs[-2], ks[-2], qs[-1])
+    if qs[-2] > _INT_MAX or ks[-2] > _INT_MAX or qs[-1] > _INT_MAX:
+        raise _too_wide(qs[-2], ks[-2], qs[-1])
     (q, ldq), (k, ldk) = _pitched(q), _pitched(k)
     positions = positions.contiguous()
     qo, ko = _empty(q, memory_format=_CONTIGUOUS), _empty(k, memory_format=_CONTIGUOUS)
@@ -242,7 +243,8 @@ def launch_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     K = ks[-2]
     if K < 1 or H % K:
         raise ValueError(f"{H} query heads are not a multiple of {K} key heads")
-    _narrow(H, D)
+    if H > _INT_MAX or D > _INT_MAX:
+        raise _too_wide(H, D)
     if lengths is not None:
         if lengths.shape != lead:
             raise ValueError(f"lengths of shape {tuple(lengths.shape)} do not match the sequences {tuple(lead)}")
@@ -302,7 +304,8 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> torch.Size:
         raise ValueError("key and value pages must be contiguous")
     if shape[1] < 1 or shape[2] < 1 or shape[3] < 1:
         raise ValueError(f"pages of shape {tuple(shape)} hold nothing")
-    _narrow(*shape[1:])
+    if shape[1] > _INT_MAX or shape[2] > _INT_MAX or shape[3] > _INT_MAX:
+        raise _too_wide(*shape[1:])
     return shape
 
 
@@ -310,7 +313,8 @@ def _table(page_table: torch.Tensor, lengths: torch.Tensor, lead: torch.Size) ->
     if page_table.ndim < 1 or page_table.shape[:-1] != lead or lengths.shape != lead:
         raise ValueError(f"a page table of shape {tuple(page_table.shape)} and lengths {tuple(lengths.shape)} do not "
                          f"match the sequences {tuple(lead)}")
-    _narrow(page_table.shape[-1])
+    if page_table.shape[-1] > _INT_MAX:
+        raise _too_wide(page_table.shape[-1])
     return _int32(page_table, "the page table"), _int32(lengths, "lengths")
 
 
@@ -406,7 +410,8 @@ def launch_paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if q.dtype is not dt:
         raise TypeError(f"q must have the pages' type {dt}, got {q.dtype}")
     lead, H = qs[:-2], qs[-2]
-    _narrow(H)
+    if H > _INT_MAX:
+        raise _too_wide(H)
     table, had = _table(page_table, lengths, lead)
     B, M = math.prod(lead), table.shape[-1]
     code = L.dtype_code(dt)

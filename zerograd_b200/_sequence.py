@@ -282,12 +282,13 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     [...] (int32 or int64): the tokens of each sequence of a padded batch;
     rows behind a sequence's length are zeros, whatever their inputs hold,
     and a length outside [0, S] gives NaN rows.  D is at most 256; float32 or
-    bf16.
+    bf16, q's type (k and v are taken in it).
 
     bf16 with D up to 128, a multiple of 8, runs on the tensor cores (scores
     and sums in float32, weights rounded to bf16), other shapes and float32
-    on the FMA pipe.  q, k and v may be views of one fused projection; the
-    output is contiguous."""
+    on the FMA pipe.  Keys and values that a row does not see do not reach it,
+    infinities and NaN included.  q, k and v may be views of one fused
+    projection; the output is contiguous."""
     w, s = _span(window, sinks)
     args = (q, k, v, lengths, w, s)
     return launch_window_attention(*args) if _plain_call(q, k, v, lengths) else _window_op(*args)

@@ -155,8 +155,8 @@ constexpr int PG_CHUNK = 128;  // positions of a chunk at least: less would be t
 // Positions of a chunk of `vis`, a multiple of 64.  Above the eight chunks of
 // a cluster those of the tensor-core kernel are twice as long at least, as
 // each costs a whole unit's warps their fold: 64 sequences of 1000 to 4000 take
-// 84.7 us with 256, 89 with 128 (and 79.5 cut not at all); one of 8000 over 12
-// heads 11.8, with 512 14.9.  (float32's products take longer for the same
+// 83 us with 256, 86 with 128 (and 81 cut not at all); one of 8000 over 12
+// heads 11.5, with 512 14.9.  (float32's products take longer for the same
 // bytes: 2 sequences of 9000, 10 heads of one key head, 22 us with 128, 28 with 256.)
 __device__ __forceinline__ int chunk_of(const PagedArgs& a, int vis) {
     const int even = (vis + a.each - 1) / a.each, least = vis <= 8 * PG_CHUNK ? PG_CHUNK : a.least;
@@ -455,8 +455,11 @@ __device__ __forceinline__ void join_warps(const PagedArgs& a, const float* ms, 
 // meet once, at the end.  The products are a small part of the time the
 // bytes take: 16 rows of which G are used cost nothing that matters, and a
 // larger tile of the tensor cores of this chip would have to wait for 128
-// positions where a warp goes on after 16.
-template <int DP, int STAGES, bool SHARE>
+// positions where a warp goes on after 16.  What costs is the instructions
+// around them: with up to 8 heads (TALL not set) a lane's second row is none,
+// and has no weights, sums or folds (64 sequences of 1000 to
+// 4000: 84.7 -> 83.1 us; 250 of up to 250: 43 -> 39; 64 of up to 2000 at D = 256: 89 -> 80).
+template <int DP, int STAGES, bool SHARE, bool TALL>
 __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArgs a) {
     using T = __nv_bfloat16;
     constexpr int CPR = DP / 8;             // 16-byte chunks of a row
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = lane / 4 + (e & 1) * 8, d = k * 16 + (lane % 4) * 2 + (e >> 1) * 8;
-                qf[k][e] = r < rows && d < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)r * a.D + d) : 0u;
+                qf[k][e] = (TALL || e % 2 == 0) && r < rows && d < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)r * a.D + d) : 0u;
             }
     }
     float o[DP / 8][4];
@@ -532,7 +535,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
     const int v_row = (lane % 8) + 8 * ((lane / 8) % 2), v_chunk = lane / 16;
     // The chunks before this one.  With DP = 256 in shared memory: behind the
     // ring of three stages there is room for 8 rows, behind one of two for 16.
-    constexpr int ROWS = DP == 256 && STAGES == 3 ? 8 : 16;
+    static_assert(DP < 256 || SHARE || TALL == (STAGES == 2), "room for the chunks before");
+    constexpr int ROWS = TALL ? 16 : 8;
     float M[2] = {-INFINITY, -INFINITY}, L[2] = {0.f, 0.f};
     float kept[DP == 256 ? 1 : DP / 8][4];
     float* kept_far = reinterpret_cast<float*>(smem + PG_WARPS * STAGES * 2 * TILE) + warp * ROWS * DP + lane;
@@ -575,7 +579,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < ROWS / 4; ++e) {
                     s[j][e] = t0 + j * 8 + (lane % 4) * 2 + (e & 1) < end ? __fmul_rn(s[j][e], a.scale) : -INFINITY;
                     if (e < 2) n0 = fmaxf(n0, s[j][e]);
                     else n1 = fmaxf(n1, s[j][e]);
@@ -583,7 +587,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 #pragma unroll
             for (int x = 1; x < 4; x <<= 1) {
                 n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, x));
-                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
+                if (TALL) n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, x));
             }
             n0 = fmaxf(n0, m0);
             n1 = fmaxf(n1, m1);
@@ -597,8 +601,10 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
                 for (int d = 0; d < DP / 8; ++d) {
                     o[d][0] *= f0;
                     o[d][1] *= f0;
-                    o[d][2] *= f1;
-                    o[d][3] *= f1;
+                    if (TALL) {
+                        o[d][2] *= f1;
+                        o[d][3] *= f1;
+                    }
                 }
                 m0 = n0;
                 m1 = n1;
@@ -609,11 +615,14 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float p0 = exp2_fast(s[j][0] - b0l), p1 = exp2_fast(s[j][1] - b0l);
-                const float p2 = exp2_fast(s[j][2] - b1l), p3 = exp2_fast(s[j][3] - b1l);
                 l0 += p0 + p1;
-                l1 += p2 + p3;
                 p[2 * j] = pack_bf16(p0, p1);
-                p[2 * j + 1] = pack_bf16(p2, p3);
+                p[2 * j + 1] = 0u;
+                if (TALL) {
+                    const float p2 = exp2_fast(s[j][2] - b1l), p3 = exp2_fast(s[j][3] - b1l);
+                    l1 += p2 + p3;
+                    p[2 * j + 1] = pack_bf16(p2, p3);
+                }
             }
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) {
@@ -627,14 +636,14 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
 #pragma unroll
         for (int x = 1; x < 4; x <<= 1) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, x);
-            l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+            if (TALL) l1 += __shfl_xor_sync(0xffffffffu, l1, x);
         }
         if constexpr (SHARE) {
             if (__any_sync(0xffffffffu, bad)) l0 = l1 = __int_as_float(0x7fffffff);
             float* leaf = leaf_of(a, w, c);
             const int pitch = pad4(a.D);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < ROWS / 8; ++e) {
                 const int r = lane / 4 + 8 * e;
                 if (r >= rows) continue;
 #pragma unroll
@@ -647,18 +656,19 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
                 }
             }
         } else {
-            const Fold f0(M[0], L[0], m0, l0), f1(M[1], L[1], m1, l1);
 #pragma unroll
-            for (int d = 0; d < DP / 8; ++d) {
+            for (int r = 0; r < ROWS / 8; ++r) {
+                const Fold fold(M[r], L[r], r ? m1 : m0, r ? l1 : l0);
 #pragma unroll
-                for (int e = 0; e < ROWS / 4; ++e) {
-                    float& x = so_far(d, e);
-                    x = (e < 2 ? f0 : f1)(x, o[d][e]);
-                }
+                for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+                    for (int e = 2 * r; e < 2 * r + 2; ++e) so_far(d, e) = fold(so_far(d, e), o[d][e]);
             }
         }
 #pragma unroll
-        for (int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < ROWS / 4; ++e) o[d][e] = 0.f;
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.f;
     }
@@ -669,15 +679,17 @@ __global__ void __launch_bounds__(PG_WARPS * 32) paged_mma_kernel(const PagedArg
         const int r = lane / 4;
         if (lane % 4 == 0) {
             ms[warp * 16 + r] = M[0];
-            ms[warp * 16 + r + 8] = M[1];
             ls[warp * 16 + r] = bad ? __int_as_float(0x7fffffff) : L[0];
-            ls[warp * 16 + r + 8] = bad ? __int_as_float(0x7fffffff) : L[1];
+            if (TALL) {
+                ms[warp * 16 + r + 8] = M[1];
+                ls[warp * 16 + r + 8] = bad ? __int_as_float(0x7fffffff) : L[1];
+            }
         }
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d) {
             float* to = os + (warp * 16 + r) * DP + d * 8 + (lane % 4) * 2;
             *reinterpret_cast<float2*>(to) = make_float2(so_far(d, 0), so_far(d, 1));
-            if (ROWS > 8) *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(so_far(d, 2), so_far(d, 3));
+            if (TALL) *reinterpret_cast<float2*>(to + 8 * DP) = make_float2(so_far(d, 2), so_far(d, 3));
         }
         __syncthreads();
         join_warps<T>(a, ms, ls, os, DP, os + PG_WARPS * 16 * DP, w, rows, h0, see.vis);
@@ -1068,14 +1080,20 @@ int launch_split(void (*f)(P...), const PagedArgs& a, int64_t blocks, size_t sme
     return zg::check_launch("zg_paged_attention");
 }
 
-template <int DP, int STAGES>
+// STAGES of the ring, OWN of those of a kernel that keeps its chunks' sums.
+template <int DP, int STAGES, int OWN, bool TALL>
 int launch_mma(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
-    const size_t smem = (size_t)PG_WARPS * STAGES * 2 * 16 * DP * 2  +
-                        (DP == 256 && !a.part ? PG_WARPS * (STAGES == 3 ? 8 : 16) * DP * sizeof(float) : 0);
-    const auto f = a.part ? paged_mma_kernel<DP, STAGES, true> : paged_mma_kernel<DP, STAGES, false>;
+    const size_t smem = (size_t)PG_WARPS * (a.part ? STAGES : OWN) * 2 * 16 * DP * 2 +
+                        (DP == 256 && !a.part ? PG_WARPS * (TALL ? 16 : 8) * DP * sizeof(float) : 0);
+    const auto f = a.part ? paged_mma_kernel<DP, STAGES, true, TALL> : paged_mma_kernel<DP, OWN, false, TALL>;
     if (int rc = set_smem(f, smem)) return rc;
     zg::LaunchTimer zg_lt_("paged_attention", st);
     return launch_split(f, a, blocks, smem, st, a);
+}
+template <bool TALL>
+int launch_mma_any(const PagedArgs& a, int64_t blocks, cudaStream_t st) {
+    return a.D <= 64    ? launch_mma<64, 4, 4, TALL>(a, blocks, st)
+           : a.D <= 128 ? launch_mma<128, 3, 3, TALL>(a, blocks, st) : launch_mma<256, 3, TALL ? 2 : 3, TALL>(a, blocks, st);
 }
 
 template <typename T, int PARTS, int GT>
@@ -1179,9 +1197,7 @@ extern "C" int zg_paged_attention(const void* q, int64_t ldq, const void* k_page
     cudaStream_t st = zg::as_stream(stream);
     int rc;
     if (p.mma && vec && ldq % 2 == 0 && (reinterpret_cast<uintptr_t>(q) & 3) == 0) {
-        rc = D <= 64 ? launch_mma<64, 4>(a, blocks, st)
-             : D <= 128 ? launch_mma<128, 3>(a, blocks, st)
-             : p.P <= 8 || p.leaves ? launch_mma<256, 3>(a, blocks, st) : launch_mma<256, 2>(a, blocks, st);
+        rc = p.P > 8 ? launch_mma_any<true>(a, blocks, st) : launch_mma_any<false>(a, blocks, st);
     } else if (p.mma) {
         return zg::fail(ZG_ERR_INVALID, "zg_paged_attention: bf16 pages with D a multiple of 8 must be 16-byte "
                                         "aligned, q 4-byte aligned with an even pitch");
